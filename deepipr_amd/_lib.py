@@ -73,6 +73,10 @@ SIGNATURES = {
     'deepipr_sgd_momentum_step_dev': (_int, [_f32p, _f32p, _f32p, _sz, _f32p, _vp]),
     'deepipr_sgd_momentum_chunk': (_int, []),
     'deepipr_sgd_momentum_step_multi': (_int, [_f32p, _f32p, _vp, _int, _sz, _f32p, _vp]),
+    'deepipr_grad_norm_workspace_bytes': (_sz, []),
+    'deepipr_grad_norm': (_int, [_vp, _int, _int, _f32p, _vp, _sz, _vp]),
+    'deepipr_grad_clip': (_int, [_vp, _int, _int, _flt, _f32p, _vp, _sz, _vp]),
+    'deepipr_sgd_momentum_step_clipped': (_int, [_f32p, _f32p, _vp, _int, _f32p, _f32p, _vp, _sz, _vp]),
     'deepipr_passport_bn_workspace_bytes': (_sz, [_int, _int, _int]),
     'deepipr_passport_bn_fwd': (_int, [_f32p, _f32p, _f64p, _f32p, _f32p, _f32p, _flt, _flt, _flt, _f32p, _f32p, _vp,
                                        _flt, _flt, _int, _int, _int, _int, _int, _int, _f32p, _f32p, _f32p, _f32p,
@@ -126,11 +130,12 @@ TEST_HOOK_SIGNATURES = {
     'deepipr_debug_trace': (_int, [_vp]),
     'deepipr_debug_wino_trace': (_int, [_vp]),
 }
-ABI_VERSION = 12
+ABI_VERSION = 13
 SYNC_WORDS = 2 * (256 * 30 * 4 + 4096 + 63 * 2048) + 16     # DEEPIPR_SYNC_WORDS
 SYNC_TIMEOUT_WORD = 2 * (256 * 30 * 4 + 4096 + 63 * 2048)   # DEEPIPR_SYNC_TIMEOUT_WORD
 
 
+F32, BF16, F16 = 0, 1, 2                # DEEPIPR_F32 / _BF16 / _F16
 GEMV_MAX_LAYERS = 16                    # DEEPIPR_GEMV_MAX_LAYERS
 
 
@@ -198,7 +203,8 @@ PROFILE_KERNELS = ['pooled_patch_mean', 'gamma_beta_fwd', 'gamma_beta_bwd', 'aff
                    'reduce_partials', 'passport_bwd_finish', 'sign_loss_fwd', 'sign_loss_bwd', 'dkey', 'reserved',
                    'bn_stats', 'bn_affine_fwd', 'bn_bwd_reduce', 'bn_affine_bwd', 'sgd', 'add_relu', 'bn_res_fwd',
                    'bn_res_bwd', 'gn_fwd', 'gn_bwd', 'conv_wgrad', 'conv_wgrad_reduce', 'conv_fwd', 'conv_dgrad', 'conv_wgrad_b3', 'conv_split_sum',
-                   'conv_wino_fwd', 'conv_wino_dgrad', 'conv_wino_wgrad', 'conv_wino_weights', 'conv1x1_wgrad', 'maxpool', 'resample2', 'conv1x1_fwd', 'conv1x1_dgrad', 'head']
+                   'conv_wino_fwd', 'conv_wino_dgrad', 'conv_wino_wgrad', 'conv_wino_weights', 'conv1x1_wgrad', 'maxpool', 'resample2', 'conv1x1_fwd', 'conv1x1_dgrad', 'head',
+                   'grad_norm', 'grad_clip']
 
 
 class ExternalEvent:

@@ -36,6 +36,7 @@
 
 #include "../../include/deepipr_hip.h"
 #include "deepipr_conv_plan.h"
+#include "deepipr_host.h"
 
 namespace {
 
@@ -111,6 +112,7 @@ struct ProfScope {
         b = take();
         if (!a || !b) a = b = nullptr;
     }
+    ProfScope(int kernel, hipEvent_t start, hipEvent_t stop) : k(kernel), a(start), b(stop) {}
     ~ProfScope() {
         if (!a) return;
         std::lock_guard<std::mutex> lk(g_prof.mu);
@@ -3080,6 +3082,29 @@ int launch_passport_finish(const double *part, int NS, int C, const float *gamma
 bool bad_dims(int N, int C, int HW) { return N <= 0 || C <= 0 || HW <= 0; }
 
 }  // namespace
+
+// ---------------------------------------------------------------------------------------------
+// Host plumbing for the other translation units (deepipr_host.h)
+int dipr_fail(int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+int dipr_check_launch(const char *what) { return check_launch(what); }
+DiprProf::DiprProf(int kernel) : k(kernel) {
+    ProfScope taken(kernel, nullptr);
+    a = taken.a;
+    b = taken.b;
+    taken.a = nullptr;                    // this object hands the pair back
+}
+DiprProf::~DiprProf() {
+    if (!a) return;
+    ProfScope give(k, a, b);
+    give.used = used;
+    give.bytes = bytes;
+}
 
 // =============================================================================================
 // C ABI

@@ -30,7 +30,13 @@ _ALIGN = 64            # floats: every parameter starts on a 256-byte boundary o
 
 class FlatSGD(torch.optim.Optimizer):
     def __init__(self, params, lr=0.01, momentum=0.9, weight_decay=1e-4, bucket_fractions=(0.45, 0.8, 0.95),
-                 process_group=None):
+                 process_group=None, max_grad_norm=None):
+        """max_grad_norm: the step uses the gradients scaled by min(1, max_grad_norm / (norm + 1e-6)), the norm that of the averaged
+        gradients of ALL parameters (torch.nn.utils.clip_grad_norm_'s rule); the gradients themselves stay as they are and
+        `grad_norm` (0-d, on the device) holds the norm of the last step.  None: no norm is computed.  The value can be changed
+        between steps (`opt.max_grad_norm = 0.5`), captured ones included; switching it on or off after a capture cannot follow."""
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise ValueError('max_grad_norm must not be negative or NaN (got %r)' % (max_grad_norm,))
         # like torch.optim.SGD, frozen parameters (requires_grad=False) are never touched: they stay out of the
         # flat buffers altogether (no weight decay, no momentum, no exchange)
         params = [p for p in params if p.requires_grad]
@@ -71,7 +77,11 @@ class FlatSGD(torch.optim.Optimizer):
         # captured into a hipGraph (launch arguments frozen at capture) then still follows an lr schedule --
         # sync_hyper() rewrites the four floats whenever param_groups changed (GraphedTrainStep calls it before
         # every replay; step() calls it when it runs eagerly).
-        self._hyper = torch.zeros(4, dtype=torch.float32, device=dev)
+        # With clipping {.., max_grad_norm} is the fifth.
+        self.max_grad_norm = max_grad_norm
+        self._clips = max_grad_norm is not None
+        self.grad_norm = torch.zeros((), dtype=torch.float32, device=dev) if self._clips else None
+        self._hyper = torch.zeros(5 if self._clips else 4, dtype=torch.float32, device=dev)
         self._hyper_host = None
         # chunk table of the in-place update (_step_in_place): pinned host rows + their device copy, allocated here
         # because nothing may be allocated on the host side while a stream is being captured
@@ -79,7 +89,7 @@ class FlatSGD(torch.optim.Optimizer):
         self._table_ready = None          # the pair prepare_in_place_capture() made for the next capture
         self.in_place_captures = 0
         self._tab_rows = 0
-        if dev.type == 'cuda' and not self.comm and hasattr(P.kernels, 'sgd_chunk'):
+        if dev.type == 'cuda' and not self.comm and not self._clips and hasattr(P.kernels, 'sgd_chunk'):
             chunk = P.kernels.sgd_chunk()
             self._tab_rows = sum((p.numel() + chunk - 1) // chunk for p in plist)
             self.prepare_in_place_capture()
@@ -291,6 +301,13 @@ class FlatSGD(torch.optim.Optimizer):
         capture / replay (it is a host-to-device copy of four floats on the current stream)."""
         g = self.param_groups[0]
         host = (float(g['lr']), float(g['momentum']), float(g['weight_decay']), 1.0 / self.world)
+        if (self.max_grad_norm is not None) != self._clips:
+            raise RuntimeError('FlatSGD: clipping is chosen when the optimiser is built (max_grad_norm=...); later only its value can '
+                               'change')
+        if self._clips:
+            if not float(self.max_grad_norm) >= 0.0:
+                raise ValueError('max_grad_norm must not be negative or NaN (got %r)' % (self.max_grad_norm,))
+            host += (float(self.max_grad_norm),)
         if host != self._hyper_host:
             self._hyper.copy_(torch.tensor(host, dtype=torch.float32), non_blocking=False)
             self._hyper_host = host
@@ -310,7 +327,9 @@ class FlatSGD(torch.optim.Optimizer):
         elif self._hyper_host is None:
             raise RuntimeError('FlatSGD: call sync_hyper() once before capturing step() into a hipGraph')
         missing = self._missing_grads()
-        if capturing and not self.comm and not missing and self._step_in_place():
+        if self._clips and not self.comm and self._step_clipped_in_place():
+            return loss
+        if capturing and not self.comm and not missing and not self._clips and self._step_in_place():
             return loss                                   # gradients read where autograd left them: no packing pass
         # The collective layout follows the MODE, which the driver of the step sets identically on every rank -- never
         # rank-local state such as which hooks happened to fire (ranks issuing different sets of collectives hang).
@@ -341,7 +360,17 @@ class FlatSGD(torch.optim.Optimizer):
                     self._launch(b, async_op=False)
             for w in self._works:
                 w.wait()
-        if not missing:
+        if self._clips:
+            # the same rule for every rank: norm and factor come from the exchanged sum (parameters without a gradient stay out)
+            skip = set(missing)
+            have = [(self.flat_grad[off:off + p.numel()], off) for i, (p, off) in enumerate(self._slots) if i not in skip] \
+                if missing else [(self.flat_grad, 0)]
+            if have:
+                P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, [g for g, _ in have], [o for _, o in have],
+                                                    self._hyper, self.grad_norm)
+            else:
+                self.grad_norm.zero_()
+        elif not missing:
             P.kernels.sgd_momentum_step_dev(self.flat_param, self.flat_grad, self.flat_buf, self._hyper)
         else:
             # torch.optim.SGD skips parameters whose grad is None (no weight decay, no momentum update): update the
@@ -402,6 +431,28 @@ class FlatSGD(torch.optim.Optimizer):
         table.copy_(tab_host[:len(rows)], non_blocking=True)         # a memcpy node: replays re-read the pinned rows
         P.kernels.sgd_momentum_step_multi(self.flat_param, self.flat_buf, table, total, self._hyper)
         self.in_place_captures += 1
+        self._works = []
+        self._launched = [False] * len(self._buckets)
+        self._pending = [hi - lo for lo, hi in self._buckets]
+        return True
+
+    def _step_clipped_in_place(self):
+        """One GPU, clipping: norm and update read the gradients where autograd left them (their addresses travel in the launch
+        arguments), eager and captured alike; parameters without a gradient are left alone.  -> False if a gradient cannot be
+        addressed that way (the packed path is taken then)."""
+        grads, offsets = [], []
+        for p, off in self._slots:
+            g = p.grad
+            if g is None:
+                continue
+            if g.dtype != torch.float32 or g.device != self.flat_param.device or not g.is_contiguous():
+                return False
+            grads.append(g)
+            offsets.append(off)
+        if grads:
+            P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, grads, offsets, self._hyper, self.grad_norm)
+        else:
+            self.grad_norm.zero_()
         self._works = []
         self._launched = [False] * len(self._buckets)
         self._pending = [hi - lo for lo, hi in self._buckets]

@@ -16,6 +16,7 @@ import os
 import threading
 import weakref
 
+import numpy as np
 import torch
 import torch.utils.weak
 
@@ -937,6 +938,81 @@ class HipKernels:
             _lib.check(_lib.lib().deepipr_sgd_momentum_step_dev(_p(flat_param), _p(flat_grad), _p(flat_buf),
                                                                flat_param.numel(), _p(hyper), _stream(dev)),
                        'sgd_momentum_step_dev')
+
+    # ---- global norm of a list of tensors, clipping, the step behind it (include/deepipr_hip.h: deepipr_grad_*) ----
+    _DTYPE_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+    @staticmethod
+    def _dense(t):
+        """Every element of t's storage range belongs to exactly one element of t, whatever the order of its dimensions."""
+        if t.is_contiguous():
+            return True
+        span = 1
+        for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+            if stride != span:
+                return False
+            span *= size
+        return True
+
+    def _tensor_list(self, what, tensors, offsets=None):
+        """-> (device, host rows {address, elements, offset, type} as include/deepipr_hip.h: DeepiprTensor has them)."""
+        rows = np.zeros((len(tensors), 4), dtype=np.int64)
+        if not tensors:
+            raise RuntimeError('%s: an empty list of tensors' % what)
+        devs = set(map(torch.Tensor.get_device, tensors))
+        if len(devs) != 1 or -1 in devs:
+            raise RuntimeError('deepipr_amd %s runs on the GPU only, all tensors on one device (got %s); there is no CPU fallback'
+                               % (what, sorted({str(t.device) for t in tensors})))
+        try:
+            rows[:, 3] = [self._DTYPE_CODE[t.dtype] for t in tensors]
+        except KeyError as e:
+            raise RuntimeError('deepipr_amd %s takes float32, bfloat16 and float16 tensors (got %s)' % (what, e)) from None
+        if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(map(self._dense, tensors)):
+            raise RuntimeError('deepipr_amd %s needs dense tensors (no gaps, no element twice)' % what)
+        rows[:, 0] = list(map(torch.Tensor.data_ptr, tensors))
+        rows[:, 1] = list(map(torch.Tensor.numel, tensors))
+        if offsets is not None:
+            rows[:, 2] = offsets
+        return tensors[0].device, rows
+
+    def _norm_scratch(self, dev):
+        n = _lib.lib().deepipr_grad_norm_workspace_bytes()
+        return torch.empty(n, dtype=torch.uint8, device=dev), n
+
+    def grad_norm(self, tensors, norm_type):
+        """-> 0-d float32 norm over all elements of the list; norm_type 1, 2, or 0 for the largest magnitude."""
+        dev, rows = self._tensor_list('grad_norm', tensors)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        with _on(dev):
+            ws, nbytes = self._norm_scratch(dev)
+            _lib.check(_lib.lib().deepipr_grad_norm(rows.ctypes.data, len(rows), norm_type, norm.data_ptr(), ws.data_ptr(), nbytes,
+                                                    _stream(dev)), 'grad_norm')
+        return norm
+
+    def grad_clip(self, tensors, max_norm, norm_type):
+        """Scales the list in place by min(1, max_norm / (norm + 1e-6)); -> the norm before."""
+        dev, rows = self._tensor_list('grad_clip', tensors)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        with _on(dev):
+            ws, nbytes = self._norm_scratch(dev)
+            _lib.check(_lib.lib().deepipr_grad_clip(rows.ctypes.data, len(rows), norm_type, max_norm, norm.data_ptr(), ws.data_ptr(),
+                                                    nbytes, _stream(dev)), 'grad_clip')
+        return norm
+
+    def sgd_momentum_step_clipped(self, flat_param, flat_buf, grads, offsets, hyper, norm):
+        """SGD on clipped gradients that lie where autograd left them: grads[i] belongs at offsets[i] of the flat buffers; `hyper`
+        = {lr, momentum, weight_decay, grad_scale, max_norm} on the device; the norm of grad_scale * grads goes to `norm`."""
+        dev = _chk(flat_param, flat_buf, hyper, norm)
+        gdev, rows = self._tensor_list('sgd_momentum_step_clipped', grads, offsets)
+        if gdev != dev or hyper.numel() != 5 or flat_buf.numel() != flat_param.numel():
+            raise RuntimeError('sgd_momentum_step_clipped: five hyper-parameters, buffers of one size, all on one device')
+        if rows[:, 2].min() < 0 or (rows[:, 1] + rows[:, 2]).max() > flat_param.numel():
+            raise RuntimeError('sgd_momentum_step_clipped: a gradient reaches past the flat buffers')
+        with _on(dev):
+            ws, nbytes = self._norm_scratch(dev)
+            _lib.check(_lib.lib().deepipr_sgd_momentum_step_clipped(_p(flat_param), _p(flat_buf), rows.ctypes.data, len(rows),
+                                                                    _p(hyper), _p(norm), ws.data_ptr(), nbytes, _stream(dev)),
+                       'sgd_momentum_step_clipped')
 
 
 kernels = HipKernels()

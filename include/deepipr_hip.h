@@ -31,7 +31,7 @@ extern "C" {
 #define DEEPIPR_ELAUNCH (-2)  /* hipLaunchKernel reported an error */
 #define DEEPIPR_EUNSUPPORTED (-3)  /* shape outside the fused form (nothing was enqueued): use the unfused entry points */
 
-#define DEEPIPR_ABI_VERSION 12
+#define DEEPIPR_ABI_VERSION 13
 
 int deepipr_abi_version(void);
 const char *deepipr_last_error(void);
@@ -95,7 +95,9 @@ int deepipr_event_synchronize(void *event);
 #define DEEPIPR_K_CONV1X1_FWD 34          /* 1x1 stride-1 forward / backward-data GEMM over NCHW (deepipr_conv_1x1.inc): FLOPs */
 #define DEEPIPR_K_CONV1X1_DGRAD 35
 #define DEEPIPR_K_HEAD 36                 /* avg-pool + Linear of the CIFAR-geometry classifier, forward / backward (bytes) */
-#define DEEPIPR_PROFILE_KERNELS 37
+#define DEEPIPR_K_GRAD_NORM 37            /* partial sums of a gradient list's norm (bytes) */
+#define DEEPIPR_K_GRAD_CLIP 38            /* the list scaled in place (bytes) */
+#define DEEPIPR_PROFILE_KERNELS 39
 int deepipr_profile_enable(int on);   /* 1 = reset counters and enable, 2 = resume without reset, 0 = pause */
 int deepipr_profile_read(int kernel, double *total_ms, long long *launches);
 /* algorithmic HBM bytes of the launches timed so far, for the streaming kernels (0 for the others) */
@@ -396,6 +398,42 @@ int deepipr_sgd_momentum_step_dev(float *param, const float *grad, float *moment
 int deepipr_sgd_momentum_chunk(void);
 int deepipr_sgd_momentum_step_multi(float *param, float *momentum_buf, const long long *table, int entries,
                                     size_t total_elements, const float *hyper, void *stream);
+
+/* ------------------------------------------------------------------ global norm of a gradient list, clipping (ABI v13)
+ * n = (sum over all elements of all tensors of |g|^p)^(1/p), p = norm_type 1 or 2, or norm_type 0: max |g|.  Elements are widened
+ * to 64 bits before they are squared or added, partial sums are added in a fixed order: bit-reproducible, no overflow or underflow
+ * inside the sum.  A NaN anywhere gives NaN, an infinity without NaN gives infinity; an empty list gives 0.
+ *   deepipr_grad_norm   *norm = n.
+ *   deepipr_grad_clip   g *= f in place, f = min(1, max_norm / (n + 1e-6)) (torch.nn.utils.clip_grad_norm_'s rule); *norm = n, the norm
+ *                       BEFORE clipping.  f == 1 writes nothing (1 * g is g in every type).  A NaN norm makes every gradient NaN, an
+ *                       infinite one makes the finite gradients 0.  Products are rounded once to the tensor's type.  Tensors that
+ *                       share memory are refused.
+ *   deepipr_sgd_momentum_step_clipped   the step of deepipr_sgd_momentum_step_dev behind that rule, on gradients that lie where
+ *                       autograd left them: d = (f * grad_scale) * g + weight_decay * p; buf = momentum * buf + d; p -= lr * buf, with
+ *                       n the 2-norm of grad_scale * g over the whole list.  hyper (device) = {lr, momentum, weight_decay, grad_scale,
+ *                       max_norm}: read when the kernel runs, so a captured step follows the host's rewrites.  `offset` of an entry
+ *                       is its place in param / momentum_buf (floats, a multiple of 64; places must not overlap).
+ * The list is HOST memory, read before the call returns (captured launches keep it); `data` is device memory of `count` elements, any
+ * alignment that fits the element type; entries with count 0 are skipped.  workspace: deepipr_grad_norm_workspace_bytes() bytes, used
+ * between the launches of one call: calls that may run at the same time need one each.
+ * replaces: torch.nn.utils.clip_grad_norm_ in front of optimizer.step() (experiments/trainer.py:144-145 has no clipping). */
+#define DEEPIPR_F32 0
+#define DEEPIPR_BF16 1
+#define DEEPIPR_F16 2
+typedef struct {
+    const void *data;
+    long long count;
+    long long offset;
+    long long dtype;             /* DEEPIPR_F32 / _BF16 / _F16 */
+} DeepiprTensor;
+size_t deepipr_grad_norm_workspace_bytes(void);
+int deepipr_grad_norm(const DeepiprTensor *host_tensors, int n, int norm_type, float *norm, void *workspace,
+                      size_t workspace_bytes, void *stream);
+int deepipr_grad_clip(const DeepiprTensor *host_tensors, int n, int norm_type, float max_norm, float *norm, void *workspace,
+                      size_t workspace_bytes, void *stream);
+int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const DeepiprTensor *host_grads, int n,
+                                      const float *hyper, float *norm, void *workspace, size_t workspace_bytes,
+                                      void *stream);
 
 /* ------------------------------------------------------------------ head of the train step
  * loss = mean_n( logsumexp(logits[n]) - logits[n][target[n]] ),  top1_pct = 100 * mean_n( argmax(logits[n]) ==
