@@ -19,7 +19,7 @@ LIB_PATH = os.environ.get('DEEPIPR_LIB') or os.path.join(_HERE, 'csrc', 'libdeep
 
 _c = ctypes
 _f32p, _f64p, _i8p, _vp = _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p   # raw device addresses
-_int, _flt, _sz = _c.c_int, _c.c_float, _c.c_size_t
+_int, _flt, _sz, _i64 = _c.c_int, _c.c_float, _c.c_size_t, _c.c_longlong
 
 # name -> (restype, argtypes); mirrors include/deepipr_hip.h one to one
 SIGNATURES = {
@@ -77,6 +77,13 @@ SIGNATURES = {
     'deepipr_grad_norm': (_int, [_vp, _int, _int, _f32p, _vp, _sz, _vp]),
     'deepipr_grad_clip': (_int, [_vp, _int, _int, _flt, _f32p, _vp, _sz, _vp]),
     'deepipr_sgd_momentum_step_clipped': (_int, [_f32p, _f32p, _vp, _int, _f32p, _f32p, _vp, _sz, _vp]),
+    'deepipr_mx4_code_bytes': (_sz, [_i64, _i64]),
+    'deepipr_mx4_scale_bytes': (_sz, [_i64, _i64]),
+    'deepipr_mx4_quantize_workspace_bytes': (_sz, [_i64, _i64]),
+    'deepipr_mx4_quantize': (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _f32p, _vp, _sz, _vp]),
+    'deepipr_mx4_dequantize': (_int, [_vp, _vp, _i64, _i64, _int, _vp, _int, _vp]),
+    'deepipr_mx4_matmul_workspace_bytes': (_sz, [_i64, _i64, _i64]),
+    'deepipr_mx4_matmul': (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _sz, _vp]),
     'deepipr_passport_bn_workspace_bytes': (_sz, [_int, _int, _int]),
     'deepipr_passport_bn_fwd': (_int, [_f32p, _f32p, _f64p, _f32p, _f32p, _f32p, _flt, _flt, _flt, _f32p, _f32p, _vp,
                                        _flt, _flt, _int, _int, _int, _int, _int, _int, _f32p, _f32p, _f32p, _f32p,
@@ -204,7 +211,7 @@ PROFILE_KERNELS = ['pooled_patch_mean', 'gamma_beta_fwd', 'gamma_beta_bwd', 'aff
                    'bn_stats', 'bn_affine_fwd', 'bn_bwd_reduce', 'bn_affine_bwd', 'sgd', 'add_relu', 'bn_res_fwd',
                    'bn_res_bwd', 'gn_fwd', 'gn_bwd', 'conv_wgrad', 'conv_wgrad_reduce', 'conv_fwd', 'conv_dgrad', 'conv_wgrad_b3', 'conv_split_sum',
                    'conv_wino_fwd', 'conv_wino_dgrad', 'conv_wino_wgrad', 'conv_wino_weights', 'conv1x1_wgrad', 'maxpool', 'resample2', 'conv1x1_fwd', 'conv1x1_dgrad', 'head',
-                   'grad_norm', 'grad_clip']
+                   'grad_norm', 'grad_clip', 'mx4_quantize', 'mx4_dequantize', 'mx4_matmul']
 
 
 class ExternalEvent:

@@ -1014,6 +1014,75 @@ class HipKernels:
                                                                     _p(hyper), _p(norm), ws.data_ptr(), nbytes, _stream(dev)),
                        'sgd_momentum_step_clipped')
 
+    # ---- matrices in 4 bits (include/deepipr_hip.h: deepipr_mx4_*; deepipr_amd/mx4.py is the public face) ----
+    def _mx4_chk(self, what, *tensors):
+        dev = None
+        for t in tensors:
+            if t is None:
+                continue
+            if not t.is_cuda:
+                raise RuntimeError('deepipr_amd %s runs on the GPU only (got a %s tensor); there is no CPU fallback' % (what, t.device))
+            if dev is None:
+                dev = t.device
+            elif t.device != dev:
+                raise RuntimeError('deepipr_amd %s: tensors on different devices (%s, %s)' % (what, dev, t.device))
+        return dev
+
+    def _mx4_type(self, what, dtype):
+        code = self._DTYPE_CODE.get(dtype)
+        if code is None:
+            raise RuntimeError('deepipr_amd %s takes float32, bfloat16 and float16 (got %s)' % (what, dtype))
+        return code
+
+    def _mx4_buffers(self, rows, cols, dev):
+        lib = _lib.lib()
+        return (torch.empty(lib.deepipr_mx4_code_bytes(rows, cols), dtype=torch.uint8, device=dev),
+                torch.empty(lib.deepipr_mx4_scale_bytes(rows, cols), dtype=torch.uint8, device=dev))
+
+    def mx4_quantize(self, x, along_rows, along_cols, col_sums=False):
+        """x [R, C], columns contiguous -> ((codes, scales) of x or None, (codes, scales) of x^T or None, column sums or None)."""
+        dev = self._mx4_chk('mx4_quantize', x)
+        code = self._mx4_type('mx4_quantize', x.dtype)
+        rows, cols = x.shape
+        if cols > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < cols:
+            raise RuntimeError('deepipr_amd mx4_quantize needs a matrix with contiguous rows (got strides %s)' % (tuple(x.stride()),))
+        lib = _lib.lib()
+        with _on(dev):
+            a = self._mx4_buffers(rows, cols, dev) if along_rows else (None, None)
+            b = self._mx4_buffers(cols, rows, dev) if along_cols else (None, None)
+            sums = ws = None
+            nbytes = 0
+            if col_sums:
+                nbytes = lib.deepipr_mx4_quantize_workspace_bytes(rows, cols)
+                sums = torch.empty(cols, dtype=torch.float32, device=dev)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            _lib.check(lib.deepipr_mx4_quantize(x.data_ptr(), code, rows, cols, x.stride(0) if rows > 1 else cols, _p(a[0]), _p(a[1]),
+                                                _p(b[0]), _p(b[1]), _p(sums), _p(ws), nbytes, _stream(dev)), 'mx4_quantize')
+        return (a if along_rows else None), (b if along_cols else None), sums
+
+    def mx4_dequantize(self, codes, scales, rows, cols, transposed, dtype):
+        dev = self._mx4_chk('mx4_dequantize', codes, scales)
+        code = self._mx4_type('mx4_dequantize', dtype)
+        with _on(dev):
+            out = torch.empty((cols, rows) if transposed else (rows, cols), dtype=dtype, device=dev)
+            _lib.check(_lib.lib().deepipr_mx4_dequantize(_p(codes), _p(scales), rows, cols, int(transposed), _p(out), code, _stream(dev)),
+                       'mx4_dequantize')
+        return out
+
+    def mx4_matmul(self, a, b, m, n, k, bias, dtype):
+        """a, b: (codes, scales) of [m, k] and [n, k] -> a b^T + bias, [m, n] of `dtype`."""
+        dev = self._mx4_chk('mx4_matmul', a[0], a[1], b[0], b[1], bias)
+        code = self._mx4_type('mx4_matmul', dtype)
+        bcode = 0 if bias is None else self._mx4_type('mx4_matmul', bias.dtype)
+        lib = _lib.lib()
+        with _on(dev):
+            out = torch.empty((m, n), dtype=dtype, device=dev)
+            nbytes = lib.deepipr_mx4_matmul_workspace_bytes(m, n, k)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            _lib.check(lib.deepipr_mx4_matmul(_p(a[0]), _p(a[1]), _p(b[0]), _p(b[1]), _p(bias), bcode, m, n, k, _p(out), code, _p(ws),
+                                              nbytes, _stream(dev)), 'mx4_matmul')
+        return out
+
 
 kernels = HipKernels()
 

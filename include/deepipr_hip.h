@@ -97,7 +97,10 @@ int deepipr_event_synchronize(void *event);
 #define DEEPIPR_K_HEAD 36                 /* avg-pool + Linear of the CIFAR-geometry classifier, forward / backward (bytes) */
 #define DEEPIPR_K_GRAD_NORM 37            /* partial sums of a gradient list's norm (bytes) */
 #define DEEPIPR_K_GRAD_CLIP 38            /* the list scaled in place (bytes) */
-#define DEEPIPR_PROFILE_KERNELS 39
+#define DEEPIPR_K_MX4_QUANTIZE 39         /* bytes */
+#define DEEPIPR_K_MX4_DEQUANTIZE 40       /* bytes */
+#define DEEPIPR_K_MX4_MATMUL 41           /* FLOPs */
+#define DEEPIPR_PROFILE_KERNELS 42
 int deepipr_profile_enable(int on);   /* 1 = reset counters and enable, 2 = resume without reset, 0 = pause */
 int deepipr_profile_read(int kernel, double *total_ms, long long *launches);
 /* algorithmic HBM bytes of the launches timed so far, for the streaming kernels (0 for the others) */
@@ -434,6 +437,39 @@ int deepipr_grad_clip(const DeepiprTensor *host_tensors, int n, int norm_type, f
 int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const DeepiprTensor *host_grads, int n,
                                       const float *hyper, float *norm, void *workspace, size_t workspace_bytes,
                                       void *stream);
+
+/* ------------------------------------------------------------------ matrices in microscaled 4-bit floating point (ABI v13)
+ * MXFP4 of the open microscaling specification: 32 neighbouring values of a row share a power of two X = 2^(code - 127) (one byte,
+ * E8M0; code 255: not a number), each value is X times a 4-bit float E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives).
+ * Quantising a block: code = max(0, biased fp32 exponent of its largest magnitude - 2); every value is divided by X (exact) and rounded
+ * to the nearest code, ties to the even code, magnitudes above 6 to 6 (the largest magnitude lies in [4, 8) X).  Subnormal inputs count
+ * with their value.  A block that holds a NaN or an infinity gets code 255 and reads as NaN throughout; a row's last block may be
+ * short: what is missing counts as zero.
+ * A quantised matrix of `rows` x `cols` is two buffers, 16-byte aligned:
+ *   codes   deepipr_mx4_code_bytes():  [rows][Kp / 2] bytes, Kp = cols rounded up to 128, lower index in the low half byte, zero behind cols
+ *   scales  deepipr_mx4_scale_bytes(): [Kp / 128][ceil(rows / 64)][4][16][4] bytes: scale of block b (0..3) of these 128 columns, for the
+ *           row 16 t + r of the 64-row group, at [..][..][b][r][t] -- the order in which the matrix instruction's lanes take them.
+ *   deepipr_mx4_quantize    x [rows][cols] (row_stride elements between rows) in one pass: blocks along the rows (row_codes / row_scales),
+ *           and / or blocks along the columns, i.e. the matrix x^T [cols][rows] (col_codes / col_scales); either pair may be NULL.
+ *           col_sums (may be NULL; needs the column direction): the sums of x's columns, fp32 sums of 32 and 64 rows, then 64-bit in row
+ *           order; workspace: deepipr_mx4_quantize_workspace_bytes() bytes when col_sums is given.
+ *   deepipr_mx4_dequantize  the values in `dtype`: [rows][cols], or with transposed = 1 [cols][rows].
+ *   deepipr_mx4_matmul      out [M][N] = A B^T (+ bias [N]), A [M][K] and B [N][K] quantised, on the block-scaled matrix instructions;
+ *           fp32 products and sums, one rounding to `dtype`.  A NaN block makes NaN of every output whose row or column holds it.  workspace:
+ *           deepipr_mx4_matmul_workspace_bytes(M, N, K) bytes (may be 0); calls that may run at the same time need one each.
+ * There is no counterpart in the reference (its classifiers are nn.Linear in fp32, models/alexnet_passport.py:27-36). */
+size_t deepipr_mx4_code_bytes(long long rows, long long cols);
+size_t deepipr_mx4_scale_bytes(long long rows, long long cols);
+size_t deepipr_mx4_quantize_workspace_bytes(long long rows, long long cols);
+int deepipr_mx4_quantize(const void *x, int dtype, long long rows, long long cols, long long row_stride, void *row_codes,
+                         void *row_scales, void *col_codes, void *col_scales, float *col_sums, void *workspace,
+                         size_t workspace_bytes, void *stream);
+int deepipr_mx4_dequantize(const void *codes, const void *scales, long long rows, long long cols, int transposed, void *out,
+                           int dtype, void *stream);
+size_t deepipr_mx4_matmul_workspace_bytes(long long M, long long N, long long K);
+int deepipr_mx4_matmul(const void *a_codes, const void *a_scales, const void *b_codes, const void *b_scales, const void *bias,
+                       int bias_dtype, long long M, long long N, long long K, void *out, int dtype, void *workspace,
+                       size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------ head of the train step
  * loss = mean_n( logsumexp(logits[n]) - logits[n][target[n]] ),  top1_pct = 100 * mean_n( argmax(logits[n]) ==
