@@ -8,10 +8,11 @@
 //
 // In memory a quantised matrix of R rows and K columns, Kp = K rounded up to 128:
 //   codes   [R][Kp / 2] bytes, the value with the lower index in the low half; the columns behind K are zero;
-//   scales  [Kp / 128][ceil(R / 64)][64] words of 4 bytes: word l = 16 * b + r of a 64-row group holds the scale of block b (of the
-//           four of these 128 columns) for the rows r, 16 + r, 32 + r, 48 + r -- the order in which the lanes of
-//           v_mfma_scale_f32_16x16x128_f8f6f4 take them: one coalesced 256-byte load serves four matrix instructions' rows.
+//   scales  [Kp / 128][ceil(R / 64)][64] words of 4 bytes: word 32 (b % 2) + r % 32 of a 64-row group holds the scales of the blocks b % 2
+//           and 2 + b % 2 (of the four of these 128 columns) of the rows r % 32 and 32 + r % 32; byte 2 (b / 2) + r / 32.  That is the order
+//           in which the lanes of v_mfma_scale_f32_32x32x64_f8f6f4 take them: one coalesced 256-byte load serves 64 rows x 128 columns.
 #include <cmath>
+#include <cstdlib>
 
 #include "deepipr_host.h"
 
@@ -24,6 +25,9 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 __host__ __device__ inline long long round_up(long long v, long long m) { return (v + m - 1) / m * m; }
@@ -57,22 +61,17 @@ template <int T> __device__ __forceinline__ void store1(void *p, long long i, fl
     if (T == F32) static_cast<float *>(p)[i] = v;
     else static_cast<unsigned short *>(p)[i] = static_cast<unsigned short>(T == BF16 ? f32_to_bf16(v) : f32_to_f16(v));
 }
-// four neighbours at once (the caller checked the alignment)
-template <int T> __device__ __forceinline__ void store4(void *p, long long i, f32x4 v) {
+// four neighbours at once (the caller checked the alignment); gfx950 converts pairs, to nearest, ties to even
+template <int T> __device__ __forceinline__ void store4(void *p, f32x4 v) {
     if (T == F32) {
-        *reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i) = v;
+        *static_cast<f32x4 *>(p) = v;
+    } else if (T == BF16) {
+        *static_cast<bf16x4 *>(p) = __builtin_convertvector(v, bf16x4);
     } else {
-        u32x2 o;
-        if (T == BF16) {
-            o.x = f32_to_bf16(v.x) | f32_to_bf16(v.y) << 16;
-            o.y = f32_to_bf16(v.z) | f32_to_bf16(v.w) << 16;
-        } else {
-            o.x = f32_to_f16(v.x) | f32_to_f16(v.y) << 16;
-            o.y = f32_to_f16(v.z) | f32_to_f16(v.w) << 16;
-        }
-        *reinterpret_cast<u32x2 *>(static_cast<unsigned short *>(p) + i) = o;
+        *static_cast<f16x4 *>(p) = __builtin_convertvector(v, f16x4);
     }
 }
+template <int T> __device__ __forceinline__ void *element(void *p, long long i) { return static_cast<char *>(p) + i * (T == F32 ? 4 : 2); }
 
 // ------------------------------------------------------------------------------------------------------- one block of 32 values
 // `top`: the largest magnitude's bits (NaN and infinity compare above every finite value as integers).  -> the scale byte
@@ -163,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
         unsigned code;
         const u32x4 q = quantise32(v, code);
         if (r0 + r < R) *reinterpret_cast<u32x4 *>(row_codes + (r0 + r) * (tiles_c * (kQC / 2)) + c0 / 2 + b * 16) = q;
-        sc[0][(b * 16 + (r & 15)) * 4 + (r >> 4)] = static_cast<unsigned char>(code);
+        sc[0][((b & 1) * 32 + (r & 31)) * 4 + (b >> 1) * 2 + (r >> 5)] = static_cast<unsigned char>(code);
     }
     if (COL) {
         const int c = tid & 127, h = tid >> 7;
@@ -177,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
         const u32x4 q = quantise32(v, code);
         const long long pitch = round_up(R, 128) / 2;
         if (c0 + c < C) *reinterpret_cast<u32x4 *>(col_codes + (c0 + c) * pitch + r0 / 2 + h * 16) = q;
-        sc[1][(c >> 6) * 128 + (h * 16 + (c & 15)) * 4 + ((c & 63) >> 4)] = static_cast<unsigned char>(code);
+        sc[1][(c >> 6) * 128 + (h * 32 + (c & 31)) * 2 + (c >> 5 & 1)] = static_cast<unsigned char>(code);
         if (SUM) {
             __syncthreads();                             // the tile has been read: its first row takes the upper half's sums
             if (h == 1) s[c] = sum;
@@ -188,11 +187,11 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
     __syncthreads();
     // (with the column direction the grid covers the rows' padding too: row groups that do not exist there)
     if (ROW && tid < 64 && r0 < R) row_scales[(c0 / 128 * row_groups(R) + r0 / 64) * 64 + tid] = reinterpret_cast<const unsigned *>(sc[0])[tid];
-    if (COL && tid < 64) {
-        const int g = tid >> 5;                          // of the tile's two 64-column groups
-        const long long rg = c0 / 64 + g;
+    if (COL && tid < 128) {                              // these 64 rows are one half (two of four blocks) of every word
+        const long long rg = c0 / 64 + (tid >> 6);
         if (rg < row_groups(C))
-            col_scales[(r0 / 128 * row_groups(C) + rg) * 64 + (r0 / 64 & 1) * 32 + (tid & 31)] = reinterpret_cast<const unsigned *>(sc[1])[tid];
+            reinterpret_cast<unsigned short *>(col_scales)[((r0 / 128 * row_groups(C) + rg) * 64 + (tid & 63)) * 2 + (r0 / 64 & 1)] =
+                reinterpret_cast<const unsigned short *>(sc[1])[tid];
     }
 }
 
@@ -208,8 +207,8 @@ __global__ __launch_bounds__(kThreads) void k_mx4_colsum(const float *__restrict
 // ----------------------------------------------------------------------------------------------------------------- dequantise
 // The matrix [R][K] of values, or its transpose [K][R].  A thread decodes 8 codes; the transposed form goes through LDS.
 __device__ __forceinline__ unsigned scale_at(const unsigned *scales, long long rows, long long r, long long b) {
-    const unsigned w = scales[((b >> 2) * row_groups(rows) + (r >> 6)) * 64 + (b & 3) * 16 + (r & 15)];
-    return w >> ((r >> 4 & 3) * 8) & 0xffu;
+    const unsigned w = scales[((b >> 2) * row_groups(rows) + (r >> 6)) * 64 + (b & 1) * 32 + (r & 31)];
+    return w >> (((b >> 1 & 1) * 2 + (r >> 5 & 1)) * 8) & 0xffu;
 }
 __device__ __forceinline__ void decode8(unsigned w, float x, float *v) {
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
@@ -227,8 +226,8 @@ __global__ __launch_bounds__(kThreads) void k_mx4_dequantise(const unsigned char
         float v[8];
         decode8(*reinterpret_cast<const unsigned *>(codes + r * pitch + k / 2), scale_value(scale_at(scales, R, r, k / 32)), v);
         if (vec && k + 8 <= K) {
-            store4<T>(out, r * K + k, f32x4{v[0], v[1], v[2], v[3]});
-            store4<T>(out, r * K + k + 4, f32x4{v[4], v[5], v[6], v[7]});
+            store4<T>(element<T>(out, r * K + k), f32x4{v[0], v[1], v[2], v[3]});
+            store4<T>(element<T>(out, r * K + k + 4), f32x4{v[4], v[5], v[6], v[7]});
         } else {
             for (int j = 0; j < 8 && k + j < K; ++j) store1<T>(out, r * K + k + j, v[j]);
         }
@@ -260,77 +259,276 @@ __global__ __launch_bounds__(kThreads) void k_mx4_dequantise_t(const unsigned ch
 }
 
 // -------------------------------------------------------------------------------------------------------------------- product
-// out[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]), A [M][K] and B [N][K] quantised.  v_mfma_scale_f32_16x16x128_f8f6f4: lane l gives 32
-// codes of row l % 16 (block l / 16 of the 128 columns) and that block's scale; B is the instruction's first operand, so that a lane
-// holds four neighbouring n of one m.  Products and sums in 32 bits.
+// out[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]), A [M][K] and B [N][K] quantised.  v_mfma_scale_f32_32x32x64_f8f6f4: lane l gives 32
+// codes of row l % 32 (block l / 32 of 64 columns) and that block's scale, a byte of a word; B is the instruction's first operand, so
+// that a lane holds four times four neighbouring n of one m.  Products and sums in 32 bits.
+// (Measured: one wave per SIMD issues these at 9.1 PFLOP/s over the card, v_mfma_scale_f32_16x16x128_f8f6f4 at 5.2.)
 __device__ __forceinline__ float bias_at(const void *bias, int type, long long n) {
     return type == F32 ? load1<F32>(bias, n) : type == BF16 ? load1<BF16>(bias, n) : load1<F16>(bias, n);
 }
 
 template <int SA, int SB>
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, unsigned sa, unsigned sb) {
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c, unsigned sa, unsigned sb) {
     const i32x8 av = {static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z), static_cast<int>(a.w), 0, 0, 0, 0};
     const i32x8 bv = {static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z), static_cast<int>(b.w), 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, SA, static_cast<int>(sa), SB, static_cast<int>(sb));
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, SA, static_cast<int>(sa), SB, static_cast<int>(sb));
 }
 
+// The outputs of a wave, TM x TN tiles of 32 x 32 (acc[n tile][m tile]; a lane holds n = 8 q + 4 (lane / 32) .. + 3 of m = lane % 32), to
+// rows m0 .. of `out`, 32 rows at a time through `strip` (32 rows of 32 TN + 4 floats of this wave's own): whole cache lines per row.
+template <int T, int TM, int TN>
+__device__ __forceinline__ void store_tiles(const f32x16 (&acc)[TN][TM], float *strip, const void *bias, int bias_type, long long m0, long long n0,
+                                            long long M, long long N, int vec, void *out) {
+    constexpr int P = 32 * TN + 4, PER = 8 * TN, STEP = 64 / PER;          // lanes per row (a lane keeps its columns), rows per pass
+    const int lane = threadIdx.x & 63, row = lane / PER;
+    const long long n = n0 + lane % PER * 4;
+    f32x4 add = {};
+    if (bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < N) add[j] = bias_at(bias, bias_type, n + j);
+    }
+    const bool whole = vec && m0 + 32 * TM <= M && n0 + 32 * TN <= N;      // uniform: nearly every tile of a large product
+    const float *from = strip + row * P + lane % PER * 4;
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f32x4 *>(strip + (lane & 31) * P + i * 32 + q * 8 + (lane >> 5) * 4) =
+                    f32x4{acc[i][t][4 * q], acc[i][t][4 * q + 1], acc[i][t][4 * q + 2], acc[i][t][4 * q + 3]};
+        if (whole) {
+            char *to = static_cast<char *>(element<T>(out, (m0 + t * 32 + row) * N + n));
+            const long long step = N * (STEP * (T == F32 ? 4 : 2));
+#pragma unroll
+            for (int r = 0; r < 32; r += STEP) {
+                store4<T>(to, *reinterpret_cast<const f32x4 *>(from + r * P) + add);
+                to += step;
+            }
+        } else {
+            for (int r = 0; r < 32; r += STEP) {
+                const long long m = m0 + t * 32 + row + r;
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(from + r * P) + add;
+                if (m >= M) continue;
+                if (vec && n + 4 <= N) {
+                    store4<T>(element<T>(out, m * N + n), v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (n + j < N) store1<T>(out, m * N + n + j, v[j]);
+                }
+            }
+        }
+    }
+}
+
+// Small products: a wave takes 64 x 64 outputs straight from the caches.
 template <int T>
 __global__ __launch_bounds__(kThreads) void k_mx4_gemm(const unsigned char *__restrict__ a, const unsigned *__restrict__ sa,
                                                        const unsigned char *__restrict__ b, const unsigned *__restrict__ sb,
                                                        const void *__restrict__ bias, int bias_type, long long M, long long N, long long kt,
                                                        int vec, void *__restrict__ out) {
+    __shared__ __align__(16) float strips[4 * 32 * 68];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long tiles_n = (N + 127) / 128;
     const long long m0 = static_cast<long long>(blockIdx.x) / tiles_n * 128 + (wave >> 1) * 64;
     const long long n0 = static_cast<long long>(blockIdx.x) % tiles_n * 128 + (wave & 1) * 64;
     if (m0 >= M || n0 >= N) return;
     const long long pitch = kt * 64;
-    const unsigned char *pa[4], *pb[4];
+    const unsigned char *pa[2], *pb[2];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {                        // rows behind the end read the last one; what they give is not stored
-        pa[t] = a + min(m0 + t * 16 + (lane & 15), M - 1) * pitch + (lane >> 4) * 16;
-        pb[t] = b + min(n0 + t * 16 + (lane & 15), N - 1) * pitch + (lane >> 4) * 16;
+    for (int t = 0; t < 2; ++t) {                        // rows behind the end read the last one; what they give is not stored
+        pa[t] = a + min(m0 + t * 32 + (lane & 31), M - 1) * pitch + (lane >> 5) * 16;
+        pb[t] = b + min(n0 + t * 32 + (lane & 31), N - 1) * pitch + (lane >> 5) * 16;
     }
     const unsigned *qa = sa + m0 / 64 * 64 + lane, *qb = sb + n0 / 64 * 64 + lane;
-    f32x4 acc[4][4] = {};
+    f32x16 acc[2][2] = {};
     for (long long k = 0; k < kt; ++k) {
-        u32x4 fa[4], fb[4];
+        u32x4 fa[2][2], fb[2][2];
         const unsigned wa = qa[k * row_groups(M) * 64], wb = qb[k * row_groups(N) * 64];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            fa[t] = *reinterpret_cast<const u32x4 *>(pa[t] + k * 64);
-            fb[t] = *reinterpret_cast<const u32x4 *>(pb[t] + k * 64);
-        }
-#define MX4_ROW(J)                                                                      \
-        acc[0][J] = mfma<0, J>(fb[0], fa[J], acc[0][J], wb, wa);                        \
-        acc[1][J] = mfma<1, J>(fb[1], fa[J], acc[1][J], wb, wa);                        \
-        acc[2][J] = mfma<2, J>(fb[2], fa[J], acc[2][J], wb, wa);                        \
-        acc[3][J] = mfma<3, J>(fb[3], fa[J], acc[3][J], wb, wa);
-        MX4_ROW(0) MX4_ROW(1) MX4_ROW(2) MX4_ROW(3)
-#undef MX4_ROW
-    }
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long long n = n0 + i * 16 + (lane >> 4) * 4;
-        f32x4 add = {};
-        if (bias)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < N) add[j] = bias_at(bias, bias_type, n + j);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const long long m = m0 + t * 16 + (lane & 15);
-            if (m >= M) continue;
-            const f32x4 v = acc[i][t] + add;
-            if (vec && n + 4 <= N) {
-                store4<T>(out, m * N + n, v);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n + j < N) store1<T>(out, m * N + n + j, v[j]);
+            for (int h = 0; h < 2; ++h) {
+                fa[t][h] = *reinterpret_cast<const u32x4 *>(pa[t] + k * 64 + h * 32);
+                fb[t][h] = *reinterpret_cast<const u32x4 *>(pb[t] + k * 64 + h * 32);
             }
-        }
+#define MX4_HALF(H)                                                                       \
+        acc[0][0] = mfma<2 * H, 2 * H>(fb[0][H], fa[0][H], acc[0][0], wb, wa);            \
+        acc[1][0] = mfma<2 * H + 1, 2 * H>(fb[1][H], fa[0][H], acc[1][0], wb, wa);        \
+        acc[0][1] = mfma<2 * H, 2 * H + 1>(fb[0][H], fa[1][H], acc[0][1], wb, wa);        \
+        acc[1][1] = mfma<2 * H + 1, 2 * H + 1>(fb[1][H], fa[1][H], acc[1][1], wb, wa);
+        MX4_HALF(0) MX4_HALF(1)
+#undef MX4_HALF
     }
+    store_tiles<T, 2, 2>(acc, strips + wave * 32 * 68, bias, bias_type, m0, n0, M, N, vec, out);
+}
+
+// Large products: a workgroup of four waves takes a tile of 64 TM x 64 TN outputs, a wave 32 TM x 32 TN of it (TM, TN even).
+// A step is 256 columns, 128 bytes of every row: one cache line.  Its codes and scales go to LDS without passing registers while the
+// step before is worked on (two stages); the fragments of the next 64 columns are read from LDS while the matrix cores work on these.
+//   codes in LDS: 128 bytes a row, the 16-byte block b of row r at slot b ^ (r / 2 % 8): eight lanes fetch one row's line, and the 16
+//   lanes that LDS serves at once (rows 0-3, 12-15, 20-27 or 4-11, 16-19, 28-31 of a fragment) touch every bank once.
+// Per step and workgroup (TM = TN = 4): 64 matrix instructions of 32 cycles on each of four SIMDs = 2048 cycles, 128 KB of LDS reads
+// (512 cycles at 256 B per cycle) and 68 KB from the caches.
+typedef __attribute__((address_space(3))) void *lptr;
+__device__ __forceinline__ unsigned lds_offset(const void *p) { return static_cast<unsigned>(reinterpret_cast<uintptr_t>((lptr)p)); }
+// 16 (4) bytes per lane from `src` to LDS offset `to` + 16 (4) * lane.  Written as assembly because the compiler would wait for ALL of
+// them in front of every LDS read; there is no result register, the kernel waits itself.
+__device__ __forceinline__ void to_lds16(const void *src, unsigned to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ void to_lds4(const void *src, unsigned to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(to) : "memory", "m0");
+}
+
+template <int TM, int TN> struct Tile {
+    static constexpr int BM = 64 * TM, BN = 64 * TN;
+    static constexpr int kCodes = (BM + BN) * 128, kWords = (BM + BN) * 4, kStage = kCodes + 2 * kWords;
+    static constexpr int kCodeLoads = (BM + BN) / 32, kWordLoads = (BM + BN) / 256;         // 1 KB pieces and pairs of 256 B pieces, per wave
+};
+
+__device__ __forceinline__ int slot_of(int r, int b) { return b ^ (r >> 1 & 7); }
+
+template <int T, int TM, int TN>
+__global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const unsigned char *__restrict__ a, const unsigned *__restrict__ sa,
+                                                                const unsigned char *__restrict__ b, const unsigned *__restrict__ sb,
+                                                                const void *__restrict__ bias, int bias_type, long long M, long long N,
+                                                                int kt, int vec, void *__restrict__ out) {
+    typedef Tile<TM, TN> G;
+    __shared__ __align__(16) unsigned char lds[2 * G::kStage];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles_m = static_cast<int>((M + G::BM - 1) / G::BM), tiles_n = static_cast<int>((N + G::BN - 1) / G::BN);
+    // one XCD's workgroups walk neighbouring tiles, 8 tile rows at a time: operands meet in its L2
+    const int id = dipr_xcd_contiguous(blockIdx.x, gridDim.x);
+    const int group = 8 * tiles_n, first = id / group * 8, high = min(8, tiles_m - first);
+    const long long m0 = static_cast<long long>(first + id % group % high) * G::BM, n0 = static_cast<long long>(id % group / high) * G::BN;
+    const long long pitch = static_cast<long long>(kt) * 64;
+    const int steps = (kt + 1) / 2;
+
+    // this lane's source addresses: code pieces of 8 rows (rows 0 .. BM - 1 of a, then BN of b), scale pieces of 64 rows.  An odd number
+    // of 128-column groups: the last step's upper half does not exist, the lower one is fetched in its place and not used.
+    const unsigned char *src[G::kCodeLoads];
+#pragma unroll
+    for (int j = 0; j < G::kCodeLoads; ++j) {
+        const int piece = wave * G::kCodeLoads + j, r = (piece & 1) * 8 + (lane >> 3);
+        const bool of_a = piece < G::BM / 8;
+        const long long row = of_a ? min(m0 + piece * 8 + (lane >> 3), M - 1) : min(n0 + (piece - G::BM / 8) * 8 + (lane >> 3), N - 1);
+        src[j] = (of_a ? a : b) + row * pitch + slot_of(r, lane & 7) * 16;
+    }
+    const unsigned *ssrc[G::kWordLoads];
+    long long sstep[G::kWordLoads];
+#pragma unroll
+    for (int j = 0; j < G::kWordLoads; ++j) {
+        const int piece = wave * G::kWordLoads + j;
+        const bool of_a = piece < G::BM / 64;
+        const long long groups = of_a ? row_groups(M) : row_groups(N);
+        const long long g = of_a ? min(m0 / 64 + piece, groups - 1) : min(n0 / 64 + piece - G::BM / 64, groups - 1);
+        ssrc[j] = (of_a ? sa : sb) + g * 64 + lane;
+        sstep[j] = groups * 64;
+    }
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds));
+    auto fetch = [&](int s) {
+        const unsigned base = lds0 + (s & 1) * G::kStage;
+        const bool half = 2 * s + 1 == kt;
+#pragma unroll
+        for (int j = 0; j < G::kCodeLoads; ++j) {
+            const int piece = wave * G::kCodeLoads + j, r = (piece & 1) * 8 + (lane >> 3);
+            const int back = half && slot_of(r, lane & 7) >= 4 ? 64 : 0;
+            to_lds16(src[j] - back, base + piece * 1024);
+            src[j] += 128;
+        }
+#pragma unroll
+        for (int j = 0; j < G::kWordLoads; ++j) {
+            const unsigned to = base + G::kCodes + (wave * G::kWordLoads + j) * 256;
+            to_lds4(ssrc[j], to);
+            to_lds4(half ? ssrc[j] : ssrc[j] + sstep[j], to + G::kWords);
+            ssrc[j] += 2 * sstep[j];
+        }
+    };
+    const int wm = (wave >> 1) * TM, wn = (wave & 1) * TN;              // this wave's first 32-row tile of a and of b
+    int frag[4];                                                        // where this lane's block of the q-th 64 columns lies in a tile of 32 rows
+#pragma unroll
+    for (int q = 0; q < 4; ++q) frag[q] = (lane & 31) * 128 + slot_of(lane & 31, 2 * q + (lane >> 5)) * 16;
+    struct Frags {
+        u32x4 a[TM], b[TN];
+    };
+    struct Words {
+        unsigned a[TM / 2], b[TN / 2];
+    };
+    auto read = [&](Frags &f, int s, int q) {
+        const unsigned char *base = lds + (s & 1) * G::kStage;
+#pragma unroll
+        for (int t = 0; t < TN; ++t) f.b[t] = *reinterpret_cast<const u32x4 *>(base + G::BM * 128 + (wn + t) * 4096 + frag[q]);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) f.a[t] = *reinterpret_cast<const u32x4 *>(base + (wm + t) * 4096 + frag[q]);
+    };
+    auto read_words = [&](Words &w, int s, int half) {
+        const unsigned char *base = lds + (s & 1) * G::kStage + G::kCodes + half * G::kWords;
+#pragma unroll
+        for (int t = 0; t < TN / 2; ++t) w.b[t] = reinterpret_cast<const unsigned *>(base + G::BM * 4 + (wn / 2 + t) * 256)[lane];
+#pragma unroll
+        for (int t = 0; t < TM / 2; ++t) w.a[t] = reinterpret_cast<const unsigned *>(base + (wm / 2 + t) * 256)[lane];
+    };
+    f32x16 acc[TN][TM] = {};
+#define MX4_MULTIPLY(F, W, H)                                                                                                 \
+    _Pragma("unroll") for (int j = 0; j < TM; j += 2) _Pragma("unroll") for (int i = 0; i < TN; i += 2) {                     \
+        acc[i][j] = mfma<2 * H, 2 * H>(F.b[i], F.a[j], acc[i][j], W.b[i / 2], W.a[j / 2]);                                    \
+        acc[i + 1][j] = mfma<2 * H + 1, 2 * H>(F.b[i + 1], F.a[j], acc[i + 1][j], W.b[i / 2], W.a[j / 2]);                    \
+        acc[i][j + 1] = mfma<2 * H, 2 * H + 1>(F.b[i], F.a[j + 1], acc[i][j + 1], W.b[i / 2], W.a[j / 2]);                    \
+        acc[i + 1][j + 1] = mfma<2 * H + 1, 2 * H + 1>(F.b[i + 1], F.a[j + 1], acc[i + 1][j + 1], W.b[i / 2], W.a[j / 2]);    \
+    }
+    // one LDS read behind each of the first matrix instructions
+    auto interleave = [&](int reads) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+        for (int i = 0; i < reads; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // everything fetched is in LDS, everything read from it is in registers; for all waves
+    auto arrived = [&]() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    };
+    fetch(0);
+    Frags f0, f1;
+    Words w0, w1;
+    arrived();
+    if (steps > 1) fetch(1);
+    read(f0, 0, 0);
+    read_words(w0, 0, 0);
+    for (int s = 0; s < kt / 2; ++s) {
+        read(f1, s, 1);
+        MX4_MULTIPLY(f0, w0, 0)
+        interleave(TM + TN);
+        read_words(w1, s, 1);
+        read(f0, s, 2);
+        MX4_MULTIPLY(f1, w0, 1)
+        interleave(TM + TN + TM / 2 + TN / 2);
+        read(f1, s, 3);
+        MX4_MULTIPLY(f0, w1, 0)
+        interleave(TM + TN);
+        // the next step is in LDS; behind the barrier every wave has read this one, whose stage is free
+        arrived();
+        if (s + 2 < steps) fetch(s + 2);
+        read_words(w0, s + 1, 0);                        // (behind the last step: what is read there is not used)
+        read(f0, s + 1, 0);
+        MX4_MULTIPLY(f1, w1, 1)
+        interleave(TM + TN + TM / 2 + TN / 2);
+    }
+    if (kt & 1) {
+        read(f1, steps - 1, 1);
+        MX4_MULTIPLY(f0, w0, 0)
+        MX4_MULTIPLY(f1, w0, 1)
+    }
+#undef MX4_MULTIPLY
+
+    __syncthreads();                                     // every wave is through with the stages
+    store_tiles<T, TM, TN>(acc, reinterpret_cast<float *>(lds) + wave * 32 * (32 * TN + 4), bias, bias_type, m0 + wm * 32, n0 + wn * 32, M, N, vec, out);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host side
@@ -446,15 +644,29 @@ int deepipr_mx4_matmul(const void *a_codes, const void *a_scales, const void *b_
     if (workspace_bytes < deepipr_mx4_matmul_workspace_bytes(M, N, K) || (!workspace && deepipr_mx4_matmul_workspace_bytes(M, N, K)))
         return dipr_fail(DEEPIPR_EINVAL, "%s: workspace too small", what);
     const long long tiles = ((M + 127) / 128) * ((N + 127) / 128);
-    if (tiles > kMaxGrid) return dipr_fail(DEEPIPR_EINVAL, "%s: matrix too large", what);
+    const long long steps = round_up(K, 128) / 128;
+    if (tiles > kMaxGrid || steps > kMaxGrid) return dipr_fail(DEEPIPR_EINVAL, "%s: matrix too large", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int vec = N % 4 == 0 && aligned(out, 4 * elem_bytes(dtype));
     DiprProf prof(DEEPIPR_K_MX4_MATMUL);
     prof.bytes = 2.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+    const unsigned char *a = static_cast<const unsigned char *>(a_codes), *b = static_cast<const unsigned char *>(b_codes);
+    const unsigned *sa = static_cast<const unsigned *>(a_scales), *sb = static_cast<const unsigned *>(b_scales);
+    const long long big = ((M + 255) / 256) * ((N + 255) / 256);
+    int form = big >= 128 ? 2 : tiles >= 64 ? 1 : 0;
+    if (getenv("MX4_FORM")) form = atoi(getenv("MX4_FORM"));
 #define MX4_GEMM(T)                                                                                                                  \
-    DIPR_LAUNCH(prof, (k_mx4_gemm<T>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), st, static_cast<const unsigned char *>(a_codes), \
-                static_cast<const unsigned *>(a_scales), static_cast<const unsigned char *>(b_codes), static_cast<const unsigned *>(b_scales), \
-                bias, bias_dtype, M, N, round_up(K, 128) / 128, vec, out)
+    do {                                                                                                                             \
+        if (form == 2)                                                                                                               \
+            DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 4, 4>), dim3(static_cast<unsigned>(big)), dim3(kThreads), st, a, sa, b, sb, bias, bias_dtype, M, \
+                        N, static_cast<int>(steps), vec, out);                                                                       \
+        else if (form == 1)                                                                                                          \
+            DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 2, 2>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), st, a, sa, b, sb, bias, bias_dtype, \
+                        M, N, static_cast<int>(steps), vec, out);                                                                    \
+        else                                                                                                                         \
+            DIPR_LAUNCH(prof, (k_mx4_gemm<T>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), st, a, sa, b, sb, bias, bias_dtype, M, N, steps, \
+                        vec, out);                                                                                                   \
+    } while (0)
     switch (dtype) {
         case F32: MX4_GEMM(F32); break;
         case BF16: MX4_GEMM(BF16); break;

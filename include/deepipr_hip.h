@@ -447,8 +447,8 @@ int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const D
  * short: what is missing counts as zero.
  * A quantised matrix of `rows` x `cols` is two buffers, 16-byte aligned:
  *   codes   deepipr_mx4_code_bytes():  [rows][Kp / 2] bytes, Kp = cols rounded up to 128, lower index in the low half byte, zero behind cols
- *   scales  deepipr_mx4_scale_bytes(): [Kp / 128][ceil(rows / 64)][4][16][4] bytes: scale of block b (0..3) of these 128 columns, for the
- *           row 16 t + r of the 64-row group, at [..][..][b][r][t] -- the order in which the matrix instruction's lanes take them.
+ *   scales  deepipr_mx4_scale_bytes(): [Kp / 128][ceil(rows / 64)][2][32][2][2] bytes: scale of block 2 h + e (0..3) of these 128 columns, for
+ *           the row 32 t + r of the 64-row group, at [..][..][e][r][h][t] -- the order in which the matrix instruction's lanes take them.
  *   deepipr_mx4_quantize    x [rows][cols] (row_stride elements between rows) in one pass: blocks along the rows (row_codes / row_scales),
  *           and / or blocks along the columns, i.e. the matrix x^T [cols][rows] (col_codes / col_scales); either pair may be NULL.
  *           col_sums (may be NULL; needs the column direction): the sums of x's columns, fp32 sums of 32 and 64 rows, then 64-bit in row

@@ -50,6 +50,6 @@ def unpack(codes, scales, rows, cols):
     b = codes.cpu().numpy().reshape(rows, kp // 2)
     full = np.stack([b & 15, b >> 4], -1).reshape(rows, kp)
     rg = -(-rows // 64)
-    s = scales.cpu().numpy().reshape(kp // KP, rg, 4, 16, 4)    # [k128][group][block][row % 16][tile]
-    s = s.transpose(1, 4, 3, 0, 2).reshape(rg * 64, kp // 32)[:rows]
+    s = scales.cpu().numpy().reshape(kp // KP, rg, 2, 32, 2, 2)    # [k128][group][block % 2][row % 32][block / 2][row / 32]
+    s = s.transpose(1, 5, 3, 0, 4, 2).reshape(rg * 64, kp // 32)[:rows]
     return full[:, :cols].astype(np.int64), s[:, :-(-cols // 32)].astype(np.int64), not full[:, cols:].any()
