@@ -7,7 +7,9 @@
 // A block that holds a NaN or an infinity gets code 255: all of it reads as NaN.
 //
 // In memory a quantised matrix of R rows and K columns, Kp = K rounded up to 128:
-//   codes   [R][Kp / 2] bytes, the value with the lower index in the low half; the columns behind K are zero;
+//   codes   [Kp / 128][R][64] bytes: 128 columns of a row are 64 bytes, neighbouring rows' neighbours in memory (a tile of a product
+//           is then whole cache lines however few columns it takes); the value with the lower index in the low half byte; the columns
+//           behind K are zero;
 //   scales  [Kp / 128][ceil(R / 64)][64] words of 4 bytes: word 32 (b % 2) + r % 32 of a 64-row group holds the scales of the blocks b % 2
 //           and 2 + b % 2 (of the four of these 128 columns) of the rows r % 32 and 32 + r % 32; byte 2 (b / 2) + r / 32.  That is the order
 //           in which the lanes of v_mfma_scale_f32_32x32x64_f8f6f4 take them: one coalesced 256-byte load serves 64 rows x 128 columns.
@@ -161,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
         for (int k = 0; k < 8; ++k) *reinterpret_cast<f32x4 *>(v + 4 * k) = *reinterpret_cast<const f32x4 *>(s + r * kQP + b * 32 + 4 * k);
         unsigned code;
         const u32x4 q = quantise32(v, code);
-        if (r0 + r < R) *reinterpret_cast<u32x4 *>(row_codes + (r0 + r) * (tiles_c * (kQC / 2)) + c0 / 2 + b * 16) = q;
+        if (r0 + r < R) *reinterpret_cast<u32x4 *>(row_codes + (c0 / 128 * R + r0 + r) * 64 + b * 16) = q;
         sc[0][((b & 1) * 32 + (r & 31)) * 4 + (b >> 1) * 2 + (r >> 5)] = static_cast<unsigned char>(code);
     }
     if (COL) {
@@ -174,8 +176,7 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
         }
         unsigned code;
         const u32x4 q = quantise32(v, code);
-        const long long pitch = round_up(R, 128) / 2;
-        if (c0 + c < C) *reinterpret_cast<u32x4 *>(col_codes + (c0 + c) * pitch + r0 / 2 + h * 16) = q;
+        if (c0 + c < C) *reinterpret_cast<u32x4 *>(col_codes + (r0 / 128 * C + c0 + c) * 64 + (r0 / 64 & 1) * 32 + h * 16) = q;
         sc[1][(c >> 6) * 128 + (h * 32 + (c & 31)) * 2 + (c >> 5 & 1)] = static_cast<unsigned char>(code);
         if (SUM) {
             __syncthreads();                             // the tile has been read: its first row takes the upper half's sums
@@ -210,6 +211,9 @@ __device__ __forceinline__ unsigned scale_at(const unsigned *scales, long long r
     const unsigned w = scales[((b >> 2) * row_groups(rows) + (r >> 6)) * 64 + (b & 1) * 32 + (r & 31)];
     return w >> (((b >> 1 & 1) * 2 + (r >> 5 & 1)) * 8) & 0xffu;
 }
+__device__ __forceinline__ unsigned codes_at(const unsigned char *codes, long long rows, long long r, long long k) {     // k a multiple of 8
+    return *reinterpret_cast<const unsigned *>(codes + ((k >> 7) * rows + r) * 64 + (k & 127) / 2);
+}
 __device__ __forceinline__ void decode8(unsigned w, float x, float *v) {
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
     const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
@@ -220,11 +224,11 @@ __device__ __forceinline__ void decode8(unsigned w, float x, float *v) {
 template <int T>
 __global__ __launch_bounds__(kThreads) void k_mx4_dequantise(const unsigned char *__restrict__ codes, const unsigned *__restrict__ scales,
                                                              long long R, long long K, int vec, void *__restrict__ out) {
-    const long long per = (K + 7) / 8, n = R * per, pitch = round_up(K, 128) / 2;
+    const long long per = (K + 7) / 8, n = R * per;
     for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads) {
         const long long r = i / per, k = i % per * 8;
         float v[8];
-        decode8(*reinterpret_cast<const unsigned *>(codes + r * pitch + k / 2), scale_value(scale_at(scales, R, r, k / 32)), v);
+        decode8(codes_at(codes, R, r, k), scale_value(scale_at(scales, R, r, k / 32)), v);
         if (vec && k + 8 <= K) {
             store4<T>(element<T>(out, r * K + k), f32x4{v[0], v[1], v[2], v[3]});
             store4<T>(element<T>(out, r * K + k + 4), f32x4{v[4], v[5], v[6], v[7]});
@@ -241,13 +245,11 @@ __global__ __launch_bounds__(kThreads) void k_mx4_dequantise_t(const unsigned ch
     __shared__ float s[64 * 65];
     const long long tiles_r = (R + 63) / 64;
     const long long r0 = static_cast<long long>(blockIdx.x) % tiles_r * 64, k0 = static_cast<long long>(blockIdx.x) / tiles_r * 64;
-    const long long pitch = round_up(K, 128) / 2;
     for (int i = threadIdx.x; i < 64 * 8; i += kThreads) {
         const int r = i >> 3, k = (i & 7) * 8;
         float v[8] = {};
         if (r0 + r < R)                                  // columns behind K lie in the padding: zero codes
-            decode8(*reinterpret_cast<const unsigned *>(codes + (r0 + r) * pitch + (k0 + k) / 2),
-                    scale_value(scale_at(scales, R, r0 + r, (k0 + k) / 32)), v);
+            decode8(codes_at(codes, R, r0 + r, k0 + k), scale_value(scale_at(scales, R, r0 + r, (k0 + k) / 32)), v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[(k + j) * 65 + r] = v[j];
     }
@@ -335,12 +337,11 @@ __global__ __launch_bounds__(kThreads) void k_mx4_gemm(const unsigned char *__re
     const long long m0 = static_cast<long long>(blockIdx.x) / tiles_n * 128 + (wave >> 1) * 64;
     const long long n0 = static_cast<long long>(blockIdx.x) % tiles_n * 128 + (wave & 1) * 64;
     if (m0 >= M || n0 >= N) return;
-    const long long pitch = kt * 64;
     const unsigned char *pa[2], *pb[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {                        // rows behind the end read the last one; what they give is not stored
-        pa[t] = a + min(m0 + t * 32 + (lane & 31), M - 1) * pitch + (lane >> 5) * 16;
-        pb[t] = b + min(n0 + t * 32 + (lane & 31), N - 1) * pitch + (lane >> 5) * 16;
+        pa[t] = a + min(m0 + t * 32 + (lane & 31), M - 1) * 64 + (lane >> 5) * 16;
+        pb[t] = b + min(n0 + t * 32 + (lane & 31), N - 1) * 64 + (lane >> 5) * 16;
     }
     const unsigned *qa = sa + m0 / 64 * 64 + lane, *qb = sb + n0 / 64 * 64 + lane;
     f32x16 acc[2][2] = {};
@@ -351,8 +352,8 @@ __global__ __launch_bounds__(kThreads) void k_mx4_gemm(const unsigned char *__re
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                fa[t][h] = *reinterpret_cast<const u32x4 *>(pa[t] + k * 64 + h * 32);
-                fb[t][h] = *reinterpret_cast<const u32x4 *>(pb[t] + k * 64 + h * 32);
+                fa[t][h] = *reinterpret_cast<const u32x4 *>(pa[t] + k * M * 64 + h * 32);
+                fb[t][h] = *reinterpret_cast<const u32x4 *>(pb[t] + k * N * 64 + h * 32);
             }
 #define MX4_HALF(H)                                                                       \
         acc[0][0] = mfma<2 * H, 2 * H>(fb[0][H], fa[0][H], acc[0][0], wb, wa);            \
@@ -366,16 +367,18 @@ __global__ __launch_bounds__(kThreads) void k_mx4_gemm(const unsigned char *__re
 }
 
 // Large products: a workgroup of four waves takes a tile of 64 TM x 64 TN outputs, a wave 32 TM x 32 TN of it (TM, TN even).
-// A step is 256 columns, 128 bytes of every row: one cache line.  Its codes and scales go to LDS without passing registers while the
-// step before is worked on (two stages); the fragments of the next 64 columns are read from LDS while the matrix cores work on these.
-//   codes in LDS: 128 bytes a row, the 16-byte block b of row r at slot b ^ (r / 2 % 8): eight lanes fetch one row's line, and the 16
-//   lanes that LDS serves at once (rows 0-3, 12-15, 20-27 or 4-11, 16-19, 28-31 of a fragment) touch every bank once.
-// Per step and workgroup (TM = TN = 4): 64 matrix instructions of 32 cycles on each of four SIMDs = 2048 cycles, 128 KB of LDS reads
-// (512 cycles at 256 B per cycle) and 68 KB from the caches.
+// A step is 128 columns.  Its codes and scales go to LDS without passing registers, into a ring of four stages and up to four steps
+// ahead of their use; the fragments of the next 64 columns are read from LDS while the matrix cores work on these.  Fetches and reads
+// stand between the matrix instructions, a few behind every fourth: a wave issues in order, and a run of fetches would hold up what
+// comes behind it (measured on 8192^3: a step's fetches in one run 295 us, spread out 253).
+//   codes in LDS: 64 bytes a row, the 16-byte block b of row r at slot b ^ (r / 4 % 4): the 16 lanes that LDS serves at once (rows
+//   0-3, 12-15, 20-27 or 4-11, 16-19, 28-31 of a fragment) touch every bank once (measured: no bank conflicts).
+// Per step and workgroup (TM = TN = 4): 32 matrix instructions of 32 cycles on each of four SIMDs = 1024 cycles, 64 KB of LDS reads
+// (256 cycles at 256 B per cycle) and 34 KB from the caches.
 typedef __attribute__((address_space(3))) void *lptr;
 __device__ __forceinline__ unsigned lds_offset(const void *p) { return static_cast<unsigned>(reinterpret_cast<uintptr_t>((lptr)p)); }
 // 16 (4) bytes per lane from `src` to LDS offset `to` + 16 (4) * lane.  Written as assembly because the compiler would wait for ALL of
-// them in front of every LDS read; there is no result register, the kernel waits itself.
+// them in front of every LDS read; there is no result register, the kernel counts and waits itself.
 __device__ __forceinline__ void to_lds16(const void *src, unsigned to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(to) : "memory", "m0");
 }
@@ -385,11 +388,13 @@ __device__ __forceinline__ void to_lds4(const void *src, unsigned to) {
 
 template <int TM, int TN> struct Tile {
     static constexpr int BM = 64 * TM, BN = 64 * TN;
-    static constexpr int kCodes = (BM + BN) * 128, kWords = (BM + BN) * 4, kStage = kCodes + 2 * kWords;
-    static constexpr int kCodeLoads = (BM + BN) / 32, kWordLoads = (BM + BN) / 256;         // 1 KB pieces and pairs of 256 B pieces, per wave
+    static constexpr int kCodes = (BM + BN) * 64, kStage = kCodes + (BM + BN) * 4, kStages = 4;
+    static constexpr int kCodeLoads = (BM + BN) / 64, kWordLoads = (BM + BN) / 256;         // 1 KB and 256 B pieces per wave and step
+    static constexpr int kLoads = kCodeLoads + kWordLoads;
+    static constexpr int kGroups = TM * TN / 4;                                             // of four matrix instructions, per 64 columns
 };
 
-__device__ __forceinline__ int slot_of(int r, int b) { return b ^ (r >> 1 & 7); }
+__device__ __forceinline__ int slot_of(int r, int b) { return b ^ (r >> 2 & 3); }
 
 template <int T, int TM, int TN>
 __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const unsigned char *__restrict__ a, const unsigned *__restrict__ sa,
@@ -397,28 +402,26 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const unsigned c
                                                                 const void *__restrict__ bias, int bias_type, long long M, long long N,
                                                                 int kt, int vec, void *__restrict__ out) {
     typedef Tile<TM, TN> G;
-    __shared__ __align__(16) unsigned char lds[2 * G::kStage];
+    __shared__ __align__(16) unsigned char lds[G::kStages * G::kStage];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_m = static_cast<int>((M + G::BM - 1) / G::BM), tiles_n = static_cast<int>((N + G::BN - 1) / G::BN);
     // one XCD's workgroups walk neighbouring tiles, 8 tile rows at a time: operands meet in its L2
     const int id = dipr_xcd_contiguous(blockIdx.x, gridDim.x);
     const int group = 8 * tiles_n, first = id / group * 8, high = min(8, tiles_m - first);
     const long long m0 = static_cast<long long>(first + id % group % high) * G::BM, n0 = static_cast<long long>(id % group / high) * G::BN;
-    const long long pitch = static_cast<long long>(kt) * 64;
-    const int steps = (kt + 1) / 2;
 
-    // this lane's source addresses: code pieces of 8 rows (rows 0 .. BM - 1 of a, then BN of b), scale pieces of 64 rows.  An odd number
-    // of 128-column groups: the last step's upper half does not exist, the lower one is fetched in its place and not used.
+    // this lane's source addresses: code pieces of 16 rows (rows 0 .. BM - 1 of a, then BN of b), scale pieces of 64 rows
     const unsigned char *src[G::kCodeLoads];
+    const unsigned *ssrc[G::kWordLoads];
+    long long move[G::kCodeLoads], smove[G::kWordLoads];                // uniform: what a step moves them on by
 #pragma unroll
     for (int j = 0; j < G::kCodeLoads; ++j) {
-        const int piece = wave * G::kCodeLoads + j, r = (piece & 1) * 8 + (lane >> 3);
-        const bool of_a = piece < G::BM / 8;
-        const long long row = of_a ? min(m0 + piece * 8 + (lane >> 3), M - 1) : min(n0 + (piece - G::BM / 8) * 8 + (lane >> 3), N - 1);
-        src[j] = (of_a ? a : b) + row * pitch + slot_of(r, lane & 7) * 16;
+        const int piece = wave * G::kCodeLoads + j, r = lane >> 2;
+        const bool of_a = piece < G::BM / 16;
+        const long long row = of_a ? min(m0 + piece * 16 + r, M - 1) : min(n0 + (piece - G::BM / 16) * 16 + r, N - 1);
+        src[j] = (of_a ? a : b) + row * 64 + slot_of(r, lane & 3) * 16;
+        move[j] = (of_a ? M : N) * 64;
     }
-    const unsigned *ssrc[G::kWordLoads];
-    long long sstep[G::kWordLoads];
 #pragma unroll
     for (int j = 0; j < G::kWordLoads; ++j) {
         const int piece = wave * G::kWordLoads + j;
@@ -426,106 +429,93 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const unsigned c
         const long long groups = of_a ? row_groups(M) : row_groups(N);
         const long long g = of_a ? min(m0 / 64 + piece, groups - 1) : min(n0 / 64 + piece - G::BM / 64, groups - 1);
         ssrc[j] = (of_a ? sa : sb) + g * 64 + lane;
-        sstep[j] = groups * 64;
+        smove[j] = groups * 64;
     }
     const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds));
-    auto fetch = [&](int s) {
-        const unsigned base = lds0 + (s & 1) * G::kStage;
-        const bool half = 2 * s + 1 == kt;
-#pragma unroll
-        for (int j = 0; j < G::kCodeLoads; ++j) {
-            const int piece = wave * G::kCodeLoads + j, r = (piece & 1) * 8 + (lane >> 3);
-            const int back = half && slot_of(r, lane & 7) >= 4 ? 64 : 0;
-            to_lds16(src[j] - back, base + piece * 1024);
-            src[j] += 128;
-        }
-#pragma unroll
-        for (int j = 0; j < G::kWordLoads; ++j) {
-            const unsigned to = base + G::kCodes + (wave * G::kWordLoads + j) * 256;
-            to_lds4(ssrc[j], to);
-            to_lds4(half ? ssrc[j] : ssrc[j] + sstep[j], to + G::kWords);
-            ssrc[j] += 2 * sstep[j];
+    // piece j of step s, to its stage; the address moves on to the next step (behind the last one: the last one again, so that the number
+    // of fetches on their way is the same in every step)
+    auto fetch = [&](int s, int j) {
+        const unsigned base = lds0 + (s & 3) * G::kStage;
+        const bool on = s + 1 < kt;
+        if (j < G::kCodeLoads) {
+            to_lds16(src[j], base + (wave * G::kCodeLoads + j) * 1024);
+            src[j] += on ? move[j] : 0;
+        } else {
+            const int i = j - G::kCodeLoads;
+            to_lds4(ssrc[i], base + G::kCodes + (wave * G::kWordLoads + i) * 256);
+            ssrc[i] += on ? smove[i] : 0;
         }
     };
     const int wm = (wave >> 1) * TM, wn = (wave & 1) * TN;              // this wave's first 32-row tile of a and of b
-    int frag[4];                                                        // where this lane's block of the q-th 64 columns lies in a tile of 32 rows
-#pragma unroll
-    for (int q = 0; q < 4; ++q) frag[q] = (lane & 31) * 128 + slot_of(lane & 31, 2 * q + (lane >> 5)) * 16;
+    // where this lane's block of the first / second 64 columns lies in a tile of 32 rows
+    const int frag[2] = {(lane & 31) * 64 + slot_of(lane & 31, lane >> 5) * 16, (lane & 31) * 64 + slot_of(lane & 31, 2 + (lane >> 5)) * 16};
     struct Frags {
-        u32x4 a[TM], b[TN];
+        u32x4 b[TN], a[TM];
     };
     struct Words {
-        unsigned a[TM / 2], b[TN / 2];
+        unsigned b[TN / 2], a[TM / 2];
     };
-    auto read = [&](Frags &f, int s, int q) {
-        const unsigned char *base = lds + (s & 1) * G::kStage;
-#pragma unroll
-        for (int t = 0; t < TN; ++t) f.b[t] = *reinterpret_cast<const u32x4 *>(base + G::BM * 128 + (wn + t) * 4096 + frag[q]);
-#pragma unroll
-        for (int t = 0; t < TM; ++t) f.a[t] = *reinterpret_cast<const u32x4 *>(base + (wm + t) * 4096 + frag[q]);
+    // fragment i of the TN + TM ones
+    auto read = [&](Frags &f, int s, int h, int i) {
+        const unsigned char *base = lds + (s & 3) * G::kStage;
+        if (i < TN) f.b[i] = *reinterpret_cast<const u32x4 *>(base + G::BM * 64 + (wn + i) * 2048 + frag[h]);
+        else f.a[i - TN] = *reinterpret_cast<const u32x4 *>(base + (wm + i - TN) * 2048 + frag[h]);
     };
-    auto read_words = [&](Words &w, int s, int half) {
-        const unsigned char *base = lds + (s & 1) * G::kStage + G::kCodes + half * G::kWords;
-#pragma unroll
-        for (int t = 0; t < TN / 2; ++t) w.b[t] = reinterpret_cast<const unsigned *>(base + G::BM * 4 + (wn / 2 + t) * 256)[lane];
-#pragma unroll
-        for (int t = 0; t < TM / 2; ++t) w.a[t] = reinterpret_cast<const unsigned *>(base + (wm / 2 + t) * 256)[lane];
+    auto read_word = [&](Words &w, int s, int i) {
+        const unsigned char *base = lds + (s & 3) * G::kStage + G::kCodes;
+        if (i < TN / 2) w.b[i] = reinterpret_cast<const unsigned *>(base + G::BM * 4 + (wn / 2 + i) * 256)[lane];
+        else w.a[i - TN / 2] = reinterpret_cast<const unsigned *>(base + (wm / 2 + i - TN / 2) * 256)[lane];
     };
     f32x16 acc[TN][TM] = {};
-#define MX4_MULTIPLY(F, W, H)                                                                                                 \
-    _Pragma("unroll") for (int j = 0; j < TM; j += 2) _Pragma("unroll") for (int i = 0; i < TN; i += 2) {                     \
-        acc[i][j] = mfma<2 * H, 2 * H>(F.b[i], F.a[j], acc[i][j], W.b[i / 2], W.a[j / 2]);                                    \
-        acc[i + 1][j] = mfma<2 * H + 1, 2 * H>(F.b[i + 1], F.a[j], acc[i + 1][j], W.b[i / 2], W.a[j / 2]);                    \
-        acc[i][j + 1] = mfma<2 * H, 2 * H + 1>(F.b[i], F.a[j + 1], acc[i][j + 1], W.b[i / 2], W.a[j / 2]);                    \
-        acc[i + 1][j + 1] = mfma<2 * H + 1, 2 * H + 1>(F.b[i + 1], F.a[j + 1], acc[i + 1][j + 1], W.b[i / 2], W.a[j / 2]);    \
+    // 64 columns: H the half of the step they are; behind each group of four matrix instructions a share of the next 64 columns' reads and
+    // of the fetches FIRST .. LAST - 1 of step FS
+#define MX4_COLUMNS(F, W, H, NF, NS, NH, WORDS, NW, FS, FIRST, LAST)                                                               \
+    _Pragma("unroll") for (int g = 0; g < G::kGroups; ++g) {                                                                       \
+        const int i = g % (TN / 2) * 2, j = g / (TN / 2) * 2;                                                                      \
+        if (WORDS) {                                                                                                               \
+            _Pragma("unroll") for (int x = (TM + TN) / 2 * g / G::kGroups; x < (TM + TN) / 2 * (g + 1) / G::kGroups; ++x)          \
+                read_word(NW, NS, x);                                                                                              \
+        }                                                                                                                          \
+        _Pragma("unroll") for (int x = (TM + TN) * g / G::kGroups; x < (TM + TN) * (g + 1) / G::kGroups; ++x) read(NF, NS, NH, x); \
+        _Pragma("unroll") for (int x = FIRST + (LAST - FIRST) * g / G::kGroups; x < FIRST + (LAST - FIRST) * (g + 1) / G::kGroups; ++x) fetch(FS, x); \
+        acc[i][j] = mfma<2 * H, 2 * H>(F.b[i], F.a[j], acc[i][j], W.b[i / 2], W.a[j / 2]);                                         \
+        acc[i + 1][j] = mfma<2 * H + 1, 2 * H>(F.b[i + 1], F.a[j], acc[i + 1][j], W.b[i / 2], W.a[j / 2]);                         \
+        acc[i][j + 1] = mfma<2 * H, 2 * H + 1>(F.b[i], F.a[j + 1], acc[i][j + 1], W.b[i / 2], W.a[j / 2]);                         \
+        acc[i + 1][j + 1] = mfma<2 * H + 1, 2 * H + 1>(F.b[i + 1], F.a[j + 1], acc[i + 1][j + 1], W.b[i / 2], W.a[j / 2]);         \
+        __builtin_amdgcn_sched_barrier(0);                                                                                         \
     }
-    // one LDS read behind each of the first matrix instructions
-    auto interleave = [&](int reads) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    // waits until at most `steps` fetched steps are still on their way and everything read from LDS is here, then for all waves
+#define MX4_ARRIVED(STEPS)                                                                       \
+    do {                                                                                         \
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STEPS) * G::kLoads) : "memory");     \
+        __builtin_amdgcn_s_barrier();                                                            \
+    } while (0)
+    constexpr int kHalf = G::kLoads / 2;
 #pragma unroll
-        for (int i = 0; i < reads; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    // everything fetched is in LDS, everything read from it is in registers; for all waves
-    auto arrived = [&]() {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-    };
-    fetch(0);
+    for (int s = 0; s < 3; ++s)
+#pragma unroll
+        for (int j = 0; j < G::kLoads; ++j) fetch(s, j);
+#pragma unroll
+    for (int j = 0; j < kHalf; ++j) fetch(3, j);
     Frags f0, f1;
-    Words w0, w1;
-    arrived();
-    if (steps > 1) fetch(1);
-    read(f0, 0, 0);
-    read_words(w0, 0, 0);
-    for (int s = 0; s < kt / 2; ++s) {
-        read(f1, s, 1);
-        MX4_MULTIPLY(f0, w0, 0)
-        interleave(TM + TN);
-        read_words(w1, s, 1);
-        read(f0, s, 2);
-        MX4_MULTIPLY(f1, w0, 1)
-        interleave(TM + TN + TM / 2 + TN / 2);
-        read(f1, s, 3);
-        MX4_MULTIPLY(f0, w1, 0)
-        interleave(TM + TN);
-        // the next step is in LDS; behind the barrier every wave has read this one, whose stage is free
-        arrived();
-        if (s + 2 < steps) fetch(s + 2);
-        read_words(w0, s + 1, 0);                        // (behind the last step: what is read there is not used)
-        read(f0, s + 1, 0);
-        MX4_MULTIPLY(f1, w1, 1)
-        interleave(TM + TN + TM / 2 + TN / 2);
+    Words w, next;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * G::kLoads + kHalf) : "memory");
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int i = 0; i < TM + TN; ++i) read(f0, 0, 0, i);
+#pragma unroll
+    for (int i = 0; i < (TM + TN) / 2; ++i) read_word(w, 0, i);
+    for (int k = 0; k < kt; ++k) {
+        MX4_COLUMNS(f0, w, 0, f1, k, 1, false, next, k + 3, kHalf, G::kLoads)
+        // step k + 1 is in LDS (steps k + 2 and k + 3 may be on their way); behind the barrier every wave has read stage k & 3, which is
+        // free for step k + 4
+        MX4_ARRIVED(2);
+        MX4_COLUMNS(f1, w, 1, f0, k + 1, 0, true, next, k + 4, 0, kHalf)
+        w = next;
     }
-    if (kt & 1) {
-        read(f1, steps - 1, 1);
-        MX4_MULTIPLY(f0, w0, 0)
-        MX4_MULTIPLY(f1, w0, 1)
-    }
-#undef MX4_MULTIPLY
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // nothing may arrive in LDS behind the last use of a stage
+#undef MX4_ARRIVED
+#undef MX4_COLUMNS
 
     __syncthreads();                                     // every wave is through with the stages
     store_tiles<T, TM, TN>(acc, reinterpret_cast<float *>(lds) + wave * 32 * (32 * TN + 4), bias, bias_type, m0 + wm * 32, n0 + wn * 32, M, N, vec, out);

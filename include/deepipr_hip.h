@@ -446,7 +446,8 @@ int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const D
  * with their value.  A block that holds a NaN or an infinity gets code 255 and reads as NaN throughout; a row's last block may be
  * short: what is missing counts as zero.
  * A quantised matrix of `rows` x `cols` is two buffers, 16-byte aligned:
- *   codes   deepipr_mx4_code_bytes():  [rows][Kp / 2] bytes, Kp = cols rounded up to 128, lower index in the low half byte, zero behind cols
+ *   codes   deepipr_mx4_code_bytes():  [Kp / 128][rows][64] bytes, Kp = cols rounded up to 128: 128 columns of a row are 64 bytes, lower
+ *           index in the low half byte, zero behind cols
  *   scales  deepipr_mx4_scale_bytes(): [Kp / 128][ceil(rows / 64)][2][32][2][2] bytes: scale of block 2 h + e (0..3) of these 128 columns, for
  *           the row 32 t + r of the 64-row group, at [..][..][e][r][h][t] -- the order in which the matrix instruction's lanes take them.
  *   deepipr_mx4_quantize    x [rows][cols] (row_stride elements between rows) in one pass: blocks along the rows (row_codes / row_scales),

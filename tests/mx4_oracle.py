@@ -47,7 +47,7 @@ def values(x, dim):
 def unpack(codes, scales, rows, cols):
     """The library's buffers -> (codes [rows, cols], scale bytes [rows, blocks], whether everything behind the columns is zero)."""
     kp = -(-cols // KP) * KP
-    b = codes.cpu().numpy().reshape(rows, kp // 2)
+    b = codes.cpu().numpy().reshape(kp // KP, rows, KP // 2).transpose(1, 0, 2).reshape(rows, kp // 2)
     full = np.stack([b & 15, b >> 4], -1).reshape(rows, kp)
     rg = -(-rows // 64)
     s = scales.cpu().numpy().reshape(kp // KP, rg, 2, 32, 2, 2)    # [k128][group][block % 2][row % 32][block / 2][row / 32]
