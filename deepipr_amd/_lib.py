@@ -84,6 +84,12 @@ SIGNATURES = {
     'deepipr_mx4_dequantize': (_int, [_vp, _vp, _i64, _i64, _int, _vp, _int, _vp]),
     'deepipr_mx4_matmul_workspace_bytes': (_sz, [_i64, _i64, _i64]),
     'deepipr_mx4_matmul': (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _sz, _vp]),
+    'deepipr_mx4_linear_saved_bytes': (_sz, [_i64, _i64, _i64, _int, _int]),
+    'deepipr_mx4_linear_scratch_bytes': (_sz, [_i64, _i64, _i64, _int]),
+    'deepipr_mx4_linear_fwd': (_int, [_vp, _int, _i64, _vp, _int, _i64, _vp, _vp, _vp, _int, _i64, _i64, _i64, _int, _int, _vp, _sz,
+                                      _vp, _vp, _sz, _vp]),
+    'deepipr_mx4_linear_bwd': (_int, [_vp, _int, _i64, _i64, _i64, _i64, _int, _int, _vp, _sz, _vp, _int, _vp, _int, _f32p, _vp, _sz,
+                                      _vp]),
     'deepipr_passport_bn_workspace_bytes': (_sz, [_int, _int, _int]),
     'deepipr_passport_bn_fwd': (_int, [_f32p, _f32p, _f64p, _f32p, _f32p, _f32p, _flt, _flt, _flt, _f32p, _f32p, _vp,
                                        _flt, _flt, _int, _int, _int, _int, _int, _int, _f32p, _f32p, _f32p, _f32p,

@@ -14,7 +14,6 @@
 //           and 2 + b % 2 (of the four of these 128 columns) of the rows r % 32 and 32 + r % 32; byte 2 (b / 2) + r / 32.  That is the order
 //           in which the lanes of v_mfma_scale_f32_32x32x64_f8f6f4 take them: one coalesced 256-byte load serves 64 rows x 128 columns.
 #include <cmath>
-#include <cstdlib>
 
 #include "deepipr_host.h"
 
@@ -196,13 +195,23 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
     }
 }
 
-// sums [tiles][C] -> out [C], in tile order
+// sums [tiles][C] -> out [C]: eight threads a column, each every eighth tile in order, then the eight in order
 __global__ __launch_bounds__(kThreads) void k_mx4_colsum(const float *__restrict__ sums, long long tiles, long long C, float *__restrict__ out) {
-    const long long c = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-    if (c >= C) return;
+    __shared__ double red[8][32];
+    const int col = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const long long c = static_cast<long long>(blockIdx.x) * 32 + col;
     double v = 0.0;
-    for (long long t = 0; t < tiles; ++t) v += static_cast<double>(sums[t * C + c]);
-    out[c] = static_cast<float>(v);
+    if (c < C) {
+#pragma unroll 4
+        for (long long t = part; t < tiles; t += 8) v += static_cast<double>(sums[t * C + c]);
+    }
+    red[part][col] = v;
+    __syncthreads();
+    if (part == 0 && c < C) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) v += red[i][col];
+        out[c] = static_cast<float>(v);
+    }
 }
 
 // ----------------------------------------------------------------------------------------------------------------- dequantise
@@ -325,45 +334,120 @@ __device__ __forceinline__ void store_tiles(const f32x16 (&acc)[TN][TM], float *
     }
 }
 
-// Small products: a wave takes 64 x 64 outputs straight from the caches.
-template <int T>
-__global__ __launch_bounds__(kThreads) void k_mx4_gemm(const unsigned char *__restrict__ a, const unsigned *__restrict__ sa,
-                                                       const unsigned char *__restrict__ b, const unsigned *__restrict__ sb,
-                                                       const void *__restrict__ bias, int bias_type, long long M, long long N, long long kt,
-                                                       int vec, void *__restrict__ out) {
-    __shared__ __align__(16) float strips[4 * 32 * 68];
+struct Product {
+    const unsigned char *a, *b;                          // [kt][M][64], [kt][N][64]
+    const unsigned *sa, *sb;
+    const void *bias;
+    int bias_type, vec;
+    long long M, N;                                      // of the operands in memory
+    long long first, last;                               // rows first .. last - 1 of the output (first a multiple of 64)
+    int kt, splits;                                      // splits > 1: out is float [splits][M][N], split i adds up its share of the steps
+    void *out;
+};
+
+// Few rows (at most 16 MT): bound by reading b once.  A workgroup of eight waves takes 16 rows of b and all of a; wave i the steps
+// i, i + 8, ... of the columns, four of them on their way at once: with 16 rows a workgroup, 4096 rows of b fill 256 CUs and all
+// of b is asked for at once.  v_mfma_scale_f32_16x16x128_f8f6f4: lane l gives block l / 16 of row l % 16.  The waves' sums are added
+// through LDS in wave order.
+template <int T, int MT>
+__global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product P) {
+    constexpr int U = 4;
+    __shared__ f32x4 red[8][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long tiles_n = (N + 127) / 128;
-    const long long m0 = static_cast<long long>(blockIdx.x) / tiles_n * 128 + (wave >> 1) * 64;
-    const long long n0 = static_cast<long long>(blockIdx.x) % tiles_n * 128 + (wave & 1) * 64;
-    if (m0 >= M || n0 >= N) return;
-    const unsigned char *pa[2], *pb[2];
+    const long long n0 = static_cast<long long>(blockIdx.x) * 16;
+    const int r = lane & 15, blk = lane >> 4;
+    // the byte of a scale word that holds this lane's block for a row: (block / 2, row / 32)
+    const auto word_of = [&](long long row) { return row / 64 * 64 + (blk & 1) * 32 + (row & 31); };
+    const auto byte_of = [&](long long row) { return static_cast<int>((blk >> 1) * 2 + (row >> 5 & 1)) * 8; };
+    const long long brow = min(n0 + r, P.N - 1);
+    const unsigned char *pb = P.b + brow * 64 + blk * 16, *pa[MT];
+    const unsigned *qb = P.sb + word_of(brow), *qa[MT];
+    const int hb = byte_of(brow);
+    int ha[MT];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {                        // rows behind the end read the last one; what they give is not stored
-        pa[t] = a + min(m0 + t * 32 + (lane & 31), M - 1) * 64 + (lane >> 5) * 16;
-        pb[t] = b + min(n0 + t * 32 + (lane & 31), N - 1) * 64 + (lane >> 5) * 16;
+    for (int t = 0; t < MT; ++t) {
+        const long long row = min(P.first + t * 16 + r, P.last - 1);
+        pa[t] = P.a + row * 64 + blk * 16;
+        qa[t] = P.sa + word_of(row);
+        ha[t] = byte_of(row);
     }
-    const unsigned *qa = sa + m0 / 64 * 64 + lane, *qb = sb + n0 / 64 * 64 + lane;
-    f32x16 acc[2][2] = {};
-    for (long long k = 0; k < kt; ++k) {
-        u32x4 fa[2][2], fb[2][2];
-        const unsigned wa = qa[k * row_groups(M) * 64], wb = qb[k * row_groups(N) * 64];
+    const long long gm = row_groups(P.M) * 64, gn = row_groups(P.N) * 64;
+    f32x4 acc[MT] = {};
+    for (int k0 = wave; k0 < P.kt; k0 += 8 * U) {
+        u32x4 fb[U], fa[U][MT];
+        unsigned wb[U], wa[U][MT];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int u = 0; u < U; ++u) {
+            const long long k = min(k0 + 8 * u, P.kt - 1);
+            fb[u] = *reinterpret_cast<const u32x4 *>(pb + k * P.N * 64);
+            wb[u] = qb[k * gn];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                fa[t][h] = *reinterpret_cast<const u32x4 *>(pa[t] + k * M * 64 + h * 32);
-                fb[t][h] = *reinterpret_cast<const u32x4 *>(pb[t] + k * N * 64 + h * 32);
+            for (int t = 0; t < MT; ++t) {
+                fa[u][t] = *reinterpret_cast<const u32x4 *>(pa[t] + k * P.M * 64);
+                wa[u][t] = qa[t][k * gm];
             }
-#define MX4_HALF(H)                                                                       \
-        acc[0][0] = mfma<2 * H, 2 * H>(fb[0][H], fa[0][H], acc[0][0], wb, wa);            \
-        acc[1][0] = mfma<2 * H + 1, 2 * H>(fb[1][H], fa[0][H], acc[1][0], wb, wa);        \
-        acc[0][1] = mfma<2 * H, 2 * H + 1>(fb[0][H], fa[1][H], acc[0][1], wb, wa);        \
-        acc[1][1] = mfma<2 * H + 1, 2 * H + 1>(fb[1][H], fa[1][H], acc[1][1], wb, wa);
-        MX4_HALF(0) MX4_HALF(1)
-#undef MX4_HALF
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + 8 * u >= P.kt) break;
+            const i32x8 bv = {static_cast<int>(fb[u].x), static_cast<int>(fb[u].y), static_cast<int>(fb[u].z), static_cast<int>(fb[u].w), 0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const i32x8 av = {static_cast<int>(fa[u][t].x), static_cast<int>(fa[u][t].y), static_cast<int>(fa[u][t].z),
+                                  static_cast<int>(fa[u][t].w), 0, 0, 0, 0};
+                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv, av, acc[t], 4, 4, 0, static_cast<int>(wb[u] >> hb), 0,
+                                                                          static_cast<int>(wa[u][t] >> ha[t]));
+            }
+        }
     }
-    store_tiles<T, 2, 2>(acc, strips + wave * 32 * 68, bias, bias_type, m0, n0, M, N, vec, out);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+    __syncthreads();
+    if (wave >= MT) return;
+    f32x4 v = red[0][wave][lane];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += red[i][wave][lane];
+    const long long m = P.first + wave * 16 + r, n = n0 + blk * 4;
+    if (m >= P.last) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (P.bias && n + j < P.N) v[j] += bias_at(P.bias, P.bias_type, n + j);
+    if (P.vec && n + 4 <= P.N) {
+        store4<T>(element<T>(P.out, m * P.N + n), v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < P.N) store1<T>(P.out, m * P.N + n + j, v[j]);
+    }
+}
+
+// The splits' sums, in order: out [M][N] = sum_i part[i][M][N] + bias
+template <int T>
+__global__ __launch_bounds__(kThreads) void k_mx4_gemm_sum(const float *__restrict__ part, int splits, const void *__restrict__ bias, int bias_type,
+                                                           long long M, long long N, int vec, void *__restrict__ out) {
+    const long long per = (N + 3) / 4, n = M * per;
+    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads) {
+        const long long row = i / per, c = i % per * 4, at = row * N + c;
+        f32x4 v = {};
+        if (vec) {
+            for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4 *>(part + s * M * N + at);
+        } else {
+            for (int s = 0; s < splits; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < N) v[j] += part[s * M * N + at + j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (bias && c + j < N) v[j] += bias_at(bias, bias_type, c + j);
+        if (vec) {
+            store4<T>(element<T>(out, at), v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < N) store1<T>(out, at + j, v[j]);
+        }
+    }
 }
 
 // Large products: a workgroup of four waves takes a tile of 64 TM x 64 TN outputs, a wave 32 TM x 32 TN of it (TM, TN even).
@@ -397,18 +481,22 @@ template <int TM, int TN> struct Tile {
 __device__ __forceinline__ int slot_of(int r, int b) { return b ^ (r >> 2 & 3); }
 
 template <int T, int TM, int TN>
-__global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const unsigned char *__restrict__ a, const unsigned *__restrict__ sa,
-                                                                const unsigned char *__restrict__ b, const unsigned *__restrict__ sb,
-                                                                const void *__restrict__ bias, int bias_type, long long M, long long N,
-                                                                int kt, int vec, void *__restrict__ out) {
+__global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P) {
     typedef Tile<TM, TN> G;
     __shared__ __align__(16) unsigned char lds[G::kStages * G::kStage];
+    const long long M = P.M, N = P.N;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tiles_m = static_cast<int>((M + G::BM - 1) / G::BM), tiles_n = static_cast<int>((N + G::BN - 1) / G::BN);
+    const int tiles_m = static_cast<int>((P.last - P.first + G::BM - 1) / G::BM), tiles_n = static_cast<int>((N + G::BN - 1) / G::BN);
     // one XCD's workgroups walk neighbouring tiles, 8 tile rows at a time: operands meet in its L2
-    const int id = dipr_xcd_contiguous(blockIdx.x, gridDim.x);
+    const int all = dipr_xcd_contiguous(blockIdx.x, gridDim.x), split = all / (tiles_m * tiles_n), id = all % (tiles_m * tiles_n);
     const int group = 8 * tiles_n, first = id / group * 8, high = min(8, tiles_m - first);
-    const long long m0 = static_cast<long long>(first + id % group % high) * G::BM, n0 = static_cast<long long>(id % group / high) * G::BN;
+    const long long m0 = P.first + static_cast<long long>(first + id % group % high) * G::BM;
+    const long long n0 = static_cast<long long>(id % group / high) * G::BN;
+    const int k_first = static_cast<int>(static_cast<long long>(P.kt) * split / P.splits);
+    const int kt = static_cast<int>(static_cast<long long>(P.kt) * (split + 1) / P.splits) - k_first;
+    const unsigned char *a = P.a + k_first * M * 64, *b = P.b + k_first * N * 64;
+    const unsigned *sa = P.sa + k_first * row_groups(M) * 64, *sb = P.sb + k_first * row_groups(N) * 64;
+    void *out = P.splits > 1 ? static_cast<float *>(P.out) + split * M * N : P.out;
 
     // this lane's source addresses: code pieces of 16 rows (rows 0 .. BM - 1 of a, then BN of b), scale pieces of 64 rows
     const unsigned char *src[G::kCodeLoads];
@@ -518,7 +606,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const unsigned c
 #undef MX4_COLUMNS
 
     __syncthreads();                                     // every wave is through with the stages
-    store_tiles<T, TM, TN>(acc, reinterpret_cast<float *>(lds) + wave * 32 * (32 * TN + 4), bias, bias_type, m0 + wm * 32, n0 + wn * 32, M, N, vec, out);
+    store_tiles<T, TM, TN>(acc, reinterpret_cast<float *>(lds) + wave * 32 * (32 * TN + 4), P.bias, P.bias_type, m0 + wm * 32, n0 + wn * 32,
+                           P.last, N, P.vec, out);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host side
@@ -542,6 +631,202 @@ void launch_quantise(DiprProf &prof, const void *x, long long R, long long C, lo
     else if (cc) MX4_QUANTISE(false, true, false);
     else MX4_QUANTISE(true, false, false);
 #undef MX4_QUANTISE
+}
+
+
+// ---- which kernels a product takes
+// Times of one step of 128 columns and of a tile's begin and end, in ns, as measured (8192^2 x {128, 8192, 16384}, 8200 x 4096 x 4096):
+// 256 x 256 tiles, one a CU, 780 and 6 000; 128 x 128 tiles, two a CU, 690 and 3 000.
+struct Plan {
+    enum { kRows, kSmall, kLarge } form;
+    int splits;                  // kSmall only
+    long long tail;              // rows at the end that go to the kernel for few rows (0: none)
+};
+inline long long tiles_of(long long m, long long n, int side) { return ((m + side - 1) / side) * ((n + side - 1) / side); }
+inline int cu_count() {
+    const int n = dipr_device_cu_count();
+    return n > 0 ? n : 256;
+}
+inline double large_ns(long long m, long long n, long long kt) {
+    const long long rounds = (tiles_of(m, n, 256) + cu_count() - 1) / cu_count();
+    return static_cast<double>(rounds) * (780.0 * kt + 6000.0);
+}
+inline double small_ns(long long m, long long n, long long kt) {
+    const double rounds = static_cast<double>(tiles_of(m, n, 128)) / (2 * cu_count());
+    return (rounds < 1.0 ? 1.0 : rounds) * (690.0 * kt + 3000.0);
+}
+Plan plan(long long M, long long N, long long kt) {
+    Plan p = {Plan::kRows, 1, 0};
+    if (M <= 64) return p;
+    // a few rows behind whole tiles: a tile row of its own for them would cost a round
+    const long long tail = M % 256 <= 64 && M > 256 ? M % 256 : 0;
+    double best = large_ns(M, N, kt);
+    p.form = Plan::kLarge;
+    if (tail) {
+        const double t = large_ns(M - tail, N, kt) + 5000.0 + 0.2 * static_cast<double>(N * kt) / 16.0;
+        if (t < best) best = t, p.tail = tail;
+    }
+    if (small_ns(M, N, kt) < best) {
+        p.form = Plan::kSmall;
+        p.tail = 0;
+        // tiles that leave slots free share the columns out instead: the partial sums cost a second launch
+        const long long tiles = tiles_of(M, N, 128), slots = 2 * cu_count();
+        long long splits = slots / tiles;
+        if (splits > kt / 4) splits = kt / 4;
+        if (splits > 16) splits = 16;
+        if (splits > 1) p.splits = static_cast<int>(splits);
+    }
+    return p;
+}
+
+template <int T> void launch_product(DiprProf &prof, const Plan &plan, Product P, float *part, hipStream_t st) {
+    const dim3 block(kThreads);
+    if (plan.form == Plan::kRows || plan.tail) {
+        Product Q = P;
+        Q.first = plan.tail ? P.M - plan.tail : 0;
+        const dim3 grid(static_cast<unsigned>((P.N + 15) / 16));
+        const long long rows = Q.last - Q.first;
+        if (rows <= 16) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 1>), grid, dim3(512), st, Q);
+        else if (rows <= 32) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 2>), grid, dim3(512), st, Q);
+        else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4>), grid, dim3(512), st, Q);
+        if (plan.form == Plan::kRows) return;
+        P.last -= plan.tail;
+    }
+    if (plan.form == Plan::kLarge) {
+        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 4, 4>), dim3(static_cast<unsigned>(tiles_of(P.last, P.N, 256))), block, st, P);
+        return;
+    }
+    const unsigned tiles = static_cast<unsigned>(tiles_of(P.last, P.N, 128));
+    if (plan.splits == 1) {
+        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 2, 2>), dim3(tiles), block, st, P);
+        return;
+    }
+    Product Q = P;
+    Q.splits = plan.splits;
+    Q.out = part;
+    Q.bias = nullptr;
+    Q.vec = P.N % 4 == 0;
+    DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<F32, 2, 2>), dim3(tiles * plan.splits), block, st, Q);
+    const long long want = (P.M * ((P.N + 3) / 4) + kThreads - 1) / kThreads;
+    hipLaunchKernelGGL((k_mx4_gemm_sum<T>), dim3(static_cast<unsigned>(want < 8192 ? want : 8192)), block, 0, st, part, plan.splits, P.bias, P.bias_type,
+                       P.M, P.N, P.vec, P.out);
+}
+
+// ---- the pieces that the C entries share; arguments are checked by then
+void quantise(const void *x, int dtype, long long R, long long C, long long stride, void *rc, void *rs, void *cc, void *cs, float *col_sums,
+              void *workspace, hipStream_t st) {
+    const int vec = aligned(x, 16) && (R == 1 || stride * elem_bytes(dtype) % 16 == 0);
+    float *sums = col_sums ? static_cast<float *>(workspace) : nullptr;
+    DiprProf prof(DEEPIPR_K_MX4_QUANTIZE);
+    prof.bytes = static_cast<double>(R) * static_cast<double>(C) * (elem_bytes(dtype) + 0.53125 * ((rc ? 1 : 0) + (cc ? 1 : 0)));
+    switch (dtype) {
+        case F32: launch_quantise<F32>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
+        case BF16: launch_quantise<BF16>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
+        default: launch_quantise<F16>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
+    }
+    if (col_sums)
+        hipLaunchKernelGGL(k_mx4_colsum, dim3(static_cast<unsigned>((C + 31) / 32)), dim3(kThreads), 0, st, sums, round_up(R, 128) / kQR, C, col_sums);
+}
+inline bool quantise_fits(long long R, long long C) {
+    return R <= kMaxSide && C <= kMaxSide && round_up(R, 128) / kQR * ((C + kQC - 1) / kQC) <= kMaxGrid;
+}
+inline bool product_fits(long long M, long long N, long long K) {
+    return M <= kMaxSide && N <= kMaxSide && K <= kMaxSide && tiles_of(M, N, 128) <= kMaxGrid / 16 && (N + 15) / 16 <= kMaxGrid &&
+           round_up(K, 128) / 128 <= kMaxGrid;
+}
+inline size_t product_bytes(long long M, long long N, long long K) {
+    const Plan p = plan(M, N, round_up(K, 128) / 128);
+    return p.splits > 1 ? static_cast<size_t>(p.splits) * static_cast<size_t>(M) * static_cast<size_t>(N) * sizeof(float) : 0;
+}
+void product(const void *a, const void *sa, const void *b, const void *sb, const void *bias, int bias_dtype, long long M, long long N, long long K,
+             void *out, int dtype, void *workspace, hipStream_t st) {
+    const long long steps = round_up(K, 128) / 128;
+    Product P;
+    P.a = static_cast<const unsigned char *>(a);
+    P.b = static_cast<const unsigned char *>(b);
+    P.sa = static_cast<const unsigned *>(sa);
+    P.sb = static_cast<const unsigned *>(sb);
+    P.bias = bias;
+    P.bias_type = bias_dtype;
+    P.vec = N % 4 == 0 && aligned(out, 4 * elem_bytes(dtype));
+    P.M = P.last = M;
+    P.N = N;
+    P.first = 0;
+    P.kt = static_cast<int>(steps);
+    P.splits = 1;
+    P.out = out;
+    const Plan p = plan(M, N, steps);
+    DiprProf prof(DEEPIPR_K_MX4_MATMUL);
+    prof.bytes = 2.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+    switch (dtype) {
+        case F32: launch_product<F32>(prof, p, P, static_cast<float *>(workspace), st); break;
+        case BF16: launch_product<BF16>(prof, p, P, static_cast<float *>(workspace), st); break;
+        default: launch_product<F16>(prof, p, P, static_cast<float *>(workspace), st); break;
+    }
+}
+
+// Cuts one buffer into pieces of whole 256-byte units.
+struct Cut {
+    char *base;
+    size_t used = 0;
+    explicit Cut(const void *p) : base(static_cast<char *>(const_cast<void *>(p))) {}
+    void *take(size_t bytes) {
+        void *p = base ? base + used : nullptr;
+        used += static_cast<size_t>(round_up(static_cast<long long>(bytes), 256));
+        return p;
+    }
+};
+struct Quantised {
+    void *codes = nullptr, *scales = nullptr;
+};
+Quantised take_matrix(Cut &c, long long rows, long long cols) {
+    Quantised q;
+    q.codes = c.take(deepipr_mx4_code_bytes(rows, cols));
+    q.scales = c.take(deepipr_mx4_scale_bytes(rows, cols));
+    return q;
+}
+struct Saved {                   // what a forward pass leaves for its backward pass: blocks along the rows of the batch / the output features
+    Quantised x_t, w_t;
+    size_t bytes;
+    Saved(const void *p, long long M, long long N, long long K, bool dx, bool dw) {
+        Cut c(p);
+        if (dw) x_t = take_matrix(c, K, M);
+        if (dx) w_t = take_matrix(c, K, N);
+        bytes = c.used;
+    }
+};
+struct ForwardScratch {
+    Quantised x, w;
+    void *work;
+    size_t bytes;
+    ForwardScratch(void *p, long long M, long long N, long long K) {
+        Cut c(p);
+        x = take_matrix(c, M, K);
+        w = take_matrix(c, N, K);
+        work = c.take(product_bytes(M, N, K));
+        bytes = c.used;
+    }
+};
+struct BackwardScratch {
+    Quantised y, y_t;
+    void *sums, *work;
+    size_t bytes;
+    BackwardScratch(void *p, long long M, long long N, long long K) {
+        Cut c(p);
+        y = take_matrix(c, M, N);
+        y_t = take_matrix(c, N, M);
+        sums = c.take(static_cast<size_t>(round_up(M, 128) / kQR) * static_cast<size_t>(N) * sizeof(float));
+        const size_t dx = product_bytes(M, K, N), dw = product_bytes(N, K, M);       // one after the other
+        work = c.take(dx > dw ? dx : dw);
+        bytes = c.used;
+    }
+};
+inline bool linear_fits(long long M, long long N, long long K) {
+    return M > 0 && N > 0 && K > 0 && quantise_fits(M, K) && quantise_fits(N, K) && quantise_fits(M, N) && product_fits(M, N, K) &&
+           product_fits(M, K, N) && product_fits(N, K, M);
+}
+inline bool good_matrix(const void *p, int dtype, long long rows, long long cols, long long stride) {
+    return p && good_dtype(dtype) && aligned(p, elem_bytes(dtype)) && (rows <= 1 || stride >= cols);
 }
 
 }  // namespace
@@ -569,21 +854,8 @@ int deepipr_mx4_quantize(const void *x, int dtype, long long rows, long long col
         return dipr_fail(DEEPIPR_EINVAL, "%s: column sums need the column direction and a workspace", what);
     if (!aligned(x, elem_bytes(dtype)) || !aligned(row_codes, 16) || !aligned(row_scales, 16) || !aligned(col_codes, 16) || !aligned(col_scales, 16))
         return dipr_fail(DEEPIPR_EINVAL, "%s: misaligned pointer", what);
-    const long long tiles = round_up(rows, 128) / kQR * ((cols + kQC - 1) / kQC);
-    if (tiles > kMaxGrid) return dipr_fail(DEEPIPR_EINVAL, "%s: matrix too large", what);
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    const int vec = aligned(x, 16) && (rows == 1 || row_stride * elem_bytes(dtype) % 16 == 0);
-    float *sums = col_sums ? static_cast<float *>(workspace) : nullptr;
-    DiprProf prof(DEEPIPR_K_MX4_QUANTIZE);
-    prof.bytes = static_cast<double>(rows) * static_cast<double>(cols) * (elem_bytes(dtype) + 0.53125 * ((row_codes ? 1 : 0) + (col_codes ? 1 : 0)));
-    switch (dtype) {
-        case F32: launch_quantise<F32>(prof, x, rows, cols, row_stride, vec, row_codes, row_scales, col_codes, col_scales, sums, st); break;
-        case BF16: launch_quantise<BF16>(prof, x, rows, cols, row_stride, vec, row_codes, row_scales, col_codes, col_scales, sums, st); break;
-        default: launch_quantise<F16>(prof, x, rows, cols, row_stride, vec, row_codes, row_scales, col_codes, col_scales, sums, st); break;
-    }
-    if (col_sums)
-        hipLaunchKernelGGL(k_mx4_colsum, dim3(static_cast<unsigned>((cols + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, sums,
-                           round_up(rows, 128) / kQR, cols, col_sums);
+    if (!quantise_fits(rows, cols)) return dipr_fail(DEEPIPR_EINVAL, "%s: matrix too large", what);
+    quantise(x, dtype, rows, cols, row_stride, row_codes, row_scales, col_codes, col_scales, col_sums, workspace, static_cast<hipStream_t>(stream));
     return dipr_check_launch(what);
 }
 
@@ -620,49 +892,73 @@ int deepipr_mx4_dequantize(const void *codes, const void *scales, long long rows
     return dipr_check_launch(what);
 }
 
-size_t deepipr_mx4_matmul_workspace_bytes(long long, long long, long long) { return 0; }
+size_t deepipr_mx4_matmul_workspace_bytes(long long M, long long N, long long K) {
+    return M <= 0 || N <= 0 || K <= 0 || !product_fits(M, N, K) ? 0 : product_bytes(M, N, K);
+}
 
 int deepipr_mx4_matmul(const void *a_codes, const void *a_scales, const void *b_codes, const void *b_scales, const void *bias, int bias_dtype,
                        long long M, long long N, long long K, void *out, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
     const char *what = "mx4_matmul";
-    if (!a_codes || !a_scales || !b_codes || !b_scales || !out || !good_dtype(dtype) || (bias && !good_dtype(bias_dtype)) || M <= 0 || N <= 0 ||
-        K <= 0 || M > kMaxSide || N > kMaxSide || K > kMaxSide)
+    if (!a_codes || !a_scales || !b_codes || !b_scales || !out || !good_dtype(dtype) || (bias && !good_dtype(bias_dtype)) || M <= 0 || N <= 0 || K <= 0)
         return dipr_fail(DEEPIPR_EINVAL, "%s: bad argument", what);
     if (!aligned(a_codes, 16) || !aligned(a_scales, 16) || !aligned(b_codes, 16) || !aligned(b_scales, 16) || !aligned(out, elem_bytes(dtype)) ||
         (bias && !aligned(bias, elem_bytes(bias_dtype))))
         return dipr_fail(DEEPIPR_EINVAL, "%s: misaligned pointer", what);
-    if (workspace_bytes < deepipr_mx4_matmul_workspace_bytes(M, N, K) || (!workspace && deepipr_mx4_matmul_workspace_bytes(M, N, K)))
-        return dipr_fail(DEEPIPR_EINVAL, "%s: workspace too small", what);
-    const long long tiles = ((M + 127) / 128) * ((N + 127) / 128);
-    const long long steps = round_up(K, 128) / 128;
-    if (tiles > kMaxGrid || steps > kMaxGrid) return dipr_fail(DEEPIPR_EINVAL, "%s: matrix too large", what);
+    if (!product_fits(M, N, K)) return dipr_fail(DEEPIPR_EINVAL, "%s: matrix too large", what);
+    const size_t need = product_bytes(M, N, K);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return dipr_fail(DEEPIPR_EINVAL, "%s: workspace too small or misaligned", what);
+    product(a_codes, a_scales, b_codes, b_scales, bias, bias_dtype, M, N, K, out, dtype, workspace, static_cast<hipStream_t>(stream));
+    return dipr_check_launch(what);
+}
+
+size_t deepipr_mx4_linear_saved_bytes(long long M, long long N, long long K, int need_dx, int need_dw) {
+    return M <= 0 || N <= 0 || K <= 0 ? 0 : Saved(nullptr, M, N, K, need_dx != 0, need_dw != 0).bytes;
+}
+size_t deepipr_mx4_linear_scratch_bytes(long long M, long long N, long long K, int backward) {
+    if (!linear_fits(M, N, K)) return 0;
+    return backward ? BackwardScratch(nullptr, M, N, K).bytes : ForwardScratch(nullptr, M, N, K).bytes;
+}
+
+int deepipr_mx4_linear_fwd(const void *x, int x_dtype, long long x_stride, const void *w, int w_dtype, long long w_stride, const void *w_codes,
+                           const void *w_scales, const void *bias, int bias_dtype, long long M, long long N, long long K, int need_dx, int need_dw,
+                           void *saved, size_t saved_bytes, void *out, void *scratch, size_t scratch_bytes, void *stream) {
+    const char *what = "mx4_linear_fwd";
+    if (!linear_fits(M, N, K)) return dipr_fail(DEEPIPR_EINVAL, "%s: bad or too large sizes", what);
+    const bool kept = !w;
+    if (!good_matrix(x, x_dtype, M, K, x_stride) || (!kept && !good_matrix(w, w_dtype, N, K, w_stride)) || !out || !aligned(out, elem_bytes(x_dtype)) ||
+        (kept && (!w_codes || !w_scales || !aligned(w_codes, 16) || !aligned(w_scales, 16) || need_dx || need_dw)) ||
+        (bias && (!good_dtype(bias_dtype) || !aligned(bias, elem_bytes(bias_dtype)))))
+        return dipr_fail(DEEPIPR_EINVAL, "%s: bad argument", what);
+    const Saved s(saved, M, N, K, need_dx != 0, need_dw != 0);
+    const ForwardScratch f(scratch, M, N, K);
+    if (!scratch || !aligned(scratch, 16) || scratch_bytes < f.bytes || (s.bytes && (!saved || !aligned(saved, 16) || saved_bytes < s.bytes)))
+        return dipr_fail(DEEPIPR_EINVAL, "%s: scratch or saved memory too small or misaligned", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int vec = N % 4 == 0 && aligned(out, 4 * elem_bytes(dtype));
-    DiprProf prof(DEEPIPR_K_MX4_MATMUL);
-    prof.bytes = 2.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
-    const unsigned char *a = static_cast<const unsigned char *>(a_codes), *b = static_cast<const unsigned char *>(b_codes);
-    const unsigned *sa = static_cast<const unsigned *>(a_scales), *sb = static_cast<const unsigned *>(b_scales);
-    const long long big = ((M + 255) / 256) * ((N + 255) / 256);
-    int form = big >= 128 ? 2 : tiles >= 64 ? 1 : 0;
-    if (getenv("MX4_FORM")) form = atoi(getenv("MX4_FORM"));
-#define MX4_GEMM(T)                                                                                                                  \
-    do {                                                                                                                             \
-        if (form == 2)                                                                                                               \
-            DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 4, 4>), dim3(static_cast<unsigned>(big)), dim3(kThreads), st, a, sa, b, sb, bias, bias_dtype, M, \
-                        N, static_cast<int>(steps), vec, out);                                                                       \
-        else if (form == 1)                                                                                                          \
-            DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 2, 2>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), st, a, sa, b, sb, bias, bias_dtype, \
-                        M, N, static_cast<int>(steps), vec, out);                                                                    \
-        else                                                                                                                         \
-            DIPR_LAUNCH(prof, (k_mx4_gemm<T>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), st, a, sa, b, sb, bias, bias_dtype, M, N, steps, \
-                        vec, out);                                                                                                   \
-    } while (0)
-    switch (dtype) {
-        case F32: MX4_GEMM(F32); break;
-        case BF16: MX4_GEMM(BF16); break;
-        default: MX4_GEMM(F16); break;
-    }
-#undef MX4_GEMM
+    quantise(x, x_dtype, M, K, x_stride, f.x.codes, f.x.scales, s.x_t.codes, s.x_t.scales, nullptr, nullptr, st);
+    if (!kept) quantise(w, w_dtype, N, K, w_stride, f.w.codes, f.w.scales, s.w_t.codes, s.w_t.scales, nullptr, nullptr, st);
+    product(f.x.codes, f.x.scales, kept ? w_codes : f.w.codes, kept ? w_scales : f.w.scales, bias, bias_dtype, M, N, K, out, x_dtype, f.work, st);
+    return dipr_check_launch(what);
+}
+
+int deepipr_mx4_linear_bwd(const void *dy, int dy_dtype, long long dy_stride, long long M, long long N, long long K, int need_dx, int need_dw,
+                           const void *saved, size_t saved_bytes, void *dx, int dx_dtype, void *dw, int dw_dtype, float *dbias, void *scratch,
+                           size_t scratch_bytes, void *stream) {
+    const char *what = "mx4_linear_bwd";
+    if (!linear_fits(M, N, K)) return dipr_fail(DEEPIPR_EINVAL, "%s: bad or too large sizes", what);
+    if (!good_matrix(dy, dy_dtype, M, N, dy_stride) || (dx && (!need_dx || !good_dtype(dx_dtype) || !aligned(dx, elem_bytes(dx_dtype)))) ||
+        (dw && (!need_dw || !good_dtype(dw_dtype) || !aligned(dw, elem_bytes(dw_dtype)))) || !aligned(dbias, 4) || (!dx && !dw && !dbias))
+        return dipr_fail(DEEPIPR_EINVAL, "%s: bad argument", what);
+    const Saved s(saved, M, N, K, need_dx != 0, need_dw != 0);
+    const BackwardScratch b(scratch, M, N, K);
+    if (!scratch || !aligned(scratch, 16) || scratch_bytes < b.bytes || (s.bytes && (!saved || !aligned(saved, 16) || saved_bytes < s.bytes)))
+        return dipr_fail(DEEPIPR_EINVAL, "%s: scratch or saved memory too small or misaligned", what);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool down = dw || dbias;
+    quantise(dy, dy_dtype, M, N, dy_stride, dx ? b.y.codes : nullptr, dx ? b.y.scales : nullptr, down ? b.y_t.codes : nullptr,
+             down ? b.y_t.scales : nullptr, dbias, b.sums, st);
+    if (dx) product(b.y.codes, b.y.scales, s.w_t.codes, s.w_t.scales, nullptr, 0, M, K, N, dx, dx_dtype, b.work, st);
+    if (dw) product(b.y_t.codes, b.y_t.scales, s.x_t.codes, s.x_t.scales, nullptr, 0, N, K, M, dw, dw_dtype, b.work, st);
     return dipr_check_launch(what);
 }
 

@@ -134,35 +134,36 @@ def matmul(a, b, bias=None, dtype=torch.float32):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias):
-        need_dx, need_dw = ctx.needs_input_grad[:2]
+        need_dx, need_dw, _ = ctx.needs_input_grad
         (m, k), n = x.shape, w.shape[0]
-        if m and n and k:
-            xq, xt, _ = P.kernels.mx4_quantize(x, True, need_dw)
-            wq, wt, _ = P.kernels.mx4_quantize(w, True, need_dx)
-        else:
-            xq = xt = wq = wt = (None, None)
         ctx.dims, ctx.types = (m, n, k), (x.dtype, w.dtype, None if bias is None else bias.dtype)
-        ctx.save_for_backward(*(xt or (None, None)), *(wt or (None, None)))
-        return _product(xq, wq, m, n, k, _bias_of(bias, n), x.dtype, x)
+        b = _bias_of(bias, n)
+        if m == 0 or n == 0 or k == 0:
+            ctx.save_for_backward(None)
+            return _product(None, None, m, n, k, b, x.dtype, x)
+        y, saved = P.kernels.mx4_linear_fwd(x, w, None, b, need_dx, need_dw)
+        ctx.save_for_backward(saved)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         (m, n, k), (xtype, wtype, btype) = ctx.dims, ctx.types
-        xc, xs, wc, ws = ctx.saved_tensors
+        saved, = ctx.saved_tensors
         need_dx, need_dw, need_db = ctx.needs_input_grad
-        if not (m and n and k):
+        if m == 0 or n == 0 or k == 0:
             zero = lambda *s, dtype: torch.zeros(s, dtype=dtype, device=dy.device)
             return (zero(m, k, dtype=xtype) if need_dx else None, zero(n, k, dtype=wtype) if need_dw else None,
                     dy.sum(0, dtype=torch.float32).to(btype) if need_db else None)
-        if not (dy.stride(1) == 1 and dy.stride(0) >= n) and not dy.is_contiguous():
+        if not _rows_ok(dy):
             dy = dy.contiguous()                             # e.g. the expanded gradient of a sum
-        a, b, sums = None, None, None
-        if need_dx or need_dw or need_db:
-            a, b, sums = P.kernels.mx4_quantize(dy, need_dx, need_dw or need_db, need_db)
-        dx = _product(a, (wc, ws), m, k, n, None, xtype, dy) if need_dx else None
-        dw = _product(b, (xc, xs), n, k, m, None, wtype, dy) if need_dw else None
-        return dx, dw, (sums.to(btype) if need_db else None)
+        dx, dw, db = P.kernels.mx4_linear_bwd(dy, saved, k, need_dx, need_dw, xtype, wtype, need_db)
+        return dx, dw, (db.to(btype) if need_db else None)
+
+
+def _rows_ok(x):
+    """Rows of contiguous elements that do not overlap."""
+    return (x.stride(1) == 1 or x.shape[1] <= 1) and (x.stride(0) >= x.shape[1] or x.shape[0] <= 1)
 
 
 def linear(x, weight, bias=None):
@@ -181,18 +182,17 @@ def linear(x, weight, bias=None):
     if bias is not None and bias.shape != (n,):
         raise ValueError('mx4: the bias has shape %s, not (%d,)' % (tuple(bias.shape), n))
     rows = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), k)
-    if rows.numel() and not (rows.stride(1) == 1 or k == 1) or rows.shape[0] > 1 and rows.stride(0) < k:
+    if not _rows_ok(rows):
         rows = rows.contiguous()
     if kept:
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise RuntimeError('mx4.linear: a weight kept in 4 bits has no backward pass; pass the float weight, or use torch.no_grad()')
-        rows = rows.detach()
-        if rows.shape[0] and n and k:
-            xq, _, _ = P.kernels.mx4_quantize(rows, True, False)
-            y = P.kernels.mx4_matmul(xq, (weight.codes, weight.scales), rows.shape[0], n, k, _bias_of(bias, n), x.dtype)
+        m = rows.shape[0]
+        if m == 0 or n == 0 or k == 0:
+            P.kernels._mx4_chk('mx4_linear', rows, weight.codes, bias)
+            y = _product(None, None, m, n, k, _bias_of(bias, n), x.dtype, rows)
         else:
-            y = _product(None, None, rows.shape[0], n, k, _bias_of(bias, n), x.dtype, rows)
+            y, _ = P.kernels.mx4_linear_fwd(rows.detach(), None, (weight.codes, weight.scales, n), _bias_of(bias, n), False, False)
     else:
-        w = weight if weight.stride(1) == 1 and weight.stride(0) >= k or weight.numel() == 0 else weight.contiguous()
-        y = _Linear.apply(rows, w, bias)
+        y = _Linear.apply(rows, weight if _rows_ok(weight) else weight.contiguous(), bias)
     return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (n,))

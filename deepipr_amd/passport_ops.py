@@ -1083,6 +1083,46 @@ class HipKernels:
                                               nbytes, _stream(dev)), 'mx4_matmul')
         return out
 
+    def mx4_linear_fwd(self, x, w, kept, bias, need_dx, need_dw):
+        """x [M, K], and w [N, K] or kept = (codes, scales, N) -> out [M, N] of x's type, what the backward pass needs (or None)."""
+        what = 'mx4_linear'
+        dev = self._mx4_chk(what, x, w if kept is None else kept[0], bias)
+        m, k = x.shape
+        n = w.shape[0] if kept is None else kept[2]
+        xcode = self._mx4_type(what, x.dtype)
+        lib = _lib.lib()
+        with _on(dev):
+            out = torch.empty((m, n), dtype=x.dtype, device=dev)
+            scratch = torch.empty(lib.deepipr_mx4_linear_scratch_bytes(m, n, k, 0), dtype=torch.uint8, device=dev)
+            saved = None
+            if need_dx or need_dw:
+                saved = torch.empty(lib.deepipr_mx4_linear_saved_bytes(m, n, k, need_dx, need_dw), dtype=torch.uint8, device=dev)
+            wargs = (w.data_ptr(), self._mx4_type(what, w.dtype), w.stride(0) if n > 1 else k, None, None) if kept is None else \
+                (None, 0, 0, kept[0].data_ptr(), kept[1].data_ptr())
+            _lib.check(lib.deepipr_mx4_linear_fwd(
+                x.data_ptr(), xcode, x.stride(0) if m > 1 else k, *wargs, _p(bias), 0 if bias is None else self._mx4_type(what, bias.dtype),
+                m, n, k, need_dx, need_dw, _p(saved), 0 if saved is None else saved.numel(), out.data_ptr(), scratch.data_ptr(),
+                scratch.numel(), _stream(dev)), 'mx4_linear_fwd')
+        return out, saved
+
+    def mx4_linear_bwd(self, dy, saved, k, need_dx, need_dw, dx_type, dw_type, want_db):
+        """-> dx [M, K] or None, dw [N, K] or None, dbias [N] float32 or None (need_*: as the forward call had them)."""
+        what = 'mx4_linear'
+        dev = self._mx4_chk(what, dy, saved)
+        m, n = dy.shape
+        lib = _lib.lib()
+        with _on(dev):
+            dx = torch.empty((m, k), dtype=dx_type, device=dev) if need_dx else None
+            dw = torch.empty((n, k), dtype=dw_type, device=dev) if need_dw else None
+            db = torch.empty(n, dtype=torch.float32, device=dev) if want_db else None
+            scratch = torch.empty(lib.deepipr_mx4_linear_scratch_bytes(m, n, k, 1), dtype=torch.uint8, device=dev)
+            _lib.check(lib.deepipr_mx4_linear_bwd(
+                dy.data_ptr(), self._mx4_type(what, dy.dtype), dy.stride(0) if m > 1 else n, m, n, k, need_dx, need_dw, _p(saved),
+                0 if saved is None else saved.numel(), _p(dx), 0 if dx is None else self._mx4_type(what, dx_type), _p(dw),
+                0 if dw is None else self._mx4_type(what, dw_type), _p(db), scratch.data_ptr(), scratch.numel(), _stream(dev)),
+                'mx4_linear_bwd')
+        return dx, dw, db
+
 
 kernels = HipKernels()
 

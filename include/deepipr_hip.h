@@ -458,6 +458,12 @@ int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const D
  *   deepipr_mx4_matmul      out [M][N] = A B^T (+ bias [N]), A [M][K] and B [N][K] quantised, on the block-scaled matrix instructions;
  *           fp32 products and sums, one rounding to `dtype`.  A NaN block makes NaN of every output whose row or column holds it.  workspace:
  *           deepipr_mx4_matmul_workspace_bytes(M, N, K) bytes (may be 0); calls that may run at the same time need one each.
+ *   deepipr_mx4_linear_fwd  out [M][N] = Q(x) Q(w)^T + bias in one call, `out` of x's type: x [M][K] and w [N][K] quantised along K (w == NULL:
+ *           w_codes / w_scales hold it already).  need_dx / need_dw: also w's / x's other direction, into `saved`, which the backward call
+ *           reads (the same two flags there).  x and w are read once each.
+ *   deepipr_mx4_linear_bwd  dx [M][K] = Q(dy) Q(w) with blocks along N, dw [N][K] = Q(dy)^T Q(x) with blocks along M, dbias [N] the column
+ *           sums of dy (not quantised); each may be NULL.  dy is read once.
+ *           scratch: deepipr_mx4_linear_scratch_bytes(M, N, K, backward) bytes of this call's own; saved: deepipr_mx4_linear_saved_bytes().
  * There is no counterpart in the reference (its classifiers are nn.Linear in fp32, models/alexnet_passport.py:27-36). */
 size_t deepipr_mx4_code_bytes(long long rows, long long cols);
 size_t deepipr_mx4_scale_bytes(long long rows, long long cols);
@@ -471,6 +477,16 @@ size_t deepipr_mx4_matmul_workspace_bytes(long long M, long long N, long long K)
 int deepipr_mx4_matmul(const void *a_codes, const void *a_scales, const void *b_codes, const void *b_scales, const void *bias,
                        int bias_dtype, long long M, long long N, long long K, void *out, int dtype, void *workspace,
                        size_t workspace_bytes, void *stream);
+
+size_t deepipr_mx4_linear_saved_bytes(long long M, long long N, long long K, int need_dx, int need_dw);
+size_t deepipr_mx4_linear_scratch_bytes(long long M, long long N, long long K, int backward);
+int deepipr_mx4_linear_fwd(const void *x, int x_dtype, long long x_stride, const void *w, int w_dtype, long long w_stride,
+                           const void *w_codes, const void *w_scales, const void *bias, int bias_dtype, long long M, long long N,
+                           long long K, int need_dx, int need_dw, void *saved, size_t saved_bytes, void *out, void *scratch,
+                           size_t scratch_bytes, void *stream);
+int deepipr_mx4_linear_bwd(const void *dy, int dy_dtype, long long dy_stride, long long M, long long N, long long K, int need_dx,
+                           int need_dw, const void *saved, size_t saved_bytes, void *dx, int dx_dtype, void *dw, int dw_dtype,
+                           float *dbias, void *scratch, size_t scratch_bytes, void *stream);
 
 /* ------------------------------------------------------------------ head of the train step
  * loss = mean_n( logsumexp(logits[n]) - logits[n][target[n]] ),  top1_pct = 100 * mean_n( argmax(logits[n]) ==

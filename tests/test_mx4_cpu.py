@@ -36,6 +36,27 @@ def test_c_entries_refuse_before_any_launch():
         assert mm(**bad) == -1 and b'mx4_matmul' in lib.deepipr_last_error(), bad
 
 
+def test_linear_entries_refuse_before_any_launch():
+    lib = _lib.lib()
+    p, big = 1 << 12, 1 << 30
+
+    def fwd(x=p, xt=0, xs=70, w=p, wt=0, ws=70, wc=None, wsc=None, bias=None, bt=0, m=5, n=6, k=70, dx=1, dw=1, saved=p, sb=big, out=p, scratch=p, cb=big):
+        return lib.deepipr_mx4_linear_fwd(x, xt, xs, w, wt, ws, wc, wsc, bias, bt, m, n, k, dx, dw, saved, sb, out, scratch, cb, None)
+    for bad in (dict(x=None), dict(xt=3), dict(xs=69), dict(w=None), dict(w=None, wc=p, wsc=p), dict(w=None, wc=p, dx=0, dw=0), dict(wt=-1), dict(ws=1),
+                dict(m=0), dict(n=0), dict(k=0), dict(out=None), dict(saved=None), dict(sb=1), dict(scratch=None), dict(cb=1), dict(scratch=p + 4),
+                dict(bias=p, bt=5), dict(bias=p + 2), dict(m=1 << 41)):
+        assert fwd(**bad) == -1 and b'mx4_linear_fwd' in lib.deepipr_last_error(), bad
+
+    def bwd(dy=p, t=0, s=6, m=5, n=6, k=70, ndx=1, ndw=1, saved=p, sb=big, dx=p, dxt=0, dw=p, dwt=0, db=p, scratch=p, cb=big):
+        return lib.deepipr_mx4_linear_bwd(dy, t, s, m, n, k, ndx, ndw, saved, sb, dx, dxt, dw, dwt, db, scratch, cb, None)
+    for bad in (dict(dy=None), dict(t=4), dict(s=5), dict(m=0), dict(n=-1), dict(k=0), dict(ndx=0), dict(ndw=0), dict(saved=None), dict(sb=7), dict(dxt=9),
+                dict(dwt=3), dict(db=p + 2), dict(dx=None, dw=None, db=None), dict(scratch=None), dict(cb=3)):
+        assert bwd(**bad) == -1 and b'mx4_linear_bwd' in lib.deepipr_last_error(), bad
+    assert lib.deepipr_mx4_linear_saved_bytes(5, 6, 70, 0, 0) == 0 and lib.deepipr_mx4_linear_scratch_bytes(0, 6, 70, 0) == 0
+    assert lib.deepipr_mx4_linear_saved_bytes(5, 6, 70, 1, 1) == 2 * lib.deepipr_mx4_linear_saved_bytes(5, 6, 70, 1, 0)
+    assert lib.deepipr_mx4_matmul_workspace_bytes(128, 128, 20000) > 0 == lib.deepipr_mx4_matmul_workspace_bytes(64, 128, 20000)
+
+
 def test_host_tensors_and_shapes_are_refused():
     x = torch.ones(4, 40)
     for call in (lambda: mx4.quantize(x), lambda: mx4.quantize_both(x), lambda: mx4.linear(x, x), lambda: mx4.quantize(x[:0])):

@@ -161,6 +161,21 @@ def test_products_are_exact(mnk, dtype):
     assert torch.equal(mx4.matmul(qa, qb, dtype=dtype), again)
 
 
+@pytest.mark.parametrize('mnk', [(64, 4200, 1200), (65, 300, 9000), (128, 128, 20000), (4104, 4096, 130), (4160, 4000, 300), (4352, 4100, 250),
+                                 (2500, 3000, 700)])
+def test_products_of_every_form_are_exact(mnk):
+    """Few rows; columns shared out over workgroups; whole tiles with a few rows behind them; large tiles with ragged ends."""
+    from deepipr_amd import mx4
+    m, n, k = mnk
+    a, b = _codes(m, k, 4, (0,)).to(DEV), _codes(n, k, 5, (0,)).to(DEV)                # multiples of 1/4 below 2^20: exact
+    bias = torch.randint(-8, 8, (n,), generator=torch.Generator().manual_seed(6)).float().to(DEV)
+    want = torch.mm(a.double(), b.double().t().contiguous())
+    for dtype in TYPES:
+        got = mx4.matmul(mx4.quantize(a), mx4.quantize(b), dtype=dtype)
+        assert torch.equal(got, want.to(dtype))
+        assert torch.equal(mx4.linear(a.to(dtype), mx4.quantize(b), bias), (want + bias.double()).to(dtype))
+
+
 def _bound(a, b, dtype, bias=None):
     """|out - exact| by the argument at the top of the file; a [M, K], b [N, K] float64 torch."""
     k = a.shape[1]
