@@ -62,15 +62,23 @@ template <int T> __device__ __forceinline__ void store1(void *p, long long i, fl
     if (T == F32) static_cast<float *>(p)[i] = v;
     else static_cast<unsigned short *>(p)[i] = static_cast<unsigned short>(T == BF16 ? f32_to_bf16(v) : f32_to_f16(v));
 }
-// four neighbours at once (the caller checked the alignment); gfx950 converts pairs, to nearest, ties to even
+// Four neighbours at once, on whatever address their type allows (the card takes vector accesses at any element); gfx950 converts pairs,
+// to nearest, ties to even.
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef bf16x4 bf16x4_any __attribute__((aligned(2)));
+typedef f16x4 f16x4_any __attribute__((aligned(2)));
+typedef u32x4 u32x4_any4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_any2 __attribute__((aligned(2)));
 template <int T> __device__ __forceinline__ void store4(void *p, f32x4 v) {
-    if (T == F32) {
-        *static_cast<f32x4 *>(p) = v;
-    } else if (T == BF16) {
-        *static_cast<bf16x4 *>(p) = __builtin_convertvector(v, bf16x4);
-    } else {
-        *static_cast<f16x4 *>(p) = __builtin_convertvector(v, f16x4);
-    }
+    if (T == F32) *static_cast<f32x4_any *>(p) = v;
+    else if (T == BF16) *static_cast<bf16x4_any *>(p) = __builtin_convertvector(v, bf16x4);
+    else *static_cast<f16x4_any *>(p) = __builtin_convertvector(v, f16x4);
+}
+// 16 bytes of elements
+template <int T> __device__ __forceinline__ u32x4 load16(const void *p, long long i) {
+    const char *at = static_cast<const char *>(p) + i * (T == F32 ? 4 : 2);
+    if (T == F32) return *reinterpret_cast<const u32x4_any4 *>(at);
+    return *reinterpret_cast<const u32x4_any2 *>(at);
 }
 template <int T> __device__ __forceinline__ void *element(void *p, long long i) { return static_cast<char *>(p) + i * (T == F32 ? 4 : 2); }
 
@@ -116,7 +124,7 @@ __device__ __forceinline__ u32x4 quantise32(float *v, unsigned &code) {
 constexpr int kQR = 64, kQC = 128, kQP = kQC + 4;        // pitch: 16-byte rows shifted by four banks each
 
 template <int T, bool ROW, bool COL, bool SUM>
-__global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restrict__ x, long long R, long long C, long long stride, int vec,
+__global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restrict__ x, long long R, long long C, long long stride,
                                                            unsigned char *__restrict__ row_codes, unsigned *__restrict__ row_scales,
                                                            unsigned char *__restrict__ col_codes, unsigned *__restrict__ col_scales,
                                                            float *__restrict__ sums) {
@@ -125,33 +133,49 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
     const long long tiles_c = (C + kQC - 1) / kQC;
     const long long r0 = static_cast<long long>(blockIdx.x) / tiles_c * kQR, c0 = static_cast<long long>(blockIdx.x) % tiles_c * kQC;
     const int tid = threadIdx.x;
-    if (vec && c0 + kQC <= C) {                          // whole 16-byte pieces
-        constexpr int V = T == F32 ? 4 : 8, PER = kQC / V;
-        u32x4 q[kQR * PER / kThreads];
+    constexpr int V = T == F32 ? 4 : 8, PER = kQC / V, LOADS = kQR * PER / kThreads;      // 16-byte pieces
+    const auto put = [&](int i, u32x4 q) {
+        float *d = s + i / PER * kQP + i % PER * V;
+        if (T == F32) {
+            *reinterpret_cast<u32x4 *>(d) = q;
+        } else {
 #pragma unroll
-        for (int j = 0; j < kQR * PER / kThreads; ++j) {
-            const int i = j * kThreads + tid, r = i / PER, c = i % PER * V;
-            const long long at = (r0 + r) * stride + c0 + c;
-            q[j] = r0 + r < R ? *reinterpret_cast<const u32x4 *>(static_cast<const char *>(x) + at * (T == F32 ? 4 : 2)) : u32x4{0, 0, 0, 0};
-        }
+            for (int k = 0; k < 4; k += 2) {
+                f32x4 f;
 #pragma unroll
-        for (int j = 0; j < kQR * PER / kThreads; ++j) {
-            const int i = j * kThreads + tid, r = i / PER, c = i % PER * V;
-            float *d = s + r * kQP + c;
-            if (T == F32) {
-                *reinterpret_cast<u32x4 *>(d) = q[j];
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    d[2 * k] = T == BF16 ? __uint_as_float(q[j][k] << 16) : f16_to_f32(q[j][k] & 0xffffu);
-                    d[2 * k + 1] = T == BF16 ? __uint_as_float(q[j][k] & 0xffff0000u) : f16_to_f32(q[j][k] >> 16);
+                for (int e = 0; e < 2; ++e) {
+                    f[2 * e] = T == BF16 ? __uint_as_float(q[k + e] << 16) : f16_to_f32(q[k + e] & 0xffffu);
+                    f[2 * e + 1] = T == BF16 ? __uint_as_float(q[k + e] & 0xffff0000u) : f16_to_f32(q[k + e] >> 16);
                 }
+                *reinterpret_cast<f32x4 *>(d + 2 * k) = f;
             }
         }
-    } else {
-        for (int i = tid; i < kQR * kQC; i += kThreads) {
-            const int r = i / kQC, c = i % kQC;
-            s[r * kQP + c] = r0 + r < R && c0 + c < C ? load1<T>(x, (r0 + r) * stride + c0 + c) : 0.0f;
+    };
+    if (r0 + kQR <= R && c0 + kQC <= C) {
+        u32x4 q[LOADS];
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int i = j * kThreads + tid;
+            q[j] = load16<T>(x, (r0 + i / PER) * stride + c0 + i % PER * V);
+        }
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) put(j * kThreads + tid, q[j]);
+    } else {                                             // the matrix's last rows or columns
+#pragma unroll 2
+        for (int i = tid; i < kQR * PER; i += kThreads) {
+            const long long r = r0 + i / PER, c = c0 + i % PER * V;
+            u32x4 q = {0, 0, 0, 0};
+            if (r < R && c + V <= C) {
+                q = load16<T>(x, r * stride + c);
+            } else if (r < R) {
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    if (c + k < C) {
+                        if (T == F32) q[k & 3] = static_cast<const unsigned *>(x)[r * stride + c + k];
+                        else q[k >> 1] |= static_cast<unsigned>(static_cast<const unsigned short *>(x)[r * stride + c + k]) << (k & 1) * 16;
+                    }
+            }
+            put(i, q);
         }
     }
     __syncthreads();
@@ -232,40 +256,58 @@ __device__ __forceinline__ void decode8(unsigned w, float x, float *v) {
 
 template <int T>
 __global__ __launch_bounds__(kThreads) void k_mx4_dequantise(const unsigned char *__restrict__ codes, const unsigned *__restrict__ scales,
-                                                             long long R, long long K, int vec, void *__restrict__ out) {
+                                                             long long R, long long K, void *__restrict__ out) {
     const long long per = (K + 7) / 8, n = R * per;
     for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads) {
         const long long r = i / per, k = i % per * 8;
         float v[8];
         decode8(codes_at(codes, R, r, k), scale_value(scale_at(scales, R, r, k / 32)), v);
-        if (vec && k + 8 <= K) {
+        if (k + 8 <= K) {
             store4<T>(element<T>(out, r * K + k), f32x4{v[0], v[1], v[2], v[3]});
             store4<T>(element<T>(out, r * K + k + 4), f32x4{v[4], v[5], v[6], v[7]});
         } else {
-            for (int j = 0; j < 8 && k + j < K; ++j) store1<T>(out, r * K + k + j, v[j]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (k + j < K) store1<T>(out, r * K + k + j, v[j]);
         }
     }
 }
 
-// out [K][R]: a workgroup takes 64 rows x 64 columns of the matrix
+// out [K][R]: a workgroup takes 64 rows x 128 columns of the matrix, a thread one block; 64 values of each output row go out together
 template <int T>
 __global__ __launch_bounds__(kThreads) void k_mx4_dequantise_t(const unsigned char *__restrict__ codes, const unsigned *__restrict__ scales,
                                                                long long R, long long K, void *__restrict__ out) {
-    __shared__ float s[64 * 65];
+    constexpr int P = 68;
+    __shared__ __align__(16) float s[128 * P];
     const long long tiles_r = (R + 63) / 64;
-    const long long r0 = static_cast<long long>(blockIdx.x) % tiles_r * 64, k0 = static_cast<long long>(blockIdx.x) / tiles_r * 64;
-    for (int i = threadIdx.x; i < 64 * 8; i += kThreads) {
-        const int r = i >> 3, k = (i & 7) * 8;
-        float v[8] = {};
-        if (r0 + r < R)                                  // columns behind K lie in the padding: zero codes
-            decode8(codes_at(codes, R, r0 + r, k0 + k), scale_value(scale_at(scales, R, r0 + r, (k0 + k) / 32)), v);
+    const int id = dipr_xcd_contiguous(blockIdx.x, gridDim.x);
+    const long long r0 = id % tiles_r * 64, k0 = id / tiles_r * 128;
+    const int r = threadIdx.x & 63, b = threadIdx.x >> 6;
+    if (r0 + r < R) {                                    // columns behind K lie in the padding: zero codes
+        const u32x4 q = *reinterpret_cast<const u32x4 *>(codes + (k0 / 128 * R + r0 + r) * 64 + b * 16);
+        const float x = scale_value(scale_at(scales, R, r0 + r, k0 / 32 + b));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[(k + j) * 65 + r] = v[j];
+        for (int w = 0; w < 4; ++w) {
+            float v[8];
+            decode8(q[w], x, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[(b * 32 + w * 8 + j) * P + r] = v[j];
+        }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 64; i += kThreads) {
-        const int k = i >> 6, r = i & 63;
-        if (k0 + k < K && r0 + r < R) store1<T>(out, (k0 + k) * R + r0 + r, s[k * 65 + r]);
+    const int c = threadIdx.x & 15;                      // four neighbouring rows of the matrix
+#pragma unroll 4
+    for (int k = threadIdx.x >> 4; k < 128; k += kThreads / 16) {
+        if (k0 + k >= K) break;
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(s + k * P + c * 4);
+        const long long at = (k0 + k) * R + r0 + c * 4;
+        if (r0 + c * 4 + 4 <= R) {
+            store4<T>(element<T>(out, at), v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (r0 + c * 4 + j < R) store1<T>(out, at + j, v[j]);
+        }
     }
 }
 
@@ -289,7 +331,7 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c, unsigned sa, 
 // rows m0 .. of `out`, 32 rows at a time through `strip` (32 rows of 32 TN + 4 floats of this wave's own): whole cache lines per row.
 template <int T, int TM, int TN>
 __device__ __forceinline__ void store_tiles(const f32x16 (&acc)[TN][TM], float *strip, const void *bias, int bias_type, long long m0, long long n0,
-                                            long long M, long long N, int vec, void *out) {
+                                            long long M, long long N, void *out) {
     constexpr int P = 32 * TN + 4, PER = 8 * TN, STEP = 64 / PER;          // lanes per row (a lane keeps its columns), rows per pass
     const int lane = threadIdx.x & 63, row = lane / PER;
     const long long n = n0 + lane % PER * 4;
@@ -299,7 +341,7 @@ __device__ __forceinline__ void store_tiles(const f32x16 (&acc)[TN][TM], float *
         for (int j = 0; j < 4; ++j)
             if (n + j < N) add[j] = bias_at(bias, bias_type, n + j);
     }
-    const bool whole = vec && m0 + 32 * TM <= M && n0 + 32 * TN <= N;      // uniform: nearly every tile of a large product
+    const bool whole = m0 + 32 * TM <= M && n0 + 32 * TN <= N;      // uniform: nearly every tile of a large product
     const float *from = strip + row * P + lane % PER * 4;
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
@@ -322,7 +364,7 @@ __device__ __forceinline__ void store_tiles(const f32x16 (&acc)[TN][TM], float *
                 const long long m = m0 + t * 32 + row + r;
                 const f32x4 v = *reinterpret_cast<const f32x4 *>(from + r * P) + add;
                 if (m >= M) continue;
-                if (vec && n + 4 <= N) {
+                if (n + 4 <= N) {
                     store4<T>(element<T>(out, m * N + n), v);
                 } else {
 #pragma unroll
@@ -338,7 +380,7 @@ struct Product {
     const unsigned char *a, *b;                          // [kt][M][64], [kt][N][64]
     const unsigned *sa, *sb;
     const void *bias;
-    int bias_type, vec;
+    int bias_type;
     long long M, N;                                      // of the operands in memory
     long long first, last;                               // rows first .. last - 1 of the output (first a multiple of 64)
     int kt, splits;                                      // splits > 1: out is float [splits][M][N], split i adds up its share of the steps
@@ -412,7 +454,7 @@ __global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product P) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (P.bias && n + j < P.N) v[j] += bias_at(P.bias, P.bias_type, n + j);
-    if (P.vec && n + 4 <= P.N) {
+    if (n + 4 <= P.N) {
         store4<T>(element<T>(P.out, m * P.N + n), v);
     } else {
 #pragma unroll
@@ -424,13 +466,14 @@ __global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product P) {
 // The splits' sums, in order: out [M][N] = sum_i part[i][M][N] + bias
 template <int T>
 __global__ __launch_bounds__(kThreads) void k_mx4_gemm_sum(const float *__restrict__ part, int splits, const void *__restrict__ bias, int bias_type,
-                                                           long long M, long long N, int vec, void *__restrict__ out) {
+                                                           long long M, long long N, void *__restrict__ out) {
     const long long per = (N + 3) / 4, n = M * per;
     for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads) {
         const long long row = i / per, c = i % per * 4, at = row * N + c;
         f32x4 v = {};
-        if (vec) {
-            for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4 *>(part + s * M * N + at);
+        if (c + 4 <= N) {
+#pragma unroll 4
+            for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4_any *>(part + s * M * N + at);
         } else {
             for (int s = 0; s < splits; ++s)
 #pragma unroll
@@ -440,7 +483,7 @@ __global__ __launch_bounds__(kThreads) void k_mx4_gemm_sum(const float *__restri
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (bias && c + j < N) v[j] += bias_at(bias, bias_type, c + j);
-        if (vec) {
+        if (c + 4 <= N) {
             store4<T>(element<T>(out, at), v);
         } else {
 #pragma unroll
@@ -607,7 +650,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P)
 
     __syncthreads();                                     // every wave is through with the stages
     store_tiles<T, TM, TN>(acc, reinterpret_cast<float *>(lds) + wave * 32 * (32 * TN + 4), P.bias, P.bias_type, m0 + wm * 32, n0 + wn * 32,
-                           P.last, N, P.vec, out);
+                           P.last, N, out);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host side
@@ -617,13 +660,13 @@ inline int elem_bytes(int d) { return d == F32 ? 4 : 2; }
 constexpr long long kMaxSide = 1ll << 40, kMaxGrid = 1ll << 30;
 
 template <int T>
-void launch_quantise(DiprProf &prof, const void *x, long long R, long long C, long long stride, int vec, void *rc, void *rs, void *cc, void *cs,
+void launch_quantise(DiprProf &prof, const void *x, long long R, long long C, long long stride, void *rc, void *rs, void *cc, void *cs,
                      float *sums, hipStream_t st) {
     // blocks down the columns need the padding rows' zeros too
     const long long tiles_r = cc ? round_up(R, 128) / kQR : (R + kQR - 1) / kQR, tiles_c = (C + kQC - 1) / kQC;
     const dim3 grid(static_cast<unsigned>(tiles_r * tiles_c)), block(kThreads);
 #define MX4_QUANTISE(ROW, COL, SUM)                                                                                                  \
-    DIPR_LAUNCH(prof, (k_mx4_quantise<T, ROW, COL, SUM>), grid, block, st, x, R, C, stride, vec, static_cast<unsigned char *>(rc),   \
+    DIPR_LAUNCH(prof, (k_mx4_quantise<T, ROW, COL, SUM>), grid, block, st, x, R, C, stride, static_cast<unsigned char *>(rc),   \
                 static_cast<unsigned *>(rs), static_cast<unsigned char *>(cc), static_cast<unsigned *>(cs), sums)
     if (rc && cc && sums) MX4_QUANTISE(true, true, true);
     else if (rc && cc) MX4_QUANTISE(true, true, false);
@@ -635,12 +678,15 @@ void launch_quantise(DiprProf &prof, const void *x, long long R, long long C, lo
 
 
 // ---- which kernels a product takes
-// Times of one step of 128 columns and of a tile's begin and end, in ns, as measured (8192^2 x {128, 8192, 16384}, 8200 x 4096 x 4096):
-// 256 x 256 tiles, one a CU, 780 and 6 000; 128 x 128 tiles, two a CU, 690 and 3 000.
+// Estimated from measured times (ns): a step of 128 columns costs a 256 x 256 tile 780, a 128 x 128 tile 270 where it has the CU for itself
+// and 690 where two share it; begin and end of a tile 6 000 / 3 000; a second launch that adds up partial sums 4 000 and their bytes at
+// 4 TB/s.  Measured (us): 8192^3 253 large, 355 small; 4096 x 4096 x 8200 65 / 78; 2048^3 18.3 / 10.1; 253 x 4096 x 9216 52 large, 24.5
+// small, 20.9 small with the columns in three; 512 x 512 x 16384 34.8 whole, 15.5 in eight; 1000^3 8.2 whole, 13 in two; 32 x 4096 x 9216 8.2
+// by the kernel for few rows, 12.1 at best by the others.
 struct Plan {
     enum { kRows, kSmall, kLarge } form;
     int splits;                  // kSmall only
-    long long tail;              // rows at the end that go to the kernel for few rows (0: none)
+    long long tail;              // kLarge only: rows at the end that go to the kernel for few rows (0: none)
 };
 inline long long tiles_of(long long m, long long n, int side) { return ((m + side - 1) / side) * ((n + side - 1) / side); }
 inline int cu_count() {
@@ -651,30 +697,31 @@ inline double large_ns(long long m, long long n, long long kt) {
     const long long rounds = (tiles_of(m, n, 256) + cu_count() - 1) / cu_count();
     return static_cast<double>(rounds) * (780.0 * kt + 6000.0);
 }
-inline double small_ns(long long m, long long n, long long kt) {
-    const double rounds = static_cast<double>(tiles_of(m, n, 128)) / (2 * cu_count());
-    return (rounds < 1.0 ? 1.0 : rounds) * (690.0 * kt + 3000.0);
+inline double small_ns(long long m, long long n, long long kt, int splits) {
+    const double slots = 2.0 * cu_count(), tiles = static_cast<double>(tiles_of(m, n, 128)) * splits;
+    const double step = tiles <= slots / 2 ? 270.0 : 690.0 * (tiles > slots ? tiles / slots : 1.0);
+    const double sums = splits > 1 ? 4000.0 + static_cast<double>(splits) * m * n * 8 / 4000.0 : 0.0;
+    return step * static_cast<double>((kt + splits - 1) / splits) + 3000.0 + sums;
 }
 Plan plan(long long M, long long N, long long kt) {
     Plan p = {Plan::kRows, 1, 0};
     if (M <= 64) return p;
-    // a few rows behind whole tiles: a tile row of its own for them would cost a round
-    const long long tail = M % 256 <= 64 && M > 256 ? M % 256 : 0;
-    double best = large_ns(M, N, kt);
     p.form = Plan::kLarge;
+    double best = large_ns(M, N, kt);
+    // a few rows behind whole tiles: a tile row of their own could cost a round
+    const long long tail = M % 256 <= 64 && M > 256 ? M % 256 : 0;
     if (tail) {
-        const double t = large_ns(M - tail, N, kt) + 5000.0 + 0.2 * static_cast<double>(N * kt) / 16.0;
+        const double t = large_ns(M - tail, N, kt) + 5000.0 + static_cast<double>(N * kt) / 80.0;
         if (t < best) best = t, p.tail = tail;
     }
-    if (small_ns(M, N, kt) < best) {
-        p.form = Plan::kSmall;
-        p.tail = 0;
-        // tiles that leave slots free share the columns out instead: the partial sums cost a second launch
-        const long long tiles = tiles_of(M, N, 128), slots = 2 * cu_count();
-        long long splits = slots / tiles;
-        if (splits > kt / 4) splits = kt / 4;
-        if (splits > 16) splits = 16;
-        if (splits > 1) p.splits = static_cast<int>(splits);
+    for (int splits = 1; splits <= 16 && splits <= kt; splits += splits < 4 ? 1 : splits / 2) {
+        const double t = small_ns(M, N, kt, splits);
+        if (t < best) {
+            best = t;
+            p.form = Plan::kSmall;
+            p.splits = splits;
+            p.tail = 0;
+        }
     }
     return p;
 }
@@ -705,24 +752,22 @@ template <int T> void launch_product(DiprProf &prof, const Plan &plan, Product P
     Q.splits = plan.splits;
     Q.out = part;
     Q.bias = nullptr;
-    Q.vec = P.N % 4 == 0;
     DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<F32, 2, 2>), dim3(tiles * plan.splits), block, st, Q);
     const long long want = (P.M * ((P.N + 3) / 4) + kThreads - 1) / kThreads;
     hipLaunchKernelGGL((k_mx4_gemm_sum<T>), dim3(static_cast<unsigned>(want < 8192 ? want : 8192)), block, 0, st, part, plan.splits, P.bias, P.bias_type,
-                       P.M, P.N, P.vec, P.out);
+                       P.M, P.N, P.out);
 }
 
 // ---- the pieces that the C entries share; arguments are checked by then
 void quantise(const void *x, int dtype, long long R, long long C, long long stride, void *rc, void *rs, void *cc, void *cs, float *col_sums,
               void *workspace, hipStream_t st) {
-    const int vec = aligned(x, 16) && (R == 1 || stride * elem_bytes(dtype) % 16 == 0);
     float *sums = col_sums ? static_cast<float *>(workspace) : nullptr;
     DiprProf prof(DEEPIPR_K_MX4_QUANTIZE);
     prof.bytes = static_cast<double>(R) * static_cast<double>(C) * (elem_bytes(dtype) + 0.53125 * ((rc ? 1 : 0) + (cc ? 1 : 0)));
     switch (dtype) {
-        case F32: launch_quantise<F32>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
-        case BF16: launch_quantise<BF16>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
-        default: launch_quantise<F16>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
+        case F32: launch_quantise<F32>(prof, x, R, C, stride, rc, rs, cc, cs, sums, st); break;
+        case BF16: launch_quantise<BF16>(prof, x, R, C, stride, rc, rs, cc, cs, sums, st); break;
+        default: launch_quantise<F16>(prof, x, R, C, stride, rc, rs, cc, cs, sums, st); break;
     }
     if (col_sums)
         hipLaunchKernelGGL(k_mx4_colsum, dim3(static_cast<unsigned>((C + 31) / 32)), dim3(kThreads), 0, st, sums, round_up(R, 128) / kQR, C, col_sums);
@@ -748,7 +793,6 @@ void product(const void *a, const void *sa, const void *b, const void *sb, const
     P.sb = static_cast<const unsigned *>(sb);
     P.bias = bias;
     P.bias_type = bias_dtype;
-    P.vec = N % 4 == 0 && aligned(out, 4 * elem_bytes(dtype));
     P.M = P.last = M;
     P.N = N;
     P.first = 0;
@@ -865,7 +909,7 @@ int deepipr_mx4_dequantize(const void *codes, const void *scales, long long rows
     if (!codes || !scales || !out || !good_dtype(dtype) || rows <= 0 || cols <= 0 || rows > kMaxSide || cols > kMaxSide)
         return dipr_fail(DEEPIPR_EINVAL, "%s: bad argument", what);
     if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(out, elem_bytes(dtype))) return dipr_fail(DEEPIPR_EINVAL, "%s: misaligned pointer", what);
-    const long long tiles = ((rows + 63) / 64) * ((cols + 63) / 64);
+    const long long tiles = ((rows + 63) / 64) * ((cols + 127) / 128);
     if (tiles > kMaxGrid) return dipr_fail(DEEPIPR_EINVAL, "%s: matrix too large", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
     DiprProf prof(DEEPIPR_K_MX4_DEQUANTIZE);
@@ -878,9 +922,8 @@ int deepipr_mx4_dequantize(const void *codes, const void *scales, long long rows
             DIPR_LAUNCH(prof, (k_mx4_dequantise_t<T>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), st, c, s, rows, cols, out); \
         } else {                                                                                                                     \
             const long long want = (rows * ((cols + 7) / 8) + kThreads - 1) / kThreads;                                              \
-            const int vec = cols % 4 == 0 && aligned(out, 16);                                                                       \
             DIPR_LAUNCH(prof, (k_mx4_dequantise<T>), dim3(static_cast<unsigned>(want < 16384 ? want : 16384)), dim3(kThreads), st, c, s, rows, \
-                        cols, vec, out);                                                                                             \
+                        cols, out);                                                                                                  \
         }                                                                                                                            \
     } while (0)
     switch (dtype) {
