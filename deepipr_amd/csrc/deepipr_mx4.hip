@@ -67,18 +67,14 @@ template <int T> __device__ __forceinline__ void store1(void *p, long long i, fl
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef bf16x4 bf16x4_any __attribute__((aligned(2)));
 typedef f16x4 f16x4_any __attribute__((aligned(2)));
-typedef u32x4 u32x4_any4 __attribute__((aligned(4)));
-typedef u32x4 u32x4_any2 __attribute__((aligned(2)));
 template <int T> __device__ __forceinline__ void store4(void *p, f32x4 v) {
     if (T == F32) *static_cast<f32x4_any *>(p) = v;
     else if (T == BF16) *static_cast<bf16x4_any *>(p) = __builtin_convertvector(v, bf16x4);
     else *static_cast<f16x4_any *>(p) = __builtin_convertvector(v, f16x4);
 }
-// 16 bytes of elements
+// 16 bytes of elements (the caller checked the alignment)
 template <int T> __device__ __forceinline__ u32x4 load16(const void *p, long long i) {
-    const char *at = static_cast<const char *>(p) + i * (T == F32 ? 4 : 2);
-    if (T == F32) return *reinterpret_cast<const u32x4_any4 *>(at);
-    return *reinterpret_cast<const u32x4_any2 *>(at);
+    return *reinterpret_cast<const u32x4 *>(static_cast<const char *>(p) + i * (T == F32 ? 4 : 2));
 }
 template <int T> __device__ __forceinline__ void *element(void *p, long long i) { return static_cast<char *>(p) + i * (T == F32 ? 4 : 2); }
 
@@ -124,7 +120,7 @@ __device__ __forceinline__ u32x4 quantise32(float *v, unsigned &code) {
 constexpr int kQR = 64, kQC = 128, kQP = kQC + 4;        // pitch: 16-byte rows shifted by four banks each
 
 template <int T, bool ROW, bool COL, bool SUM>
-__global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restrict__ x, long long R, long long C, long long stride,
+__global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restrict__ x, long long R, long long C, long long stride, int vec,
                                                            unsigned char *__restrict__ row_codes, unsigned *__restrict__ row_scales,
                                                            unsigned char *__restrict__ col_codes, unsigned *__restrict__ col_scales,
                                                            float *__restrict__ sums) {
@@ -151,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
             }
         }
     };
-    if (r0 + kQR <= R && c0 + kQC <= C) {
+    if (vec && r0 + kQR <= R && c0 + kQC <= C) {
         u32x4 q[LOADS];
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
@@ -160,23 +156,38 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
         }
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) put(j * kThreads + tid, q[j]);
-    } else {                                             // the matrix's last rows or columns
-#pragma unroll 2
-        for (int i = tid; i < kQR * PER; i += kThreads) {
-            const long long r = r0 + i / PER, c = c0 + i % PER * V;
-            u32x4 q = {0, 0, 0, 0};
-            if (r < R && c + V <= C) {
-                q = load16<T>(x, r * stride + c);
-            } else if (r < R) {
+    } else if (T == F32) {
+        // rows off the 16-byte grid (a wave's single elements are contiguous whatever the alignment: 200 704 x 1021 takes 179 us this way
+        // and 293 by unaligned 16-byte loads), and the matrix's last rows and columns
+        const int c = tid & 127, h = tid >> 7;
+        const long long left = c0 + c < C ? R - r0 - h : 0;              // rows h, h + 2, ... that exist
+        float e[32];
 #pragma unroll
-                for (int k = 0; k < V; ++k)
-                    if (c + k < C) {
-                        if (T == F32) q[k & 3] = static_cast<const unsigned *>(x)[r * stride + c + k];
-                        else q[k >> 1] |= static_cast<unsigned>(static_cast<const unsigned short *>(x)[r * stride + c + k]) << (k & 1) * 16;
-                    }
-            }
-            put(i, q);
+        for (int j = 0; j < 32; ++j) e[j] = 2 * j < left ? load1<T>(x, (r0 + h + 2 * j) * stride + c0 + c) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[(h + 2 * j) * kQP + c] = e[j];
+    } else {
+        // the same for 16-bit elements, two to an aligned word (loads of single ones are four times slower); a row that starts in the middle
+        // of a word is off by one: its first and last words hold one element of it, and what else they hold is not used
+        const int lane = tid & 63, first = (tid >> 6) * 16;
+        const auto row_at = [&](int r) { return reinterpret_cast<uintptr_t>(x) + static_cast<uintptr_t>(((r0 + r) * stride + c0) * 2); };
+        unsigned w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const uintptr_t at = row_at(first + j);
+            const int odd = static_cast<int>(at >> 1 & 1);
+            w[j] = r0 + first + j < R && c0 + 2 * lane - odd < C ? *reinterpret_cast<const unsigned *>(at - 2 * odd + 4 * lane) : 0u;
         }
+        const auto value = [&](unsigned h) { return T == BF16 ? bf16_to_f32(h) : f16_to_f32(h); };
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int e = 2 * lane - static_cast<int>(row_at(first + j) >> 1 & 1);
+            float *d = s + (first + j) * kQP + e;
+            if (e >= 0) d[0] = value(w[j] & 0xffffu);
+            d[1] = c0 + e + 1 < C ? value(w[j] >> 16) : 0.0f;
+        }
+        if (tid < kQR && (row_at(tid) >> 1 & 1))                         // the 128th column of a row that is off by one
+            s[tid * kQP + 127] = r0 + tid < R && c0 + 127 < C ? load1<T>(x, (r0 + tid) * stride + c0 + 127) : 0.0f;
     }
     __syncthreads();
     float v[32];
@@ -219,9 +230,13 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restric
     }
 }
 
-// sums [tiles][C] -> out [C]: eight threads a column, each every eighth tile in order, then the eight in order
+// sums [tiles][C] -> out [ceil(tiles / kSumTiles)][C]: eight threads a column, each every eighth tile in order, then the eight in order
+constexpr int kSumTiles = 128;
 __global__ __launch_bounds__(kThreads) void k_mx4_colsum(const float *__restrict__ sums, long long tiles, long long C, float *__restrict__ out) {
     __shared__ double red[8][32];
+    sums += blockIdx.y * kSumTiles * C;
+    out += blockIdx.y * C;
+    tiles = min(tiles - static_cast<long long>(blockIdx.y) * kSumTiles, static_cast<long long>(kSumTiles));
     const int col = threadIdx.x & 31, part = threadIdx.x >> 5;
     const long long c = static_cast<long long>(blockIdx.x) * 32 + col;
     double v = 0.0;
@@ -239,13 +254,10 @@ __global__ __launch_bounds__(kThreads) void k_mx4_colsum(const float *__restrict
 }
 
 // ----------------------------------------------------------------------------------------------------------------- dequantise
-// The matrix [R][K] of values, or its transpose [K][R].  A thread decodes 8 codes; the transposed form goes through LDS.
+// The matrix [R][K] of values, or its transpose [K][R].
 __device__ __forceinline__ unsigned scale_at(const unsigned *scales, long long rows, long long r, long long b) {
     const unsigned w = scales[((b >> 2) * row_groups(rows) + (r >> 6)) * 64 + (b & 1) * 32 + (r & 31)];
     return w >> (((b >> 1 & 1) * 2 + (r >> 5 & 1)) * 8) & 0xffu;
-}
-__device__ __forceinline__ unsigned codes_at(const unsigned char *codes, long long rows, long long r, long long k) {     // k a multiple of 8
-    return *reinterpret_cast<const unsigned *>(codes + ((k >> 7) * rows + r) * 64 + (k & 127) / 2);
 }
 __device__ __forceinline__ void decode8(unsigned w, float x, float *v) {
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
@@ -254,20 +266,29 @@ __device__ __forceinline__ void decode8(unsigned w, float x, float *v) {
     v[4] = c.x * x; v[5] = c.y * x; v[6] = d.x * x; v[7] = d.y * x;
 }
 
+// a workgroup takes 64 rows x 128 columns; 32 lanes write one row's 128 values
 template <int T>
 __global__ __launch_bounds__(kThreads) void k_mx4_dequantise(const unsigned char *__restrict__ codes, const unsigned *__restrict__ scales,
                                                              long long R, long long K, void *__restrict__ out) {
-    const long long per = (K + 7) / 8, n = R * per;
-    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads) {
-        const long long r = i / per, k = i % per * 8;
-        float v[8];
-        decode8(codes_at(codes, R, r, k), scale_value(scale_at(scales, R, r, k / 32)), v);
-        if (k + 8 <= K) {
-            store4<T>(element<T>(out, r * K + k), f32x4{v[0], v[1], v[2], v[3]});
-            store4<T>(element<T>(out, r * K + k + 4), f32x4{v[4], v[5], v[6], v[7]});
+    const long long panels = (K + 127) / 128;
+    const int id = dipr_xcd_contiguous(blockIdx.x, gridDim.x);           // neighbours share cache lines of `out` where rows are off the grid
+    const long long r0 = id / panels * 64, p = id % panels;
+    const int c = (threadIdx.x & 31) * 4;
+    const long long k = p * 128 + c;
+    if (k >= K) return;
+#pragma unroll 4
+    for (int i = threadIdx.x >> 5; i < 64; i += kThreads / 32) {
+        const long long r = r0 + i;
+        if (r >= R) break;
+        const unsigned w = *reinterpret_cast<const unsigned short *>(codes + (p * R + r) * 64 + c / 2);
+        const float x = scale_value(scale_at(scales, R, r, p * 4 + (c >> 5)));
+        const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+        const f32x4 v = f32x4{lo.x, lo.y, hi.x, hi.y} * x;
+        if (k + 4 <= K) {
+            store4<T>(element<T>(out, r * K + k), v);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 4; ++j)
                 if (k + j < K) store1<T>(out, r * K + k + j, v[j]);
         }
     }
@@ -660,13 +681,13 @@ inline int elem_bytes(int d) { return d == F32 ? 4 : 2; }
 constexpr long long kMaxSide = 1ll << 40, kMaxGrid = 1ll << 30;
 
 template <int T>
-void launch_quantise(DiprProf &prof, const void *x, long long R, long long C, long long stride, void *rc, void *rs, void *cc, void *cs,
+void launch_quantise(DiprProf &prof, const void *x, long long R, long long C, long long stride, int vec, void *rc, void *rs, void *cc, void *cs,
                      float *sums, hipStream_t st) {
     // blocks down the columns need the padding rows' zeros too
     const long long tiles_r = cc ? round_up(R, 128) / kQR : (R + kQR - 1) / kQR, tiles_c = (C + kQC - 1) / kQC;
     const dim3 grid(static_cast<unsigned>(tiles_r * tiles_c)), block(kThreads);
 #define MX4_QUANTISE(ROW, COL, SUM)                                                                                                  \
-    DIPR_LAUNCH(prof, (k_mx4_quantise<T, ROW, COL, SUM>), grid, block, st, x, R, C, stride, static_cast<unsigned char *>(rc),   \
+    DIPR_LAUNCH(prof, (k_mx4_quantise<T, ROW, COL, SUM>), grid, block, st, x, R, C, stride, vec, static_cast<unsigned char *>(rc),   \
                 static_cast<unsigned *>(rs), static_cast<unsigned char *>(cc), static_cast<unsigned *>(cs), sums)
     if (rc && cc && sums) MX4_QUANTISE(true, true, true);
     else if (rc && cc) MX4_QUANTISE(true, true, false);
@@ -761,19 +782,35 @@ template <int T> void launch_product(DiprProf &prof, const Plan &plan, Product P
 // ---- the pieces that the C entries share; arguments are checked by then
 void quantise(const void *x, int dtype, long long R, long long C, long long stride, void *rc, void *rs, void *cc, void *cs, float *col_sums,
               void *workspace, hipStream_t st) {
+    const int vec = aligned(x, 16) && (R == 1 || stride * elem_bytes(dtype) % 16 == 0);
     float *sums = col_sums ? static_cast<float *>(workspace) : nullptr;
     DiprProf prof(DEEPIPR_K_MX4_QUANTIZE);
     prof.bytes = static_cast<double>(R) * static_cast<double>(C) * (elem_bytes(dtype) + 0.53125 * ((rc ? 1 : 0) + (cc ? 1 : 0)));
     switch (dtype) {
-        case F32: launch_quantise<F32>(prof, x, R, C, stride, rc, rs, cc, cs, sums, st); break;
-        case BF16: launch_quantise<BF16>(prof, x, R, C, stride, rc, rs, cc, cs, sums, st); break;
-        default: launch_quantise<F16>(prof, x, R, C, stride, rc, rs, cc, cs, sums, st); break;
+        case F32: launch_quantise<F32>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
+        case BF16: launch_quantise<BF16>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
+        default: launch_quantise<F16>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
     }
-    if (col_sums)
-        hipLaunchKernelGGL(k_mx4_colsum, dim3(static_cast<unsigned>((C + 31) / 32)), dim3(kThreads), 0, st, sums, round_up(R, 128) / kQR, C, col_sums);
+    for (long long tiles = round_up(R, 128) / kQR; col_sums;) {          // at most 128 tiles in one go: long batches take a second or third pass
+        const long long groups = (tiles + kSumTiles - 1) / kSumTiles;
+        float *to = groups == 1 ? col_sums : sums + tiles * C;
+        hipLaunchKernelGGL(k_mx4_colsum, dim3(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(groups)), dim3(kThreads), 0, st, sums, tiles, C,
+                           to);
+        if (groups == 1) break;
+        sums = to;
+        tiles = groups;
+    }
+}
+inline size_t sums_bytes(long long R, long long C) {                      // every level's sums
+    size_t n = 0;
+    for (long long tiles = round_up(R, 128) / kQR;; tiles = (tiles + kSumTiles - 1) / kSumTiles) {
+        n += static_cast<size_t>(tiles);
+        if (tiles <= kSumTiles) return n * static_cast<size_t>(C) * sizeof(float);
+    }
 }
 inline bool quantise_fits(long long R, long long C) {
-    return R <= kMaxSide && C <= kMaxSide && round_up(R, 128) / kQR * ((C + kQC - 1) / kQC) <= kMaxGrid;
+    // (the grid of the column sums is 65 535 groups of 128 tiles at most)
+    return R <= 65535ll * kSumTiles * kQR && C <= kMaxSide && round_up(R, 128) / kQR * ((C + kQC - 1) / kQC) <= kMaxGrid;
 }
 inline bool product_fits(long long M, long long N, long long K) {
     return M <= kMaxSide && N <= kMaxSide && K <= kMaxSide && tiles_of(M, N, 128) <= kMaxGrid / 16 && (N + 15) / 16 <= kMaxGrid &&
@@ -859,7 +896,7 @@ struct BackwardScratch {
         Cut c(p);
         y = take_matrix(c, M, N);
         y_t = take_matrix(c, N, M);
-        sums = c.take(static_cast<size_t>(round_up(M, 128) / kQR) * static_cast<size_t>(N) * sizeof(float));
+        sums = c.take(sums_bytes(M, N));
         const size_t dx = product_bytes(M, K, N), dw = product_bytes(N, K, M);       // one after the other
         work = c.take(dx > dw ? dx : dw);
         bytes = c.used;
@@ -883,9 +920,7 @@ size_t deepipr_mx4_code_bytes(long long rows, long long cols) {
 size_t deepipr_mx4_scale_bytes(long long rows, long long cols) {
     return rows <= 0 || cols <= 0 ? 0 : static_cast<size_t>(round_up(cols, 128) / 128) * static_cast<size_t>(row_groups(rows)) * 256;
 }
-size_t deepipr_mx4_quantize_workspace_bytes(long long rows, long long cols) {
-    return rows <= 0 || cols <= 0 ? 0 : static_cast<size_t>(round_up(rows, 128) / kQR) * static_cast<size_t>(cols) * sizeof(float);
-}
+size_t deepipr_mx4_quantize_workspace_bytes(long long rows, long long cols) { return rows <= 0 || cols <= 0 ? 0 : sums_bytes(rows, cols); }
 
 int deepipr_mx4_quantize(const void *x, int dtype, long long rows, long long cols, long long row_stride, void *row_codes, void *row_scales,
                          void *col_codes, void *col_scales, float *col_sums, void *workspace, size_t workspace_bytes, void *stream) {
@@ -921,9 +956,7 @@ int deepipr_mx4_dequantize(const void *codes, const void *scales, long long rows
         if (transposed) {                                                                                                            \
             DIPR_LAUNCH(prof, (k_mx4_dequantise_t<T>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), st, c, s, rows, cols, out); \
         } else {                                                                                                                     \
-            const long long want = (rows * ((cols + 7) / 8) + kThreads - 1) / kThreads;                                              \
-            DIPR_LAUNCH(prof, (k_mx4_dequantise<T>), dim3(static_cast<unsigned>(want < 16384 ? want : 16384)), dim3(kThreads), st, c, s, rows, \
-                        cols, out);                                                                                                  \
+            DIPR_LAUNCH(prof, (k_mx4_dequantise<T>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), st, c, s, rows, cols, out);  \
         }                                                                                                                            \
     } while (0)
     switch (dtype) {

@@ -9,7 +9,7 @@ def test_sizes():
     lib = _lib.lib()
     assert [lib.deepipr_mx4_code_bytes(*s) for s in ((1, 1), (3, 128), (3, 129), (0, 5), (5, 0))] == [64, 192, 384, 0, 0]
     assert [lib.deepipr_mx4_scale_bytes(*s) for s in ((1, 1), (64, 128), (65, 129), (0, 5))] == [256, 256, 1024, 0]
-    assert lib.deepipr_mx4_quantize_workspace_bytes(65, 10) == 2 * 10 * 4
+    assert lib.deepipr_mx4_quantize_workspace_bytes(65, 10) == 2 * 10 * 4 and lib.deepipr_mx4_quantize_workspace_bytes(64 * 129, 10) == (130 + 2) * 10 * 4
     assert lib.deepipr_mx4_code_bytes(1 << 33, 200) == (1 << 33) * 128
 
 
