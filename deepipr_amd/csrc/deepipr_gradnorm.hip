@@ -5,12 +5,13 @@
 // Squares and sums are held in 64 bits (1e30 and 1e-30 square without leaving the range), summed in a fixed order.
 //
 // What bounds it: bytes.  The norm reads every gradient once; clipping reads and writes them once more; the step reads gradient,
-// parameter and momentum and writes the last two.  The list travels in the launch arguments (190 tensors a launch): no table in
+// parameter and momentum and writes the last two.  The list travels in the launch arguments (240 tensors a launch): no table in
 // device memory, no copy in front of the launch, and a captured launch keeps its own list.
 //
 // Work split: the tensors are laid end to end in units of 64 elements (a tensor's last unit may be short), and every workgroup takes
 // one run of units, across tensor borders where they fall: tensors of any sizes load all workgroups alike.  There are at most 1024
-// runs, one partial sum each; the next launch's workgroups each add all of them up (8 KB from L2) instead of a launch in between.
+// runs a launch, one partial sum each; the next launch's workgroups each add all of them up (8 KB from L2) instead of a launch in between.
+// The step's run space is the flat parameter buffer itself (parameters start on multiples of 64 floats there).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -21,10 +22,10 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kEntries = 190;                 // entries per launch: 190 * 20 bytes of the 4 KB of launch arguments
-constexpr int kMaxRuns = 1024;                // runs over one whole list: 4 workgroups of 4 waves per CU
+constexpr int kEntries = 240;                 // entries per launch: 240 * 16 bytes of the 4 KB of launch arguments
+constexpr int kMaxRuns = 1024;                // runs per launch: 4 workgroups of 4 waves per CU
 constexpr int kMinUnits = 64;                 // a run is at least 4096 elements
-constexpr int kMaxPartials = 4096;            // runs of all launches of one list: kMaxRuns + one short run per launch
+constexpr int kMaxPartials = 4096;            // runs of all launches of one list
 constexpr long long kEntryMax = 1ll << 29;    // elements per entry; longer tensors take several entries
 constexpr double kClipEps = 1e-6;
 
@@ -34,7 +35,7 @@ struct List {
     const void *ptr[kEntries];
     unsigned count[kEntries];                 // elements | dtype << 30
     unsigned start[kEntries];                 // first unit of the entry in this launch's run space
-    unsigned where[kEntries];                 // step only: the entry's place in param / momentum, in units of 64 floats
+    unsigned long long base;                  // step only: the place of unit 0 in param / momentum, in units of 64 floats
     int n;
     unsigned units;                           // of the whole launch
     unsigned per;                             // units per run
@@ -136,9 +137,9 @@ template <class F> __device__ __forceinline__ void walk(const List &L, F f) {
     for (int i = entry_of(L, lo); i < L.n && L.start[i] < hi; ++i) {
         const unsigned n = L.count[i] & 0x3fffffffu;
         const unsigned s = L.start[i];
-        const unsigned a = lo > s ? (lo - s) * 64u : 0u;
+        const unsigned long long a = lo > s ? (lo - s) * 64ull : 0ull;
         const unsigned b = min((hi - s) * 64ull, static_cast<unsigned long long>(n));
-        if (a < b) f(i, a, b);
+        if (a < b) f(i, static_cast<unsigned>(a), b);                  // (a >= b: a gap in front of the next entry)
     }
 }
 
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(kThreads) void k_sgd_clipped(const List L, const do
     const double gs = factor_of(v, hp[4]) * static_cast<double>(hp[3]);
     walk(L, [&](int i, unsigned a, unsigned b) {
         const float *g = static_cast<const float *>(L.ptr[i]) + a;
-        const size_t off = static_cast<size_t>(L.where[i]) * 64 + a;
+        const size_t off = static_cast<size_t>(L.base + L.start[i]) * 64 + a;
         float *p = param + off, *m = buf + off;
         const unsigned len = b - a;
         unsigned done = 0;
@@ -347,7 +348,7 @@ int survey(const char *what, const DeepiprTensor *t, int n, size_t *elements, un
         *units += (static_cast<unsigned long long>(t[i].count) + 63) / 64;
         *bytes += static_cast<size_t>(t[i].count) * elem_bytes(t[i].dtype);
     }
-    // a launch's units are counted in 32 bits and its runs never exceed kMaxRuns: 190 entries of 2^29 elements stay far below
+    // a launch's units are counted in 32 bits: 240 entries of 2^29 elements stay below
     if (*elements >= (1ull << 42)) return dipr_fail(DEEPIPR_EINVAL, "%s: more than 2^42 elements", what);
     return DEEPIPR_OK;
 }
@@ -368,18 +369,30 @@ template <class F> int disjoint(const char *what, const DeepiprTensor *t, int n,
     return ok ? DEEPIPR_OK : dipr_fail(DEEPIPR_EINVAL, "%s: two tensors of the list share memory", what);
 }
 
-inline unsigned units_per_run(unsigned long long units) {
-    unsigned long long per = (units + kMaxRuns - 1) / kMaxRuns;
+inline long long entries_of(const DeepiprTensor *t, int n) {
+    long long entries = 0;
+    for (int i = 0; i < n; ++i) entries += (t[i].count + kEntryMax - 1) / kEntryMax;
+    return entries;
+}
+// Units per run: every launch of the list gets up to kMaxRuns runs.  -> 0: more launches than kMaxPartials partial sums allow
+inline unsigned units_per_run(const DeepiprTensor *t, int n, unsigned long long units) {
+    const unsigned long long launches = static_cast<unsigned long long>((entries_of(t, n) + kEntries - 1) / kEntries);
+    unsigned long long runs = launches * kMaxRuns;
+    if (2 * launches > kMaxPartials) return 0;
+    if (runs > kMaxPartials - launches) runs = kMaxPartials - launches;           // a launch's last run may be short
+    unsigned long long per = runs ? (units + runs - 1) / runs : 1;
     if (per < kMinUnits) per = kMinUnits;
     return static_cast<unsigned>((per + 3) / 4 * 4);
 }
 
-// Cuts the list into launches and calls f(list, workgroups) for each; f returns false to stop.
-template <class F> bool launches(const DeepiprTensor *t, int n, unsigned per, F f) {
+// Cuts the list into launches and calls f(list, workgroups) for each; f returns false to stop.  PLACED: units are those of the entries'
+// offsets (in ascending order) instead of end to end.
+template <bool PLACED, class F> bool launches(const DeepiprTensor *t, int n, unsigned per, F f) {
     List L;
     L.n = 0;
     L.units = 0;
     L.per = per;
+    L.base = 0;
     auto flush = [&]() {
         if (!L.n) return true;
         const unsigned runs = (L.units + per - 1) / per;
@@ -392,10 +405,15 @@ template <class F> bool launches(const DeepiprTensor *t, int n, unsigned per, F 
         long long at = 0;
         while (at < t[i].count) {
             const long long len = t[i].count - at < kEntryMax ? t[i].count - at : kEntryMax;
+            if (PLACED) {
+                const unsigned long long place = static_cast<unsigned long long>(t[i].offset + at) / 64;
+                if (L.n && place - L.base > (1u << 30) && !flush()) return false;          // start stays within 32 bits
+                if (!L.n) L.base = place;
+                L.units = static_cast<unsigned>(place - L.base);
+            }
             L.ptr[L.n] = static_cast<const char *>(t[i].data) + at * elem_bytes(t[i].dtype);
             L.count[L.n] = static_cast<unsigned>(len) | static_cast<unsigned>(t[i].dtype) << 30;
             L.start[L.n] = L.units;
-            L.where[L.n] = static_cast<unsigned>((t[i].offset + at) / 64);
             L.units += static_cast<unsigned>((len + 63) / 64);
             at += len;
             if (++L.n == kEntries && !flush()) return false;
@@ -409,7 +427,7 @@ template <int P> int partials(const char *what, const DeepiprTensor *t, int n, u
     int at = 0;
     DiprProf prof(DEEPIPR_K_GRAD_NORM);
     prof.bytes = static_cast<double>(bytes);
-    const bool ok = launches(t, n, per, [&](const List &L, int runs) {
+    const bool ok = launches<false>(t, n, per, [&](const List &L, int runs) {
         if (at + runs > kMaxPartials) return false;
         DIPR_LAUNCH(prof, (k_norm_partials<P>), dim3(runs), dim3(kThreads), st, L, part + at);
         at += runs;
@@ -437,14 +455,6 @@ int list_partials(const char *what, const DeepiprTensor *t, int n, int norm_type
     }
 }
 
-// more launches than this would leave partial sums without a place
-inline bool too_many(const DeepiprTensor *t, int n, unsigned long long units, unsigned per) {
-    long long entries = 0;
-    for (int i = 0; i < n; ++i) entries += (t[i].count + kEntryMax - 1) / kEntryMax;
-    const unsigned long long runs = units / per + 1 + (entries + kEntries - 1) / kEntries;
-    return runs > kMaxPartials;
-}
-
 }  // namespace
 
 extern "C" {
@@ -462,8 +472,8 @@ int deepipr_grad_norm(const DeepiprTensor *tensors, int n, int norm_type, float 
     if (rc != DEEPIPR_OK) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     double *part = static_cast<double *>(workspace);
-    const unsigned per = units_per_run(units);
-    if (too_many(tensors, n, units, per)) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
+    const unsigned per = units_per_run(tensors, n, units);
+    if (!per) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
     int used = 0;
     if (elements) {
         rc = list_partials(what, tensors, n, norm_type, per, bytes, part, &used, st);
@@ -495,14 +505,14 @@ int deepipr_grad_clip(const DeepiprTensor *tensors, int n, int norm_type, float 
     if (rc != DEEPIPR_OK) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     double *part = static_cast<double *>(workspace);
-    const unsigned per = units_per_run(units);
-    if (too_many(tensors, n, units, per)) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
+    const unsigned per = units_per_run(tensors, n, units);
+    if (!per) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
     int used = 0;
     rc = list_partials(what, tensors, n, norm_type, per, bytes, part, &used, st);
     if (rc != DEEPIPR_OK) return rc;
     DiprProf prof(DEEPIPR_K_GRAD_CLIP);
     prof.bytes = 2.0 * static_cast<double>(bytes);
-    launches(tensors, n, per, [&](const List &L, int runs) {
+    launches<false>(tensors, n, per, [&](const List &L, int runs) {
         switch (norm_type) {
             case 2: DIPR_LAUNCH(prof, (k_clip<2>), dim3(runs), dim3(kThreads), st, L, part, used, max_norm, norm); break;
             case 1: DIPR_LAUNCH(prof, (k_clip<1>), dim3(runs), dim3(kThreads), st, L, part, used, max_norm, norm); break;
@@ -524,24 +534,23 @@ int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const D
     int rc = check_common(what, 2, workspace, workspace_bytes);
     if (rc == DEEPIPR_OK) rc = survey(what, grads, n, &elements, &units, &bytes);
     if (rc != DEEPIPR_OK) return rc;
-    for (int i = 0; i < n; ++i)
-        if (grads[i].dtype != F32 || grads[i].offset < 0 || grads[i].offset % 64 || grads[i].offset >= (1ll << 37))
-            return dipr_fail(DEEPIPR_EINVAL, "%s: gradient %d: float32, its place a multiple of 64 floats", what, i);
+    long long end = 0;
+    for (int i = 0; i < n; ++i) {
+        if (grads[i].dtype != F32 || grads[i].offset % 64 || grads[i].offset < end || grads[i].offset >= (1ll << 42))
+            return dipr_fail(DEEPIPR_EINVAL, "%s: gradient %d: float32, its place a multiple of 64 floats behind the one before", what, i);
+        end = grads[i].offset + grads[i].count;
+    }
     if (!elements) return dipr_fail(DEEPIPR_EINVAL, "%s: nothing to update", what);
-    rc = disjoint(what, grads, n, [](const DeepiprTensor &t) {
-        return std::make_pair(static_cast<unsigned long long>(t.offset), static_cast<unsigned long long>(t.offset + t.count));
-    });
-    if (rc != DEEPIPR_OK) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     double *part = static_cast<double *>(workspace);
-    const unsigned per = units_per_run(units);
-    if (too_many(grads, n, units, per)) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
+    const unsigned per = units_per_run(grads, n, units);
+    if (!per) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
     int used = 0;
     rc = list_partials(what, grads, n, 2, per, bytes, part, &used, st);
     if (rc != DEEPIPR_OK) return rc;
     DiprProf prof(DEEPIPR_K_SGD);
     prof.bytes = 20.0 * static_cast<double>(elements);
-    launches(grads, n, per, [&](const List &L, int runs) {
+    launches<true>(grads, n, per, [&](const List &L, int runs) {
         DIPR_LAUNCH(prof, k_sgd_clipped, dim3(runs), dim3(kThreads), st, L, part, used, param, momentum_buf, hyper, norm);
         return true;
     });

@@ -326,9 +326,9 @@ class FlatSGD(torch.optim.Optimizer):
             self.sync_hyper()
         elif self._hyper_host is None:
             raise RuntimeError('FlatSGD: call sync_hyper() once before capturing step() into a hipGraph')
-        missing = self._missing_grads()
         if self._clips and not self.comm and self._step_clipped_in_place():
             return loss
+        missing = self._missing_grads()
         if capturing and not self.comm and not missing and not self._clips and self._step_in_place():
             return loss                                   # gradients read where autograd left them: no packing pass
         # The collective layout follows the MODE, which the driver of the step sets identically on every rank -- never
@@ -440,15 +440,14 @@ class FlatSGD(torch.optim.Optimizer):
         """One GPU, clipping: norm and update read the gradients where autograd left them (their addresses travel in the launch
         arguments), eager and captured alike; parameters without a gradient are left alone.  -> False if a gradient cannot be
         addressed that way (the packed path is taken then)."""
-        grads, offsets = [], []
-        for p, off in self._slots:
-            g = p.grad
-            if g is None:
-                continue
-            if g.dtype != torch.float32 or g.device != self.flat_param.device or not g.is_contiguous():
-                return False
-            grads.append(g)
-            offsets.append(off)
+        grads = [p.grad for p, _ in self._slots]
+        offsets = [off for _, off in self._slots]
+        if any(g is None for g in grads):
+            offsets = [off for off, g in zip(offsets, grads) if g is not None]
+            grads = [g for g in grads if g is not None]
+        if {g.dtype for g in grads} - {torch.float32} or {g.device for g in grads} - {self.flat_param.device} or \
+                not all(map(torch.Tensor.is_contiguous, grads)):
+            return False
         if grads:
             P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, grads, offsets, self._hyper, self.grad_norm)
         else:

@@ -2,7 +2,7 @@
 
 The reference steps without clipping (experiments/trainer.py:144-145); this is what stands in front of `optimizer.step()` when a run
 clips.  n = (sum |g|^p)^(1/p) over every element of every tensor, f = min(1, max_norm / (n + 1e-6)), g *= f: the rule of
-torch.nn.utils.clip_grad_norm_, in two launches whatever the number of tensors (up to 190 each), without a host synchronisation, with
+torch.nn.utils.clip_grad_norm_, in two launches whatever the number of tensors (up to 240 each), without a host synchronisation, with
 the sum held in 64 bits and added in a fixed order.  Calls only enqueue work on the current stream and can be captured into a hipGraph;
 a captured call keeps the tensors' addresses.
 

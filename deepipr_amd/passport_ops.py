@@ -954,9 +954,9 @@ class HipKernels:
             span *= size
         return True
 
-    def _tensor_list(self, what, tensors, offsets=None):
-        """-> (device, host rows {address, elements, offset, type} as include/deepipr_hip.h: DeepiprTensor has them)."""
-        rows = np.zeros((len(tensors), 4), dtype=np.int64)
+    def _tensor_list(self, what, tensors, rows=None):
+        """-> (device, host rows {address, elements, offset, type} as include/deepipr_hip.h: DeepiprTensor has them).  rows: the rows with
+        everything but the addresses filled in (float32 tensors of known sizes)."""
         if not tensors:
             raise RuntimeError('%s: an empty list of tensors' % what)
         devs = set(map(torch.Tensor.get_device, tensors))
@@ -964,15 +964,17 @@ class HipKernels:
             raise RuntimeError('deepipr_amd %s runs on the GPU only, all tensors on one device (got %s); there is no CPU fallback'
                                % (what, sorted({str(t.device) for t in tensors})))
         try:
-            rows[:, 3] = [self._DTYPE_CODE[t.dtype] for t in tensors]
+            types = [self._DTYPE_CODE[t.dtype] for t in tensors]
         except KeyError as e:
             raise RuntimeError('deepipr_amd %s takes float32, bfloat16 and float16 tensors (got %s)' % (what, e)) from None
         if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(map(self._dense, tensors)):
             raise RuntimeError('deepipr_amd %s needs dense tensors (no gaps, no element twice)' % what)
+        if rows is None:
+            rows = np.empty((len(tensors), 4), dtype=np.int64)
+            rows[:, 1] = list(map(torch.Tensor.numel, tensors))
+            rows[:, 2] = 0
+        rows[:, 3] = types
         rows[:, 0] = list(map(torch.Tensor.data_ptr, tensors))
-        rows[:, 1] = list(map(torch.Tensor.numel, tensors))
-        if offsets is not None:
-            rows[:, 2] = offsets
         return tensors[0].device, rows
 
     def _norm_scratch(self, dev):
@@ -1003,7 +1005,10 @@ class HipKernels:
         """SGD on clipped gradients that lie where autograd left them: grads[i] belongs at offsets[i] of the flat buffers; `hyper`
         = {lr, momentum, weight_decay, grad_scale, max_norm} on the device; the norm of grad_scale * grads goes to `norm`."""
         dev = _chk(flat_param, flat_buf, hyper, norm)
-        gdev, rows = self._tensor_list('sgd_momentum_step_clipped', grads, offsets)
+        rows = np.empty((len(grads), 4), dtype=np.int64)
+        rows[:, 1] = list(map(torch.Tensor.numel, grads))
+        rows[:, 2] = offsets
+        gdev, rows = self._tensor_list('sgd_momentum_step_clipped', grads, rows)
         if gdev != dev or hyper.numel() != 5 or flat_buf.numel() != flat_param.numel():
             raise RuntimeError('sgd_momentum_step_clipped: five hyper-parameters, buffers of one size, all on one device')
         if rows[:, 2].min() < 0 or (rows[:, 1] + rows[:, 2]).max() > flat_param.numel():

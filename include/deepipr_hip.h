@@ -415,7 +415,7 @@ int deepipr_sgd_momentum_step_multi(float *param, float *momentum_buf, const lon
  *                       autograd left them: d = (f * grad_scale) * g + weight_decay * p; buf = momentum * buf + d; p -= lr * buf, with
  *                       n the 2-norm of grad_scale * g over the whole list.  hyper (device) = {lr, momentum, weight_decay, grad_scale,
  *                       max_norm}: read when the kernel runs, so a captured step follows the host's rewrites.  `offset` of an entry
- *                       is its place in param / momentum_buf (floats, a multiple of 64; places must not overlap).
+ *                       is its place in param / momentum_buf (floats, a multiple of 64; in ascending order, not overlapping).
  * The list is HOST memory, read before the call returns (captured launches keep it); `data` is device memory of `count` elements, any
  * alignment that fits the element type; entries with count 0 are skipped.  workspace: deepipr_grad_norm_workspace_bytes() bytes, used
  * between the launches of one call: calls that may run at the same time need one each.
