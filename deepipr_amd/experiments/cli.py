@@ -49,6 +49,15 @@ def make_parser(private):
     p.add_argument('--reproducible', action='store_true', default=False,
                    help='bit-reproducible steps: MIOpen in immediate mode with its atomic backward-data solver switched '
                         'off (deepipr_amd/reproducible.py) instead of find mode')
+    p.add_argument('--clip-grad-norm', type=float, default=None, metavar='MAX',
+                   help='scale the step\'s gradients down to this global norm (default: no clipping); with several GPUs the norm is that '
+                        'of the averaged gradients')
+    p.add_argument('--linear-format', default='fp32', choices=['fp32', 'mx4'],
+                   help='mx4: the classifier\'s linear layers multiply in 4-bit microscaled floating point, forward and backward '
+                        '(deepipr_amd/mx4.py)')
+    p.add_argument('--round-weights', default=None, choices=['mx4'],
+                   help='with --eval: round every convolution and linear weight to 4 bits first and report what is left of the '
+                        'signature')
     p.add_argument('--eager', action='store_true', default=False,
                    help='eager dispatch instead of hipGraph replay (several GPUs: gradient exchange launched from '
                         'gradient hooks, overlapped with backward)')

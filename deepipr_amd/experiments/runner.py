@@ -126,6 +126,21 @@ def install_keys(args, model, passport_loader, num_classes, device, example):
     passport_generator.set_key(plain, model, key_x.to(device), key_y.to(device))
 
 
+def rounded_report(model, trainer, valid_loader, device, passport):
+    """Test results and signature detection before and after every weight is rounded to 4 bits (models/layers/linear.round_weights_)."""
+    from deepipr_amd.experiments.trainer_private import TesterPrivate
+    from deepipr_amd.models.layers.linear import round_weights_
+    tester = TesterPrivate(model, device)
+    out = {'before': trainer.test(valid_loader)}
+    if passport:
+        out['signature_before'] = tester.test_signature()
+    out['weights'] = round_weights_(model)
+    out['after'] = trainer.test(valid_loader, 'Rounded to 4 bits')
+    if passport:
+        out['signature_after'] = tester.test_signature()
+    return out
+
+
 def run(args, private, train_loader=None, valid_loader=None, wm_loader=None):
     rank, local_rank, world = D.init_from_env(args.get('backend'))
     dev_name = args.get('device') or ('cuda' if torch.cuda.is_available() else None)
@@ -164,6 +179,10 @@ def run(args, private, train_loader=None, valid_loader=None, wm_loader=None):
             passport_loader = wm_loader if wm_loader is not None else \
                 SyntheticLoader(100, 2, size, ncls, device, seed=99)      # the trigger set's synthetic stand-in
         install_keys(args, model, passport_loader, ncls, device, next(iter(train_loader))[0])
+    if args.get('linear_format') == 'mx4':
+        from deepipr_amd.models.layers.linear import use_mx4_linear_
+        use_mx4_linear_(model)
+    clip = args.get('clip_grad_norm')
     # SGD(momentum .9, weight decay 1e-4) as experiments/classification.py:47-50.  Default: FlatSGD (flat buffers,
     # bucketed RCCL all-reduce overlapped with backward, one fused HIP kernel); --ddp: DistributedDataParallel +
     # torch's SGD.
@@ -171,13 +190,20 @@ def run(args, private, train_loader=None, valid_loader=None, wm_loader=None):
     if args.get('ddp'):
         opt = torch.optim.SGD(model.parameters(), lr=args['lr'], momentum=0.9, weight_decay=0.0001,
                               fused=(device.type == 'cuda'))
+        if clip is not None:
+            from deepipr_amd.grad_clip import clip_grad_norm_
+
+            def clip_first(optimizer, _args, _kwargs):
+                clip_grad_norm_(optimizer.param_groups[0]['params'], clip)
+            opt.register_step_pre_hook(clip_first)
         wrap = lambda m: D.replicate(m, device)
     else:
         from deepipr_amd.flat_sgd import FlatSGD
         if passport:
             D.check_keys_materialised(model)
         D.broadcast_state(model, 0)
-        opt = FlatSGD(model.parameters(), lr=args['lr'], momentum=0.9, weight_decay=0.0001)
+        opt = FlatSGD(model.parameters(), lr=args['lr'], momentum=0.9, weight_decay=0.0001,
+                      max_grad_norm=clip)
         wrap = lambda m: m
     sched = torch.optim.lr_scheduler.MultiStepLR(opt, steps, lr_config['gamma']) if len(steps) else None
     # hipGraph replay is the default on the GPU (--eager switches it off): at the reference's batch sizes the eager step is
@@ -204,6 +230,8 @@ def run(args, private, train_loader=None, valid_loader=None, wm_loader=None):
             model.load_state_dict(torch.load(path, map_location='cpu'))
         else:
             print('Warning: No such Experiment -> %s' % path)
+        if args.get('round_weights') == 'mx4':
+            return rounded_report(model, trainer, valid_loader, device, private or args['train_passport'])
         return trainer.test(valid_loader)
     exp_id = [next_experiment_id(root) if rank == 0 else 0]
     if world > 1:

@@ -1,0 +1,92 @@
+"""A linear layer whose products run in 4 bits (deepipr_amd.mx4): what the classifiers' nn.Linear (models/alexnet_passport.py:27-36,
+models/resnet_passport.py:127-129) becomes under `--linear-format mx4`."""
+import torch
+import torch.nn as nn
+
+from deepipr_amd import mx4
+
+
+class Mx4Linear(nn.Linear):
+    """nn.Linear with the same parameters and state_dict.  Training and evaluation quantise weight and input in the call
+    (mx4.linear: output, dx and dw in 4 bits, dbias exact).  A net that only answers can `keep()` its weight in 4 bits instead of
+    quantising it per call; the kept codes are buffers outside the state_dict and are dropped by train(), load_state_dict() and
+    release().  A kept weight has no backward pass, and changing `weight` in place without a new keep() is an error."""
+
+    def __init__(self, in_features, out_features, bias=True, device=None, dtype=None):
+        super().__init__(in_features, out_features, bias, device, dtype)
+        self._without_codes()
+
+    def _without_codes(self):
+        self.register_buffer('kept_codes', None, persistent=False)
+        self.register_buffer('kept_scales', None, persistent=False)
+        self._kept_version = None
+
+    @classmethod
+    def of(cls, linear):
+        """The layer that shares `linear`'s parameters."""
+        new = cls.__new__(cls)
+        nn.Module.__init__(new)
+        new.in_features, new.out_features = linear.in_features, linear.out_features
+        new.weight, new.bias = linear.weight, linear.bias
+        new._without_codes()
+        new.training = linear.training
+        return new
+
+    def keep(self):
+        q = mx4.quantize(self.weight.detach())
+        self.kept_codes, self.kept_scales, self._kept_version = q.codes, q.scales, self.weight._version
+        return self.eval()
+
+    def release(self):
+        self.kept_codes = self.kept_scales = self._kept_version = None
+        return self
+
+    def train(self, mode=True):
+        if mode:
+            self.release()
+        return super().train(mode)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self.release()
+        return super()._load_from_state_dict(*args, **kwargs)
+
+    def forward(self, x):
+        if self.kept_codes is None:
+            return mx4.linear(x, self.weight, self.bias)
+        if self.weight._version != self._kept_version:
+            raise RuntimeError('Mx4Linear: the weight changed after keep(); call keep() again, or release()')
+        return mx4.linear(x, mx4.Mx4Matrix(self.kept_codes, self.kept_scales, self.out_features, self.in_features, 1), self.bias)
+
+    def extra_repr(self):
+        return super().extra_repr() + (', kept in 4 bits' if self.kept_codes is not None else ', mx4')
+
+
+def use_mx4_linear_(model):
+    """Every plain nn.Linear below `model` becomes an Mx4Linear on the same parameters (optimisers built before or after see the same
+    tensors); -> how many."""
+    count = 0
+    for parent in list(model.modules()):
+        for name, child in list(parent.named_children()):
+            if type(child) is nn.Linear:
+                setattr(parent, name, Mx4Linear.of(child))
+                count += 1
+    return count
+
+
+@torch.no_grad()
+def round_weights_(model):
+    """The removal attempt: every convolution and linear weight is rounded to 4 bits in place, output channel by output channel in blocks
+    of 32 -- what a thief who serves the net in 4 bits leaves of it.  Norm layers, biases, passports and signatures stay as they are.
+    -> {parameter name: relative change (2-norm)}."""
+    changed = {}
+    for name, m in model.named_modules():
+        if isinstance(m, (nn.Conv2d, nn.Linear)):
+            w = m.weight
+            flat = w.detach().reshape(w.shape[0], -1)
+            new = mx4.quantize(flat).dequantize(w.dtype)
+            norm = float(flat.double().norm())
+            changed[(name + '.' if name else '') + 'weight'] = float((new.double() - flat.double()).norm()) / norm if norm else 0.0
+            w.copy_(new.reshape(w.shape))
+            if isinstance(m, Mx4Linear):
+                m.release()
+    return changed

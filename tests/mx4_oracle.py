@@ -53,3 +53,16 @@ def unpack(codes, scales, rows, cols):
     s = scales.cpu().numpy().reshape(kp // KP, rg, 2, 32, 2, 2)    # [k128][group][block % 2][row % 32][block / 2][row / 32]
     s = s.transpose(1, 5, 3, 0, 4, 2).reshape(rg * 64, kp // 32)[:rows]
     return full[:, :cols].astype(np.int64), s[:, :-(-cols // 32)].astype(np.int64), not full[:, cols:].any()
+
+
+def pack(code, scale):
+    """(codes [rows, cols], scale bytes [rows, blocks]) -> the library's two buffers."""
+    rows, cols = code.shape
+    kp, rg = -(-cols // KP) * KP, -(-rows // 64)
+    full = np.zeros((rows, kp), dtype=np.uint8)
+    full[:, :cols] = code
+    b = (full[:, 0::2] | full[:, 1::2] << 4).reshape(rows, kp // KP, KP // 2).transpose(1, 0, 2)
+    s = np.zeros((rg * 64, kp // 32), dtype=np.uint8)
+    s[:rows, :scale.shape[1]] = scale
+    s = s.reshape(rg, 2, 32, kp // KP, 2, 2).transpose(3, 0, 5, 2, 4, 1)      # [k128][group][block % 2][row % 32][block / 2][row / 32]
+    return torch.from_numpy(np.ascontiguousarray(b).reshape(-1)), torch.from_numpy(np.ascontiguousarray(s).reshape(-1))

@@ -10,23 +10,7 @@ import torch
 from deepipr_amd import _lib, grad_clip
 from deepipr_amd import passport_ops as P
 from deepipr_amd.flat_sgd import FlatSGD
-from tests.oracle_kernels import OracleKernels
-
-
-class ClipKernels(OracleKernels):
-    """The stand-in with the clipped step: the 64-bit definition."""
-
-    def sgd_momentum_step_clipped(self, flat_param, flat_buf, grads, offsets, hyper, norm):
-        lr, mu, wd, gs, top = [float(v) for v in hyper.tolist()]
-        n = abs(gs) * math.sqrt(sum(float(g.double().square().sum()) for g in grads))
-        f = min(1.0, top / (n + 1e-6))
-        norm.fill_(n)
-        with torch.no_grad():
-            for g, off in zip(grads, offsets):
-                s = slice(off, off + g.numel())
-                d = f * gs * g.reshape(-1) + wd * flat_param[s]
-                flat_buf[s] = mu * flat_buf[s] + d
-                flat_param[s] -= lr * flat_buf[s]
+from tests.lm_kernels import LmKernels
 
 
 def test_host_tensors_and_bad_arguments_are_refused():
@@ -95,7 +79,7 @@ def test_c_entries_refuse_before_any_launch():
 @pytest.mark.parametrize('top', [0.05, 1e6])
 @pytest.mark.parametrize('unused', [False, True])
 def test_flat_sgd_clips_like_torch(monkeypatch, top, unused):
-    monkeypatch.setattr(P, 'kernels', ClipKernels())
+    monkeypatch.setattr(P, 'kernels', LmKernels())
     torch.manual_seed(3)
 
     def net():

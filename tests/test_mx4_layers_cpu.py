@@ -1,0 +1,135 @@
+"""Mx4Linear, use_mx4_linear_, round_weights_ and the command-line options, on the CPU stand-in of the kernels."""
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+from deepipr_amd import mx4
+from deepipr_amd import passport_ops as P
+from deepipr_amd.models.layers.linear import Mx4Linear, round_weights_, use_mx4_linear_
+from tests import mx4_oracle as oracle
+from tests.lm_kernels import LmKernels
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(autouse=True)
+def cpu_kernels(monkeypatch):
+    monkeypatch.setattr(P, 'kernels', LmKernels())
+    monkeypatch.chdir(ROOT)
+
+
+def _v(x, dim):
+    return torch.from_numpy(np.ascontiguousarray(oracle.values(x, dim))).float()
+
+
+def test_the_oracle_packs_what_it_unpacks():
+    x = np.random.RandomState(0).randn(70, 200)
+    code, scale, _ = oracle.quantise(x)
+    c, s = oracle.pack(code, scale)
+    got_code, got_scale, clean = oracle.unpack(c, s, 70, 200)
+    assert clean and np.array_equal(got_code, code) and np.array_equal(got_scale, scale)
+
+
+def test_layer_matches_its_formula_and_shares_parameters():
+    torch.manual_seed(0)
+    plain = nn.Sequential(nn.Linear(40, 24), nn.ReLU(), nn.Sequential(nn.Linear(24, 10, bias=False)))
+    keys, params = list(plain.state_dict()), [id(p) for p in plain.parameters()]
+    assert use_mx4_linear_(plain) == 2 and use_mx4_linear_(plain) == 0
+    assert list(plain.state_dict()) == keys and [id(p) for p in plain.parameters()] == params
+    lin = plain[0]
+    x = torch.randn(7, 40, requires_grad=True)
+    y = lin(x)
+    dy = torch.randn(7, 24)
+    y.backward(dy)
+    assert torch.allclose(y, _v(x, 1) @ _v(lin.weight, 1).t() + lin.bias, atol=1e-5)
+    assert torch.allclose(x.grad, _v(dy, 1) @ _v(lin.weight, 0), atol=1e-5)
+    assert torch.allclose(lin.weight.grad, _v(dy, 0).t() @ _v(x, 0), atol=1e-5)
+    assert torch.allclose(lin.bias.grad, dy.sum(0), atol=1e-5)
+    assert 'mx4' in repr(lin)
+
+
+def test_keep_release_and_stale_weights():
+    torch.manual_seed(1)
+    lin = Mx4Linear(40, 8)
+    x = torch.randn(3, 40)
+    with torch.no_grad():
+        want = lin(x)
+        lin.keep()
+        assert not lin.training and 'kept' in repr(lin) and torch.equal(lin(x), want)
+        assert sorted(lin.state_dict()) == ['bias', 'weight'] and len(list(lin.buffers())) == 2
+    with pytest.raises(RuntimeError, match='no backward'):
+        lin(x)                                                     # the bias asks for a gradient
+    with torch.no_grad():
+        lin.weight.mul_(2)
+        with pytest.raises(RuntimeError, match='keep'):
+            lin(x)
+        lin.keep()
+        assert torch.equal(lin(x), 2 * (want - lin.bias) + lin.bias)
+        lin.load_state_dict({'weight': torch.zeros(8, 40), 'bias': torch.ones(8)})
+        assert lin.kept_codes is None and torch.equal(lin(x), torch.ones(3, 8))
+        lin.keep()
+        lin.train()
+        assert lin.kept_codes is None and lin.training
+
+
+def test_round_weights():
+    torch.manual_seed(2)
+    net = nn.Sequential(nn.Conv2d(3, 8, 3), nn.BatchNorm2d(8), nn.Flatten(), Mx4Linear(8, 5))
+    before = {k: v.clone() for k, v in net.state_dict().items()}
+    change = round_weights_(net)
+    assert sorted(change) == ['0.weight', '3.weight'] and all(0.01 < v < 0.3 for v in change.values())
+    for k, v in net.state_dict().items():
+        if k in change:
+            flat = before[k].reshape(v.shape[0], -1)
+            assert torch.equal(v.reshape(v.shape[0], -1), _v(flat, 1))
+        else:
+            assert torch.equal(v, before[k])
+    assert all(v == 0.0 for v in round_weights_(net).values())      # rounded once is rounded for good
+
+
+@pytest.mark.parametrize('extra', [[], ['--linear-format', 'mx4']])
+def test_train_v1_with_clipping(tmp_path, extra):
+    sys.path.insert(0, ROOT)
+    import train_v1
+    argv = ['--arch', 'alexnet', '--train-passport', '--key-type', 'random', '--epochs', '1', '--batch-size', '4', '--synthetic-samples', '8',
+            '--device', 'cpu', '--logdir', str(tmp_path), '--clip-grad-norm', '0.5'] + extra
+    out = train_v1.main(argv)
+    model = out['model']
+    assert isinstance(model.classifier, Mx4Linear) == bool(extra)
+    assert np.isfinite(out['history'][0]['train_loss'])
+    rep = train_v1.main(argv + ['--eval', '--exp-id', '1', '--round-weights', 'mx4'])
+    assert rep['weights'] and set(rep['signature_before']) == set(rep['signature_after']) != set()
+    assert np.isfinite(rep['after']['loss'])
+
+
+def test_clipping_keeps_the_step_small(tmp_path):
+    """max_grad_norm 0 with no weight decay on the bias-free first step: momentum alone moves nothing."""
+    from deepipr_amd.flat_sgd import FlatSGD
+    p = nn.Parameter(torch.randn(5))
+    opt = FlatSGD([p], lr=0.1, momentum=0.9, weight_decay=0.0, max_grad_norm=0.0)
+    before = p.detach().clone()
+    p.grad = torch.randn(5)
+    opt.step()
+    assert torch.equal(p.detach(), before) and float(opt.grad_norm) == pytest.approx(float(p.grad.norm()))
+
+
+def test_a_step_of_the_set_together():
+    """A 4-bit layer, its loss, backward, clipped FlatSGD step: what the pieces give one by one."""
+    from deepipr_amd.flat_sgd import FlatSGD
+    torch.manual_seed(3)
+    lin = Mx4Linear(64, 10)
+    w0, b0 = lin.weight.detach().clone(), lin.bias.detach().clone()
+    opt = FlatSGD(lin.parameters(), lr=0.5, momentum=0.0, weight_decay=0.0, max_grad_norm=0.1)
+    x, t = torch.randn(16, 64), torch.randint(0, 10, (16,))
+    nn.functional.cross_entropy(lin(x), t).backward()
+    gw, gb = lin.weight.grad.clone(), lin.bias.grad.clone()
+    opt.step()
+    n = float(torch.cat([gw.reshape(-1), gb]).double().norm())
+    assert n > 0.1 and float(opt.grad_norm) == pytest.approx(n, rel=1e-6)
+    f = 0.1 / (n + 1e-6)
+    assert torch.allclose(lin.weight, w0 - 0.5 * f * gw, atol=1e-6) and torch.allclose(lin.bias, b0 - 0.5 * f * gb, atol=1e-6)
+    assert mx4.quantize(lin.weight.detach()).shape == (10, 64)
