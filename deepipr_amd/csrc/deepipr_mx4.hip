@@ -406,16 +406,47 @@ struct Product {
     long long first, last;                               // rows first .. last - 1 of the output (first a multiple of 64)
     int kt, splits;                                      // splits > 1: out is float [splits][M][N], split i adds up its share of the steps
     void *out;
+    const void *x;                                       // a in its own type instead of a / sa (k_mx4_gemm_rows with X >= 0)
+    long long x_stride, K;
+    int x_vec;                                           // its rows start on 16-byte boundaries
 };
+
+// 32 values of a row from column k on, zero behind K
+template <int X> __device__ __forceinline__ void load_block(const void *x, long long at, long long k, long long K, int vec, float *v) {
+    if (vec && k + 32 <= K) {
+#pragma unroll
+        for (int i = 0; i < 32; i += X == F32 ? 4 : 8) {
+            const u32x4 q = load16<X>(x, at + i);
+            if (X == F32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i + j] = __uint_as_float(q[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[(i + 2 * j) & 31] = X == BF16 ? __uint_as_float(q[j] << 16) : f16_to_f32(q[j] & 0xffffu);
+                    v[(i + 2 * j + 1) & 31] = X == BF16 ? __uint_as_float(q[j] & 0xffff0000u) : f16_to_f32(q[j] >> 16);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = k + i < K ? load1<X>(x, at + i) : 0.0f;
+    }
+}
 
 // Few rows (at most 16 MT): bound by reading b once.  A workgroup of eight waves takes 16 rows of b and all of a; wave i the steps
 // i, i + 8, ... of the columns, four of them on their way at once: with 16 rows a workgroup, 4096 rows of b fill 256 CUs and all
 // of b is asked for at once.  v_mfma_scale_f32_16x16x128_f8f6f4: lane l gives block l / 16 of row l % 16.  The waves' sums are added
 // through LDS in wave order.
-template <int T, int MT>
+// X >= 0 (MT = 1): a comes in its own type X and the workgroup first quantises all of it into LDS, one block a thread and turn, while its
+// first fetches of b are on their way.  Every workgroup does so again, but a launch is saved (3 us of the host's time, 2 of the card's).
+constexpr int kFusedBlocks = 2048;               // rows x blocks: at most four a thread
+template <int T, int MT, int X>
 __global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product P) {
     constexpr int U = 4;
     __shared__ f32x4 red[8][MT][64];
+    __shared__ u32x4 codes[X >= 0 ? kFusedBlocks : 1];
+    __shared__ unsigned char scales[X >= 0 ? kFusedBlocks : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long n0 = static_cast<long long>(blockIdx.x) * 16;
     const int r = lane & 15, blk = lane >> 4;
@@ -427,39 +458,66 @@ __global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product P) {
     const unsigned *qb = P.sb + word_of(brow), *qa[MT];
     const int hb = byte_of(brow);
     int ha[MT];
+    if (X < 0) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const long long row = min(P.first + t * 16 + r, P.last - 1);
-        pa[t] = P.a + row * 64 + blk * 16;
-        qa[t] = P.sa + word_of(row);
-        ha[t] = byte_of(row);
+        for (int t = 0; t < MT; ++t) {
+            const long long row = min(P.first + t * 16 + r, P.last - 1);
+            pa[t] = P.a + row * 64 + blk * 16;
+            qa[t] = P.sa + word_of(row);
+            ha[t] = byte_of(row);
+        }
     }
     const long long gm = row_groups(P.M) * 64, gn = row_groups(P.N) * 64;
     f32x4 acc[MT] = {};
-    for (int k0 = wave; k0 < P.kt; k0 += 8 * U) {
-        u32x4 fb[U], fa[U][MT];
-        unsigned wb[U], wa[U][MT];
+    u32x4 fb[U], fa[U][MT];
+    unsigned wb[U], wa[U][MT];
+    const auto fetch = [&](int k0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long long k = min(k0 + 8 * u, P.kt - 1);
             fb[u] = *reinterpret_cast<const u32x4 *>(pb + k * P.N * 64);
             wb[u] = qb[k * gn];
+            if (X < 0) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                fa[u][t] = *reinterpret_cast<const u32x4 *>(pa[t] + k * P.M * 64);
-                wa[u][t] = qa[t][k * gm];
+                for (int t = 0; t < MT; ++t) {
+                    fa[u][t] = *reinterpret_cast<const u32x4 *>(pa[t] + k * P.M * 64);
+                    wa[u][t] = qa[t][k * gm] >> ha[t];
+                }
             }
         }
+    };
+    fetch(wave);
+    if (X >= 0) {
+        const int per = P.kt * 4, blocks = static_cast<int>(P.M) * per;
+        for (int i = threadIdx.x; i < blocks; i += 512) {
+            const int row = i / per;
+            const long long k = static_cast<long long>(i - row * per) * 32;
+            float v[32];
+            load_block<X < 0 ? 0 : X>(P.x, row * P.x_stride + k, k, P.K, P.x_vec, v);
+            unsigned code;
+            codes[i] = quantise32(v, code);
+            scales[i] = static_cast<unsigned char>(code);
+        }
+        __syncthreads();
+    }
+    for (int k0 = wave; k0 < P.kt; k0 += 8 * U) {
+        if (k0 != wave) fetch(k0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (k0 + 8 * u >= P.kt) break;
+            if (X >= 0) {
+                const int at = (r * P.kt + k0 + 8 * u) * 4 + blk;
+                const bool mine = r < static_cast<int>(P.M);
+                fa[u][0] = mine ? codes[at] : u32x4{0, 0, 0, 0};
+                wa[u][0] = mine ? scales[at] : 0;
+            }
             const i32x8 bv = {static_cast<int>(fb[u].x), static_cast<int>(fb[u].y), static_cast<int>(fb[u].z), static_cast<int>(fb[u].w), 0, 0, 0, 0};
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const i32x8 av = {static_cast<int>(fa[u][t].x), static_cast<int>(fa[u][t].y), static_cast<int>(fa[u][t].z),
                                   static_cast<int>(fa[u][t].w), 0, 0, 0, 0};
                 acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv, av, acc[t], 4, 4, 0, static_cast<int>(wb[u] >> hb), 0,
-                                                                          static_cast<int>(wa[u][t] >> ha[t]));
+                                                                          static_cast<int>(wa[u][t]));
             }
         }
     }
@@ -515,8 +573,9 @@ __global__ __launch_bounds__(kThreads) void k_mx4_gemm_sum(const float *__restri
 }
 
 // Large products: a workgroup of four waves takes a tile of 64 TM x 64 TN outputs, a wave 32 TM x 32 TN of it (TM, TN even).
-// A step is 128 columns.  Its codes and scales go to LDS without passing registers, into a ring of four stages and up to four steps
-// ahead of their use; the fragments of the next 64 columns are read from LDS while the matrix cores work on these.  Fetches and reads
+// A step is 128 columns.  Its codes and scales go to LDS without passing registers, into a ring of STAGES stages and as many steps ahead
+// of their use (three: 128 x 128 tiles then sit three to a CU, 5 % faster than two with four stages; 256 x 256 tiles take the same time
+// with three and four); the fragments of the next 64 columns are read from LDS while the matrix cores work on these.  Fetches and reads
 // stand between the matrix instructions, a few behind every fourth: a wave issues in order, and a run of fetches would hold up what
 // comes behind it (measured on 8192^3: a step's fetches in one run 295 us, spread out 253).
 //   codes in LDS: 64 bytes a row, the 16-byte block b of row r at slot b ^ (r / 4 % 4): the 16 lanes that LDS serves at once (rows
@@ -534,19 +593,20 @@ __device__ __forceinline__ void to_lds4(const void *src, unsigned to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(to) : "memory", "m0");
 }
 
-template <int TM, int TN> struct Tile {
+template <int TM, int TN, int STAGES> struct Tile {
     static constexpr int BM = 64 * TM, BN = 64 * TN;
-    static constexpr int kCodes = (BM + BN) * 64, kStage = kCodes + (BM + BN) * 4, kStages = 4;
-    static constexpr int kCodeLoads = (BM + BN) / 64, kWordLoads = (BM + BN) / 256;         // 1 KB and 256 B pieces per wave and step
+    static constexpr int kCodes = (BM + BN) * 64, kStage = kCodes + (BM + BN) * 4, kStages = STAGES;
+    static constexpr int kCodeLoads = (BM + BN) / 64, kWordLoads = ((BM + BN) / 64 + 3) / 4;   // 1 KB and 256 B pieces per wave and step
     static constexpr int kLoads = kCodeLoads + kWordLoads;
     static constexpr int kGroups = TM * TN / 4;                                             // of four matrix instructions, per 64 columns
 };
 
 __device__ __forceinline__ int slot_of(int r, int b) { return b ^ (r >> 2 & 3); }
 
-template <int T, int TM, int TN>
+template <int T, int TM, int TN, int STAGES>
 __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P) {
-    typedef Tile<TM, TN> G;
+    typedef Tile<TM, TN, STAGES> G;
+    static_assert(G::kStages * G::kStage >= 4 * 32 * (32 * TN + 4) * 4, "the waves' output strips take the stages' place");
     __shared__ __align__(16) unsigned char lds[G::kStages * G::kStage];
     const long long M = P.M, N = P.N;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -576,7 +636,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P)
     }
 #pragma unroll
     for (int j = 0; j < G::kWordLoads; ++j) {
-        const int piece = wave * G::kWordLoads + j;
+        const int piece = min(wave * G::kWordLoads + j, (G::BM + G::BN) / 64 - 1);      // (a spare one fetches the last again)
         const bool of_a = piece < G::BM / 64;
         const long long groups = of_a ? row_groups(M) : row_groups(N);
         const long long g = of_a ? min(m0 / 64 + piece, groups - 1) : min(n0 / 64 + piece - G::BM / 64, groups - 1);
@@ -586,15 +646,15 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P)
     const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds));
     // piece j of step s, to its stage; the address moves on to the next step (behind the last one: the last one again, so that the number
     // of fetches on their way is the same in every step)
-    auto fetch = [&](int s, int j) {
-        const unsigned base = lds0 + (s & 3) * G::kStage;
+    auto fetch = [&](int s, int stage, int j) {
+        const unsigned base = lds0 + stage * G::kStage;
         const bool on = s + 1 < kt;
         if (j < G::kCodeLoads) {
             to_lds16(src[j], base + (wave * G::kCodeLoads + j) * 1024);
             src[j] += on ? move[j] : 0;
         } else {
             const int i = j - G::kCodeLoads;
-            to_lds4(ssrc[i], base + G::kCodes + (wave * G::kWordLoads + i) * 256);
+            to_lds4(ssrc[i], base + G::kCodes + min(wave * G::kWordLoads + i, (G::BM + G::BN) / 64 - 1) * 256);
             ssrc[i] += on ? smove[i] : 0;
         }
     };
@@ -608,20 +668,20 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P)
         unsigned b[TN / 2], a[TM / 2];
     };
     // fragment i of the TN + TM ones
-    auto read = [&](Frags &f, int s, int h, int i) {
-        const unsigned char *base = lds + (s & 3) * G::kStage;
+    auto read = [&](Frags &f, int stage, int h, int i) {
+        const unsigned char *base = lds + stage * G::kStage;
         if (i < TN) f.b[i] = *reinterpret_cast<const u32x4 *>(base + G::BM * 64 + (wn + i) * 2048 + frag[h]);
         else f.a[i - TN] = *reinterpret_cast<const u32x4 *>(base + (wm + i - TN) * 2048 + frag[h]);
     };
-    auto read_word = [&](Words &w, int s, int i) {
-        const unsigned char *base = lds + (s & 3) * G::kStage + G::kCodes;
+    auto read_word = [&](Words &w, int stage, int i) {
+        const unsigned char *base = lds + stage * G::kStage + G::kCodes;
         if (i < TN / 2) w.b[i] = reinterpret_cast<const unsigned *>(base + G::BM * 4 + (wn / 2 + i) * 256)[lane];
         else w.a[i - TN / 2] = reinterpret_cast<const unsigned *>(base + (wm / 2 + i - TN / 2) * 256)[lane];
     };
     f32x16 acc[TN][TM] = {};
-    // 64 columns: H the half of the step they are; behind each group of four matrix instructions a share of the next 64 columns' reads and
-    // of the fetches FIRST .. LAST - 1 of step FS
-#define MX4_COLUMNS(F, W, H, NF, NS, NH, WORDS, NW, FS, FIRST, LAST)                                                               \
+    // 64 columns, half H of their step: in front of each group of four matrix instructions a share of the next 64 columns' reads (stage NS,
+    // half NH) and of the fetches FIRST .. LAST - 1 of step FS to stage FT
+#define MX4_COLUMNS(F, W, H, NF, NS, NH, WORDS, NW, FS, FT, FIRST, LAST)                                                           \
     _Pragma("unroll") for (int g = 0; g < G::kGroups; ++g) {                                                                       \
         const int i = g % (TN / 2) * 2, j = g / (TN / 2) * 2;                                                                      \
         if (WORDS) {                                                                                                               \
@@ -629,7 +689,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P)
                 read_word(NW, NS, x);                                                                                              \
         }                                                                                                                          \
         _Pragma("unroll") for (int x = (TM + TN) * g / G::kGroups; x < (TM + TN) * (g + 1) / G::kGroups; ++x) read(NF, NS, NH, x); \
-        _Pragma("unroll") for (int x = FIRST + (LAST - FIRST) * g / G::kGroups; x < FIRST + (LAST - FIRST) * (g + 1) / G::kGroups; ++x) fetch(FS, x); \
+        _Pragma("unroll") for (int x = FIRST + (LAST - FIRST) * g / G::kGroups; x < FIRST + (LAST - FIRST) * (g + 1) / G::kGroups; ++x) fetch(FS, FT, x); \
         acc[i][j] = mfma<2 * H, 2 * H>(F.b[i], F.a[j], acc[i][j], W.b[i / 2], W.a[j / 2]);                                         \
         acc[i + 1][j] = mfma<2 * H + 1, 2 * H>(F.b[i + 1], F.a[j], acc[i + 1][j], W.b[i / 2], W.a[j / 2]);                         \
         acc[i][j + 1] = mfma<2 * H, 2 * H + 1>(F.b[i], F.a[j + 1], acc[i][j + 1], W.b[i / 2], W.a[j / 2]);                         \
@@ -642,28 +702,31 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P)
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STEPS) * G::kLoads) : "memory");     \
         __builtin_amdgcn_s_barrier();                                                            \
     } while (0)
-    constexpr int kHalf = G::kLoads / 2;
+    constexpr int kHalf = G::kLoads / 2, kAhead = STAGES - 1;
 #pragma unroll
-    for (int s = 0; s < 3; ++s)
+    for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-        for (int j = 0; j < G::kLoads; ++j) fetch(s, j);
+        for (int j = 0; j < G::kLoads; ++j) fetch(s, s, j);
 #pragma unroll
-    for (int j = 0; j < kHalf; ++j) fetch(3, j);
+    for (int j = 0; j < kHalf; ++j) fetch(kAhead, kAhead, j);
     Frags f0, f1;
     Words w, next;
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * G::kLoads + kHalf) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kAhead - 1) * G::kLoads + kHalf) : "memory");
     __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int i = 0; i < TM + TN; ++i) read(f0, 0, 0, i);
 #pragma unroll
     for (int i = 0; i < (TM + TN) / 2; ++i) read_word(w, 0, i);
+    int here = 0;                                        // the stage of step k
     for (int k = 0; k < kt; ++k) {
-        MX4_COLUMNS(f0, w, 0, f1, k, 1, false, next, k + 3, kHalf, G::kLoads)
-        // step k + 1 is in LDS (steps k + 2 and k + 3 may be on their way); behind the barrier every wave has read stage k & 3, which is
-        // free for step k + 4
-        MX4_ARRIVED(2);
-        MX4_COLUMNS(f1, w, 1, f0, k + 1, 0, true, next, k + 4, 0, kHalf)
+        const int after = here + 1 == STAGES ? 0 : here + 1, last = here == 0 ? STAGES - 1 : here - 1;
+        MX4_COLUMNS(f0, w, 0, f1, here, 1, false, next, k + kAhead, last, kHalf, G::kLoads)
+        // step k + 1 is in LDS (the ones behind it may be on their way); behind the barrier every wave has read stage `here`, which is free
+        // for step k + STAGES
+        MX4_ARRIVED(STAGES - 2);
+        MX4_COLUMNS(f1, w, 1, f0, after, 0, true, next, k + STAGES, here, 0, kHalf)
         w = next;
+        here = after;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // nothing may arrive in LDS behind the last use of a stage
 #undef MX4_ARRIVED
@@ -754,26 +817,26 @@ template <int T> void launch_product(DiprProf &prof, const Plan &plan, Product P
         Q.first = plan.tail ? P.M - plan.tail : 0;
         const dim3 grid(static_cast<unsigned>((P.N + 15) / 16));
         const long long rows = Q.last - Q.first;
-        if (rows <= 16) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 1>), grid, dim3(512), st, Q);
-        else if (rows <= 32) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 2>), grid, dim3(512), st, Q);
-        else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4>), grid, dim3(512), st, Q);
+        if (rows <= 16) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 1, -1>), grid, dim3(512), st, Q);
+        else if (rows <= 32) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 2, -1>), grid, dim3(512), st, Q);
+        else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, -1>), grid, dim3(512), st, Q);
         if (plan.form == Plan::kRows) return;
         P.last -= plan.tail;
     }
     if (plan.form == Plan::kLarge) {
-        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 4, 4>), dim3(static_cast<unsigned>(tiles_of(P.last, P.N, 256))), block, st, P);
+        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 4, 4, 3>), dim3(static_cast<unsigned>(tiles_of(P.last, P.N, 256))), block, st, P);
         return;
     }
     const unsigned tiles = static_cast<unsigned>(tiles_of(P.last, P.N, 128));
     if (plan.splits == 1) {
-        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 2, 2>), dim3(tiles), block, st, P);
+        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 2, 2, 3>), dim3(tiles), block, st, P);
         return;
     }
     Product Q = P;
     Q.splits = plan.splits;
     Q.out = part;
     Q.bias = nullptr;
-    DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<F32, 2, 2>), dim3(tiles * plan.splits), block, st, Q);
+    DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<F32, 2, 2, 3>), dim3(tiles * plan.splits), block, st, Q);
     const long long want = (P.M * ((P.N + 3) / 4) + kThreads - 1) / kThreads;
     hipLaunchKernelGGL((k_mx4_gemm_sum<T>), dim3(static_cast<unsigned>(want < 8192 ? want : 8192)), block, 0, st, part, plan.splits, P.bias, P.bias_type,
                        P.M, P.N, P.out);
@@ -823,7 +886,7 @@ inline size_t product_bytes(long long M, long long N, long long K) {
 void product(const void *a, const void *sa, const void *b, const void *sb, const void *bias, int bias_dtype, long long M, long long N, long long K,
              void *out, int dtype, void *workspace, hipStream_t st) {
     const long long steps = round_up(K, 128) / 128;
-    Product P;
+    Product P = {};
     P.a = static_cast<const unsigned char *>(a);
     P.b = static_cast<const unsigned char *>(b);
     P.sa = static_cast<const unsigned *>(sa);
@@ -843,6 +906,33 @@ void product(const void *a, const void *sa, const void *b, const void *sb, const
         case F32: launch_product<F32>(prof, p, P, static_cast<float *>(workspace), st); break;
         case BF16: launch_product<BF16>(prof, p, P, static_cast<float *>(workspace), st); break;
         default: launch_product<F16>(prof, p, P, static_cast<float *>(workspace), st); break;
+    }
+}
+
+// The same with a in its own type, for at most 16 rows (out of a's type): one launch
+void product_of_rows(const void *x, int dtype, long long x_stride, const void *b, const void *sb, const void *bias, int bias_dtype, long long M,
+                     long long N, long long K, void *out, hipStream_t st) {
+    Product P = {};
+    P.b = static_cast<const unsigned char *>(b);
+    P.sb = static_cast<const unsigned *>(sb);
+    P.bias = bias;
+    P.bias_type = bias_dtype;
+    P.M = P.last = M;
+    P.N = N;
+    P.K = K;
+    P.kt = static_cast<int>(round_up(K, 128) / 128);
+    P.splits = 1;
+    P.out = out;
+    P.x = x;
+    P.x_stride = x_stride;
+    P.x_vec = aligned(x, 16) && (M == 1 || x_stride * elem_bytes(dtype) % 16 == 0);
+    DiprProf prof(DEEPIPR_K_MX4_MATMUL);
+    prof.bytes = 2.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+    const dim3 grid(static_cast<unsigned>((N + 15) / 16)), block(512);
+    switch (dtype) {
+        case F32: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<F32, 1, F32>), grid, block, st, P); break;
+        case BF16: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<BF16, 1, BF16>), grid, block, st, P); break;
+        default: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<F16, 1, F16>), grid, block, st, P); break;
     }
 }
 
@@ -1011,6 +1101,10 @@ int deepipr_mx4_linear_fwd(const void *x, int x_dtype, long long x_stride, const
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < f.bytes || (s.bytes && (!saved || !aligned(saved, 16) || saved_bytes < s.bytes)))
         return dipr_fail(DEEPIPR_EINVAL, "%s: scratch or saved memory too small or misaligned", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (kept && M <= 16 && M * (round_up(K, 128) / 32) <= kFusedBlocks) {
+        product_of_rows(x, x_dtype, x_stride, w_codes, w_scales, bias, bias_dtype, M, N, K, out, st);
+        return dipr_check_launch(what);
+    }
     quantise(x, x_dtype, M, K, x_stride, f.x.codes, f.x.scales, s.x_t.codes, s.x_t.scales, nullptr, nullptr, st);
     if (!kept) quantise(w, w_dtype, N, K, w_stride, f.w.codes, f.w.scales, s.w_t.codes, s.w_t.scales, nullptr, nullptr, st);
     product(f.x.codes, f.x.scales, kept ? w_codes : f.w.codes, kept ? w_scales : f.w.scales, bias, bias_dtype, M, N, K, out, x_dtype, f.work, st);

@@ -219,6 +219,25 @@ def test_linear_and_its_gradients(mnk, dtype):
     assert torch.equal(dx2, dx)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m', [1, 3, 16, 17, 40])
+def test_rows_on_kept_weights(m, dtype):
+    """Up to 16 rows are quantised inside the product, more by a launch of their own: the same codes, so the same sums, for every alignment,
+    ragged last blocks and blocks that are not numbers."""
+    from deepipr_amd import mx4
+    for n, k in ((1, 1), (40, 31), (130, 300), (17, 2048), (300, 9216)):
+        big = _random((m, k + 9), dtype, seed=m + k, spread=False)
+        if k > 40 and m > 2:
+            big[2, 37] = float('nan')
+        q = mx4.quantize(_codes(n, k, 23, (0, 1)).to(DEV))
+        bias = _random((n,), torch.float32, 24, False)
+        for x in (big[:, :k].contiguous(), big[:, 1:k + 1], big[:, 8:k + 8], big[:, :k]):
+            want = mx4.matmul(mx4.quantize(x), q, bias, dtype)
+            got = mx4.linear(x, q, bias)
+            assert got.dtype == dtype and torch.equal(torch.isnan(got), torch.isnan(want))
+            assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
 def test_gradients_against_differences():
     """Inputs on the 4-bit grid in every direction: rounding changes nothing, the layer is the linear map, and one-sided differences of
     <y, dy> along steps that stay on the grid are the gradients."""
