@@ -119,15 +119,29 @@ __device__ __forceinline__ u32x4 quantise32(float *v, unsigned &code) {
 // Bound by bytes: each value is read from HBM once for both directions.
 constexpr int kQR = 64, kQC = 128, kQP = kQC + 4;        // pitch: 16-byte rows shifted by four banks each
 
+struct Matrix {
+    const void *x;
+    long long R, C, stride;
+    int vec;                                             // rows start on 16-byte boundaries
+    unsigned char *row_codes, *col_codes;
+    unsigned *row_scales, *col_scales;
+    float *sums;
+};
+// `first` workgroups take matrix A, the others B (a layer's input and weight in one launch)
 template <int T, bool ROW, bool COL, bool SUM>
-__global__ __launch_bounds__(kThreads) void k_mx4_quantise(const void *__restrict__ x, long long R, long long C, long long stride, int vec,
-                                                           unsigned char *__restrict__ row_codes, unsigned *__restrict__ row_scales,
-                                                           unsigned char *__restrict__ col_codes, unsigned *__restrict__ col_scales,
-                                                           float *__restrict__ sums) {
+__global__ __launch_bounds__(kThreads) void k_mx4_quantise(const Matrix A, const Matrix B, unsigned first) {
+    const Matrix &m = blockIdx.x < first ? A : B;
+    const unsigned id = blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
+    const void *__restrict__ x = m.x;
+    const long long R = m.R, C = m.C, stride = m.stride;
+    const int vec = m.vec;
+    unsigned char *__restrict__ row_codes = m.row_codes, *__restrict__ col_codes = m.col_codes;
+    unsigned *__restrict__ row_scales = m.row_scales, *__restrict__ col_scales = m.col_scales;
+    float *__restrict__ sums = m.sums;
     __shared__ float s[kQR * kQP];
     __shared__ unsigned char sc[2][256];
     const long long tiles_c = (C + kQC - 1) / kQC;
-    const long long r0 = static_cast<long long>(blockIdx.x) / tiles_c * kQR, c0 = static_cast<long long>(blockIdx.x) % tiles_c * kQC;
+    const long long r0 = id / tiles_c * kQR, c0 = id % tiles_c * kQC;
     const int tid = threadIdx.x;
     constexpr int V = T == F32 ? 4 : 8, PER = kQC / V, LOADS = kQR * PER / kThreads;      // 16-byte pieces
     const auto put = [&](int i, u32x4 q) {
@@ -440,7 +454,9 @@ template <int X> __device__ __forceinline__ void load_block(const void *x, long 
 // through LDS in wave order.
 // X >= 0 (MT = 1): a comes in its own type X and the workgroup first quantises all of it into LDS, one block a thread and turn, while its
 // first fetches of b are on their way.  Every workgroup does so again, but a launch is saved (3 us of the host's time, 2 of the card's).
-constexpr int kFusedBlocks = 2048;               // rows x blocks: at most four a thread
+// Measured (us, fused / apart): 1 x 4096 x 9216 fp32 5.5 / 8.6, 4 x: 8.3 / 8.5, 8 x 4096 x 4096 7.0 / 6.9; 16 x 4096 x 4096 bf16 6.9 / 8.0,
+// fp32 10.9 / 7.0: up to 4096 bytes x blocks.
+constexpr int kFusedBlocks = 2048;
 template <int T, int MT, int X>
 __global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product P) {
     constexpr int U = 4;
@@ -604,15 +620,19 @@ template <int TM, int TN, int STAGES> struct Tile {
 __device__ __forceinline__ int slot_of(int r, int b) { return b ^ (r >> 2 & 3); }
 
 template <int T, int TM, int TN, int STAGES>
-__global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P) {
+__global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product A, const Product B, unsigned first_tiles) {
     typedef Tile<TM, TN, STAGES> G;
     static_assert(G::kStages * G::kStage >= 4 * 32 * (32 * TN + 4) * 4, "the waves' output strips take the stages' place");
     __shared__ __align__(16) unsigned char lds[G::kStages * G::kStage];
+    // the first workgroups are product A's; in each, one XCD's workgroups walk neighbouring tiles, 8 tile rows at a time: operands meet in
+    // its L2
+    const bool of_a = blockIdx.x < first_tiles;
+    const Product &P = of_a ? A : B;
+    const int all = of_a ? dipr_xcd_contiguous(blockIdx.x, first_tiles) : dipr_xcd_contiguous(blockIdx.x - first_tiles, gridDim.x - first_tiles);
     const long long M = P.M, N = P.N;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_m = static_cast<int>((P.last - P.first + G::BM - 1) / G::BM), tiles_n = static_cast<int>((N + G::BN - 1) / G::BN);
-    // one XCD's workgroups walk neighbouring tiles, 8 tile rows at a time: operands meet in its L2
-    const int all = dipr_xcd_contiguous(blockIdx.x, gridDim.x), split = all / (tiles_m * tiles_n), id = all % (tiles_m * tiles_n);
+    const int split = all / (tiles_m * tiles_n), id = all % (tiles_m * tiles_n);
     const int group = 8 * tiles_n, first = id / group * 8, high = min(8, tiles_m - first);
     const long long m0 = P.first + static_cast<long long>(first + id % group % high) * G::BM;
     const long long n0 = static_cast<long long>(id % group / high) * G::BN;
@@ -629,18 +649,18 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product P)
 #pragma unroll
     for (int j = 0; j < G::kCodeLoads; ++j) {
         const int piece = wave * G::kCodeLoads + j, r = lane >> 2;
-        const bool of_a = piece < G::BM / 16;
-        const long long row = of_a ? min(m0 + piece * 16 + r, M - 1) : min(n0 + (piece - G::BM / 16) * 16 + r, N - 1);
-        src[j] = (of_a ? a : b) + row * 64 + slot_of(r, lane & 3) * 16;
-        move[j] = (of_a ? M : N) * 64;
+        const bool is_a = piece < G::BM / 16;
+        const long long row = is_a ? min(m0 + piece * 16 + r, M - 1) : min(n0 + (piece - G::BM / 16) * 16 + r, N - 1);
+        src[j] = (is_a ? a : b) + row * 64 + slot_of(r, lane & 3) * 16;
+        move[j] = (is_a ? M : N) * 64;
     }
 #pragma unroll
     for (int j = 0; j < G::kWordLoads; ++j) {
         const int piece = min(wave * G::kWordLoads + j, (G::BM + G::BN) / 64 - 1);      // (a spare one fetches the last again)
-        const bool of_a = piece < G::BM / 64;
-        const long long groups = of_a ? row_groups(M) : row_groups(N);
-        const long long g = of_a ? min(m0 / 64 + piece, groups - 1) : min(n0 / 64 + piece - G::BM / 64, groups - 1);
-        ssrc[j] = (of_a ? sa : sb) + g * 64 + lane;
+        const bool is_a = piece < G::BM / 64;
+        const long long groups = is_a ? row_groups(M) : row_groups(N);
+        const long long g = is_a ? min(m0 / 64 + piece, groups - 1) : min(n0 / 64 + piece - G::BM / 64, groups - 1);
+        ssrc[j] = (is_a ? sa : sb) + g * 64 + lane;
         smove[j] = groups * 64;
     }
     const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds));
@@ -743,23 +763,22 @@ inline bool aligned(const void *p, unsigned n) { return (reinterpret_cast<uintpt
 inline int elem_bytes(int d) { return d == F32 ? 4 : 2; }
 constexpr long long kMaxSide = 1ll << 40, kMaxGrid = 1ll << 30;
 
-template <int T>
-void launch_quantise(DiprProf &prof, const void *x, long long R, long long C, long long stride, int vec, void *rc, void *rs, void *cc, void *cs,
-                     float *sums, hipStream_t st) {
-    // blocks down the columns need the padding rows' zeros too
-    const long long tiles_r = cc ? round_up(R, 128) / kQR : (R + kQR - 1) / kQR, tiles_c = (C + kQC - 1) / kQC;
-    const dim3 grid(static_cast<unsigned>(tiles_r * tiles_c)), block(kThreads);
-#define MX4_QUANTISE(ROW, COL, SUM)                                                                                                  \
-    DIPR_LAUNCH(prof, (k_mx4_quantise<T, ROW, COL, SUM>), grid, block, st, x, R, C, stride, vec, static_cast<unsigned char *>(rc),   \
-                static_cast<unsigned *>(rs), static_cast<unsigned char *>(cc), static_cast<unsigned *>(cs), sums)
-    if (rc && cc && sums) MX4_QUANTISE(true, true, true);
-    else if (rc && cc) MX4_QUANTISE(true, true, false);
-    else if (cc && sums) MX4_QUANTISE(false, true, true);
-    else if (cc) MX4_QUANTISE(false, true, false);
+// blocks down the columns need the padding rows' zeros too
+inline long long quantise_tiles(const Matrix &m) {
+    return (m.col_codes ? round_up(m.R, 128) / kQR : (m.R + kQR - 1) / kQR) * ((m.C + kQC - 1) / kQC);
+}
+template <int T> void launch_quantise(DiprProf &prof, const Matrix &m, const Matrix *other, hipStream_t st) {
+    const unsigned first = static_cast<unsigned>(quantise_tiles(m));
+    const dim3 grid(first + (other ? static_cast<unsigned>(quantise_tiles(*other)) : 0u)), block(kThreads);
+    const Matrix &n = other ? *other : m;
+#define MX4_QUANTISE(ROW, COL, SUM) DIPR_LAUNCH(prof, (k_mx4_quantise<T, ROW, COL, SUM>), grid, block, st, m, n, first)
+    if (m.row_codes && m.col_codes && m.sums) MX4_QUANTISE(true, true, true);
+    else if (m.row_codes && m.col_codes) MX4_QUANTISE(true, true, false);
+    else if (m.col_codes && m.sums) MX4_QUANTISE(false, true, true);
+    else if (m.col_codes) MX4_QUANTISE(false, true, false);
     else MX4_QUANTISE(true, false, false);
 #undef MX4_QUANTISE
 }
-
 
 // ---- which kernels a product takes
 // Estimated from measured times (ns): a step of 128 columns costs a 256 x 256 tile 780, a 128 x 128 tile 270 where it has the CU for itself
@@ -810,56 +829,83 @@ Plan plan(long long M, long long N, long long kt) {
     return p;
 }
 
-template <int T> void launch_product(DiprProf &prof, const Plan &plan, Product P, float *part, hipStream_t st) {
+template <int T> void launch_rows(DiprProf &prof, const Product &P, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>((P.N + 15) / 16)), block(512);
+    const long long rows = P.last - P.first;
+    if (rows <= 16) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 1, -1>), grid, block, st, P);
+    else if (rows <= 32) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 2, -1>), grid, block, st, P);
+    else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, -1>), grid, block, st, P);
+}
+
+template <int T> void launch_product(DiprProf &prof, Product P, const Product *other, float *part, hipStream_t st) {
     const dim3 block(kThreads);
-    if (plan.form == Plan::kRows || plan.tail) {
+    const Plan p = plan(P.M, P.N, P.kt);
+    if (p.form == Plan::kRows) return launch_rows<T>(prof, P, st);
+    Product O = other ? *other : P;
+    const long long tails[2] = {p.tail, other ? plan(O.M, O.N, O.kt).tail : 0};
+    Product *both[2] = {&P, &O};
+    for (int i = 0; i < 2; ++i)
+        if (tails[i]) {
+            Product Q = *both[i];
+            Q.first = Q.M - tails[i];
+            launch_rows<T>(prof, Q, st);
+            both[i]->last -= tails[i];
+        }
+    const int side = p.form == Plan::kLarge ? 256 : 128;
+    const unsigned first = static_cast<unsigned>(tiles_of(P.last, P.N, side)) * p.splits;
+    const dim3 grid(first + (other ? static_cast<unsigned>(tiles_of(O.last, O.N, side)) : 0u));
+    if (p.form == Plan::kLarge) {
+        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 4, 4, 3>), grid, block, st, P, O, first);
+    } else if (p.splits == 1) {
+        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 2, 2, 3>), grid, block, st, P, O, first);
+    } else {
         Product Q = P;
-        Q.first = plan.tail ? P.M - plan.tail : 0;
-        const dim3 grid(static_cast<unsigned>((P.N + 15) / 16));
-        const long long rows = Q.last - Q.first;
-        if (rows <= 16) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 1, -1>), grid, dim3(512), st, Q);
-        else if (rows <= 32) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 2, -1>), grid, dim3(512), st, Q);
-        else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, -1>), grid, dim3(512), st, Q);
-        if (plan.form == Plan::kRows) return;
-        P.last -= plan.tail;
+        Q.splits = p.splits;
+        Q.out = part;
+        Q.bias = nullptr;
+        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<F32, 2, 2, 3>), grid, block, st, Q, Q, first);
+        const long long want = (P.M * ((P.N + 3) / 4) + kThreads - 1) / kThreads;
+        hipLaunchKernelGGL((k_mx4_gemm_sum<T>), dim3(static_cast<unsigned>(want < 8192 ? want : 8192)), block, 0, st, part, p.splits, P.bias,
+                           P.bias_type, P.M, P.N, P.out);
     }
-    if (plan.form == Plan::kLarge) {
-        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 4, 4, 3>), dim3(static_cast<unsigned>(tiles_of(P.last, P.N, 256))), block, st, P);
-        return;
-    }
-    const unsigned tiles = static_cast<unsigned>(tiles_of(P.last, P.N, 128));
-    if (plan.splits == 1) {
-        DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 2, 2, 3>), dim3(tiles), block, st, P);
-        return;
-    }
-    Product Q = P;
-    Q.splits = plan.splits;
-    Q.out = part;
-    Q.bias = nullptr;
-    DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<F32, 2, 2, 3>), dim3(tiles * plan.splits), block, st, Q);
-    const long long want = (P.M * ((P.N + 3) / 4) + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL((k_mx4_gemm_sum<T>), dim3(static_cast<unsigned>(want < 8192 ? want : 8192)), block, 0, st, part, plan.splits, P.bias, P.bias_type,
-                       P.M, P.N, P.out);
 }
 
 // ---- the pieces that the C entries share; arguments are checked by then
-void quantise(const void *x, int dtype, long long R, long long C, long long stride, void *rc, void *rs, void *cc, void *cs, float *col_sums,
-              void *workspace, hipStream_t st) {
-    const int vec = aligned(x, 16) && (R == 1 || stride * elem_bytes(dtype) % 16 == 0);
-    float *sums = col_sums ? static_cast<float *>(workspace) : nullptr;
+Matrix matrix_of(const void *x, int dtype, long long R, long long C, long long stride, void *rc, void *rs, void *cc, void *cs, float *sums) {
+    Matrix m;
+    m.x = x;
+    m.R = R;
+    m.C = C;
+    m.stride = stride;
+    m.vec = aligned(x, 16) && (R == 1 || stride * elem_bytes(dtype) % 16 == 0);
+    m.row_codes = static_cast<unsigned char *>(rc);
+    m.row_scales = static_cast<unsigned *>(rs);
+    m.col_codes = static_cast<unsigned char *>(cc);
+    m.col_scales = static_cast<unsigned *>(cs);
+    m.sums = sums;
+    return m;
+}
+// `other`: a second matrix of the same type and directions, in the same launch
+void quantise(int dtype, const Matrix &m, const Matrix *other, hipStream_t st) {
     DiprProf prof(DEEPIPR_K_MX4_QUANTIZE);
-    prof.bytes = static_cast<double>(R) * static_cast<double>(C) * (elem_bytes(dtype) + 0.53125 * ((rc ? 1 : 0) + (cc ? 1 : 0)));
+    const auto bytes = [&](const Matrix &q) {
+        return static_cast<double>(q.R) * static_cast<double>(q.C) * (elem_bytes(dtype) + 0.53125 * ((q.row_codes ? 1 : 0) + (q.col_codes ? 1 : 0)));
+    };
+    prof.bytes = bytes(m) + (other ? bytes(*other) : 0.0);
     switch (dtype) {
-        case F32: launch_quantise<F32>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
-        case BF16: launch_quantise<BF16>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
-        default: launch_quantise<F16>(prof, x, R, C, stride, vec, rc, rs, cc, cs, sums, st); break;
+        case F32: launch_quantise<F32>(prof, m, other, st); break;
+        case BF16: launch_quantise<BF16>(prof, m, other, st); break;
+        default: launch_quantise<F16>(prof, m, other, st); break;
     }
-    for (long long tiles = round_up(R, 128) / kQR; col_sums;) {          // at most 128 tiles in one go: long batches take a second or third pass
+}
+void column_sums(const Matrix &m, float *out, hipStream_t st) {
+    float *sums = m.sums;
+    for (long long tiles = round_up(m.R, 128) / kQR;;) {                 // at most 128 tiles in one go: long batches take a second or third pass
         const long long groups = (tiles + kSumTiles - 1) / kSumTiles;
-        float *to = groups == 1 ? col_sums : sums + tiles * C;
-        hipLaunchKernelGGL(k_mx4_colsum, dim3(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(groups)), dim3(kThreads), 0, st, sums, tiles, C,
-                           to);
-        if (groups == 1) break;
+        float *to = groups == 1 ? out : sums + tiles * m.C;
+        hipLaunchKernelGGL(k_mx4_colsum, dim3(static_cast<unsigned>((m.C + 31) / 32), static_cast<unsigned>(groups)), dim3(kThreads), 0, st, sums,
+                           tiles, m.C, to);
+        if (groups == 1) return;
         sums = to;
         tiles = groups;
     }
@@ -883,9 +929,8 @@ inline size_t product_bytes(long long M, long long N, long long K) {
     const Plan p = plan(M, N, round_up(K, 128) / 128);
     return p.splits > 1 ? static_cast<size_t>(p.splits) * static_cast<size_t>(M) * static_cast<size_t>(N) * sizeof(float) : 0;
 }
-void product(const void *a, const void *sa, const void *b, const void *sb, const void *bias, int bias_dtype, long long M, long long N, long long K,
-             void *out, int dtype, void *workspace, hipStream_t st) {
-    const long long steps = round_up(K, 128) / 128;
+Product product_of(const void *a, const void *sa, const void *b, const void *sb, const void *bias, int bias_dtype, long long M, long long N,
+                   long long K, void *out) {
     Product P = {};
     P.a = static_cast<const unsigned char *>(a);
     P.b = static_cast<const unsigned char *>(b);
@@ -895,34 +940,33 @@ void product(const void *a, const void *sa, const void *b, const void *sb, const
     P.bias_type = bias_dtype;
     P.M = P.last = M;
     P.N = N;
-    P.first = 0;
-    P.kt = static_cast<int>(steps);
+    P.kt = static_cast<int>(round_up(K, 128) / 128);
     P.splits = 1;
     P.out = out;
-    const Plan p = plan(M, N, steps);
+    return P;
+}
+// Whether two products of one output type can share a launch
+bool alike(const Product &p, const Product &q) {
+    const Plan a = plan(p.M, p.N, p.kt), b = plan(q.M, q.N, q.kt);
+    return a.form == b.form && a.form != Plan::kRows && a.splits == 1 && b.splits == 1 &&
+           tiles_of(p.M, p.N, 128) + tiles_of(q.M, q.N, 128) <= kMaxGrid;
+}
+// `other`: a second product that is alike, in the same launch
+void run(const Product &P, const Product *other, int dtype, void *workspace, hipStream_t st) {
     DiprProf prof(DEEPIPR_K_MX4_MATMUL);
-    prof.bytes = 2.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+    prof.bytes = 256.0 * (static_cast<double>(P.M) * P.N * P.kt + (other ? static_cast<double>(other->M) * other->N * other->kt : 0.0));
     switch (dtype) {
-        case F32: launch_product<F32>(prof, p, P, static_cast<float *>(workspace), st); break;
-        case BF16: launch_product<BF16>(prof, p, P, static_cast<float *>(workspace), st); break;
-        default: launch_product<F16>(prof, p, P, static_cast<float *>(workspace), st); break;
+        case F32: launch_product<F32>(prof, P, other, static_cast<float *>(workspace), st); break;
+        case BF16: launch_product<BF16>(prof, P, other, static_cast<float *>(workspace), st); break;
+        default: launch_product<F16>(prof, P, other, static_cast<float *>(workspace), st); break;
     }
 }
 
 // The same with a in its own type, for at most 16 rows (out of a's type): one launch
 void product_of_rows(const void *x, int dtype, long long x_stride, const void *b, const void *sb, const void *bias, int bias_dtype, long long M,
                      long long N, long long K, void *out, hipStream_t st) {
-    Product P = {};
-    P.b = static_cast<const unsigned char *>(b);
-    P.sb = static_cast<const unsigned *>(sb);
-    P.bias = bias;
-    P.bias_type = bias_dtype;
-    P.M = P.last = M;
-    P.N = N;
+    Product P = product_of(nullptr, nullptr, b, sb, bias, bias_dtype, M, N, K, out);
     P.K = K;
-    P.kt = static_cast<int>(round_up(K, 128) / 128);
-    P.splits = 1;
-    P.out = out;
     P.x = x;
     P.x_stride = x_stride;
     P.x_vec = aligned(x, 16) && (M == 1 || x_stride * elem_bytes(dtype) % 16 == 0);
@@ -1024,7 +1068,10 @@ int deepipr_mx4_quantize(const void *x, int dtype, long long rows, long long col
     if (!aligned(x, elem_bytes(dtype)) || !aligned(row_codes, 16) || !aligned(row_scales, 16) || !aligned(col_codes, 16) || !aligned(col_scales, 16))
         return dipr_fail(DEEPIPR_EINVAL, "%s: misaligned pointer", what);
     if (!quantise_fits(rows, cols)) return dipr_fail(DEEPIPR_EINVAL, "%s: matrix too large", what);
-    quantise(x, dtype, rows, cols, row_stride, row_codes, row_scales, col_codes, col_scales, col_sums, workspace, static_cast<hipStream_t>(stream));
+    const Matrix m = matrix_of(x, dtype, rows, cols, row_stride, row_codes, row_scales, col_codes, col_scales,
+                               col_sums ? static_cast<float *>(workspace) : nullptr);
+    quantise(dtype, m, nullptr, static_cast<hipStream_t>(stream));
+    if (col_sums) column_sums(m, col_sums, static_cast<hipStream_t>(stream));
     return dipr_check_launch(what);
 }
 
@@ -1074,7 +1121,8 @@ int deepipr_mx4_matmul(const void *a_codes, const void *a_scales, const void *b_
     const size_t need = product_bytes(M, N, K);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return dipr_fail(DEEPIPR_EINVAL, "%s: workspace too small or misaligned", what);
-    product(a_codes, a_scales, b_codes, b_scales, bias, bias_dtype, M, N, K, out, dtype, workspace, static_cast<hipStream_t>(stream));
+    run(product_of(a_codes, a_scales, b_codes, b_scales, bias, bias_dtype, M, N, K, out), nullptr, dtype, workspace,
+        static_cast<hipStream_t>(stream));
     return dipr_check_launch(what);
 }
 
@@ -1101,13 +1149,21 @@ int deepipr_mx4_linear_fwd(const void *x, int x_dtype, long long x_stride, const
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < f.bytes || (s.bytes && (!saved || !aligned(saved, 16) || saved_bytes < s.bytes)))
         return dipr_fail(DEEPIPR_EINVAL, "%s: scratch or saved memory too small or misaligned", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (kept && M <= 16 && M * (round_up(K, 128) / 32) <= kFusedBlocks) {
+    if (kept && M <= 16 && M * (round_up(K, 128) / 32) * elem_bytes(x_dtype) <= 2 * kFusedBlocks) {
         product_of_rows(x, x_dtype, x_stride, w_codes, w_scales, bias, bias_dtype, M, N, K, out, st);
         return dipr_check_launch(what);
     }
-    quantise(x, x_dtype, M, K, x_stride, f.x.codes, f.x.scales, s.x_t.codes, s.x_t.scales, nullptr, nullptr, st);
-    if (!kept) quantise(w, w_dtype, N, K, w_stride, f.w.codes, f.w.scales, s.w_t.codes, s.w_t.scales, nullptr, nullptr, st);
-    product(f.x.codes, f.x.scales, kept ? w_codes : f.w.codes, kept ? w_scales : f.w.scales, bias, bias_dtype, M, N, K, out, x_dtype, f.work, st);
+    const Matrix mx = matrix_of(x, x_dtype, M, K, x_stride, f.x.codes, f.x.scales, s.x_t.codes, s.x_t.scales, nullptr);
+    if (kept) {
+        quantise(x_dtype, mx, nullptr, st);
+    } else {
+        const Matrix mw = matrix_of(w, w_dtype, N, K, w_stride, f.w.codes, f.w.scales, s.w_t.codes, s.w_t.scales, nullptr);
+        const bool together = x_dtype == w_dtype && !mx.col_codes == !mw.col_codes && quantise_tiles(mx) + quantise_tiles(mw) <= kMaxGrid;
+        quantise(x_dtype, mx, together ? &mw : nullptr, st);
+        if (!together) quantise(w_dtype, mw, nullptr, st);
+    }
+    run(product_of(f.x.codes, f.x.scales, kept ? w_codes : f.w.codes, kept ? w_scales : f.w.scales, bias, bias_dtype, M, N, K, out), nullptr, x_dtype,
+        f.work, st);
     return dipr_check_launch(what);
 }
 
@@ -1125,10 +1181,18 @@ int deepipr_mx4_linear_bwd(const void *dy, int dy_dtype, long long dy_stride, lo
         return dipr_fail(DEEPIPR_EINVAL, "%s: scratch or saved memory too small or misaligned", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool down = dw || dbias;
-    quantise(dy, dy_dtype, M, N, dy_stride, dx ? b.y.codes : nullptr, dx ? b.y.scales : nullptr, down ? b.y_t.codes : nullptr,
-             down ? b.y_t.scales : nullptr, dbias, b.sums, st);
-    if (dx) product(b.y.codes, b.y.scales, s.w_t.codes, s.w_t.scales, nullptr, 0, M, K, N, dx, dx_dtype, b.work, st);
-    if (dw) product(b.y_t.codes, b.y_t.scales, s.x_t.codes, s.x_t.scales, nullptr, 0, N, K, M, dw, dw_dtype, b.work, st);
+    const Matrix my = matrix_of(dy, dy_dtype, M, N, dy_stride, dx ? b.y.codes : nullptr, dx ? b.y.scales : nullptr, down ? b.y_t.codes : nullptr,
+                                down ? b.y_t.scales : nullptr, dbias ? static_cast<float *>(b.sums) : nullptr);
+    quantise(dy_dtype, my, nullptr, st);
+    if (dbias) column_sums(my, dbias, st);
+    const Product px = product_of(b.y.codes, b.y.scales, s.w_t.codes, s.w_t.scales, nullptr, 0, M, K, N, dx);
+    const Product pw = product_of(b.y_t.codes, b.y_t.scales, s.x_t.codes, s.x_t.scales, nullptr, 0, N, K, M, dw);
+    if (dx && dw && dx_dtype == dw_dtype && alike(px, pw)) {
+        run(pw, &px, dw_dtype, b.work, st);
+    } else {
+        if (dx) run(px, nullptr, dx_dtype, b.work, st);
+        if (dw) run(pw, nullptr, dw_dtype, b.work, st);
+    }
     return dipr_check_launch(what);
 }
 

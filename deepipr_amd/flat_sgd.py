@@ -445,8 +445,8 @@ class FlatSGD(torch.optim.Optimizer):
         if any(g is None for g in grads):
             offsets = [off for off, g in zip(offsets, grads) if g is not None]
             grads = [g for g in grads if g is not None]
-        if {g.dtype for g in grads} - {torch.float32} or {g.device for g in grads} - {self.flat_param.device} or \
-                not all(map(torch.Tensor.is_contiguous, grads)):
+        if {g.dtype for g in grads} - {torch.float32} or not all(map(torch.Tensor.is_contiguous, grads)) or \
+                set(map(torch.Tensor.get_device, grads)) - {self.flat_param.get_device()}:
             return False
         if grads:
             P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, grads, offsets, self._hyper, self.grad_norm)

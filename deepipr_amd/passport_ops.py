@@ -955,25 +955,26 @@ class HipKernels:
         return True
 
     def _tensor_list(self, what, tensors, rows=None):
-        """-> (device, host rows {address, elements, offset, type} as include/deepipr_hip.h: DeepiprTensor has them).  rows: the rows with
-        everything but the addresses filled in (float32 tensors of known sizes)."""
+        """-> (device, host rows {address, elements, offset, type} as include/deepipr_hip.h: DeepiprTensor has them).  rows: the rows of
+        float32 tensors with everything but the addresses filled in."""
         if not tensors:
             raise RuntimeError('%s: an empty list of tensors' % what)
         devs = set(map(torch.Tensor.get_device, tensors))
         if len(devs) != 1 or -1 in devs:
             raise RuntimeError('deepipr_amd %s runs on the GPU only, all tensors on one device (got %s); there is no CPU fallback'
                                % (what, sorted({str(t.device) for t in tensors})))
-        try:
-            types = [self._DTYPE_CODE[t.dtype] for t in tensors]
-        except KeyError as e:
-            raise RuntimeError('deepipr_amd %s takes float32, bfloat16 and float16 tensors (got %s)' % (what, e)) from None
         if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(map(self._dense, tensors)):
             raise RuntimeError('deepipr_amd %s needs dense tensors (no gaps, no element twice)' % what)
         if rows is None:
             rows = np.empty((len(tensors), 4), dtype=np.int64)
+            try:
+                rows[:, 3] = [self._DTYPE_CODE[t.dtype] for t in tensors]
+            except KeyError as e:
+                raise RuntimeError('deepipr_amd %s takes float32, bfloat16 and float16 tensors (got %s)' % (what, e)) from None
             rows[:, 1] = list(map(torch.Tensor.numel, tensors))
             rows[:, 2] = 0
-        rows[:, 3] = types
+        elif {t.dtype for t in tensors} != {torch.float32}:
+            raise RuntimeError('deepipr_amd %s takes float32 tensors' % what)
         rows[:, 0] = list(map(torch.Tensor.data_ptr, tensors))
         return tensors[0].device, rows
 
@@ -1008,6 +1009,7 @@ class HipKernels:
         rows = np.empty((len(grads), 4), dtype=np.int64)
         rows[:, 1] = list(map(torch.Tensor.numel, grads))
         rows[:, 2] = offsets
+        rows[:, 3] = _lib.F32
         gdev, rows = self._tensor_list('sgd_momentum_step_clipped', grads, rows)
         if gdev != dev or hyper.numel() != 5 or flat_buf.numel() != flat_param.numel():
             raise RuntimeError('sgd_momentum_step_clipped: five hyper-parameters, buffers of one size, all on one device')
