@@ -131,7 +131,10 @@ struct Matrix {
 template <int T, bool ROW, bool COL, bool SUM>
 __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const Matrix A, const Matrix B, unsigned first) {
     const Matrix &m = blockIdx.x < first ? A : B;
-    const unsigned id = blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
+    int id = static_cast<int>(blockIdx.x < first ? blockIdx.x : blockIdx.x - first);
+    // Tiles that end inside a cache line of x share it with their neighbours: those meet in one XCD's L2 (200 704 x 1016 bf16 137 -> 105 us);
+    // whole lines are better off spread (8192 x 8192 bf16 25 us, 30 in that order).
+    if (m.C % kQC) id = dipr_xcd_contiguous(id, static_cast<int>(blockIdx.x < first ? first : gridDim.x - first));
     const void *__restrict__ x = m.x;
     const long long R = m.R, C = m.C, stride = m.stride;
     const int vec = m.vec;
@@ -170,6 +173,16 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const Matrix A, const
         }
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) put(j * kThreads + tid, q[j]);
+    } else if (vec && C % V == 0) {                                      // the last rows or columns, in whole pieces
+        u32x4 q[LOADS];
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int i = j * kThreads + tid;
+            const long long r = r0 + i / PER, c = c0 + i % PER * V;
+            q[j] = r < R && c < C ? load16<T>(x, r * stride + c) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) put(j * kThreads + tid, q[j]);
     } else if (T == F32) {
         // rows off the 16-byte grid (a wave's single elements are contiguous whatever the alignment: 200 704 x 1021 takes 179 us this way
         // and 293 by unaligned 16-byte loads), and the matrix's last rows and columns
@@ -183,22 +196,32 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const Matrix A, const
     } else {
         // the same for 16-bit elements, two to an aligned word (loads of single ones are four times slower); a row that starts in the middle
         // of a word is off by one: its first and last words hold one element of it, and what else they hold is not used
-        const int lane = tid & 63, first = (tid >> 6) * 16;
+        const int lane = tid & 63, row0 = (tid >> 6) * 16;
         const auto row_at = [&](int r) { return reinterpret_cast<uintptr_t>(x) + static_cast<uintptr_t>(((r0 + r) * stride + c0) * 2); };
-        unsigned w[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const uintptr_t at = row_at(first + j);
-            const int odd = static_cast<int>(at >> 1 & 1);
-            w[j] = r0 + first + j < R && c0 + 2 * lane - odd < C ? *reinterpret_cast<const unsigned *>(at - 2 * odd + 4 * lane) : 0u;
-        }
         const auto value = [&](unsigned h) { return T == BF16 ? bf16_to_f32(h) : f16_to_f32(h); };
+        unsigned w[16];
+        if (r0 + kQR <= R && c0 + kQC <= C) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = *reinterpret_cast<const unsigned *>((row_at(row0 + j) & ~uintptr_t(3)) + 4 * lane);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const uintptr_t at = row_at(row0 + j);
+                const int odd = static_cast<int>(at >> 1 & 1);
+                w[j] = r0 + row0 + j < R && c0 + 2 * lane - odd < C ? *reinterpret_cast<const unsigned *>(at - 2 * odd + 4 * lane) : 0u;
+                if (c0 + 2 * lane - odd + 1 >= C) w[j] &= 0xffffu;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const int e = 2 * lane - static_cast<int>(row_at(first + j) >> 1 & 1);
-            float *d = s + (first + j) * kQP + e;
-            if (e >= 0) d[0] = value(w[j] & 0xffffu);
-            d[1] = c0 + e + 1 < C ? value(w[j] >> 16) : 0.0f;
+            const int odd = static_cast<int>(row_at(row0 + j) >> 1 & 1);
+            float *d = s + (row0 + j) * kQP + 2 * lane - odd;
+            if (odd == 0) {
+                *reinterpret_cast<f32x2 *>(d) = f32x2{value(w[j] & 0xffffu), value(w[j] >> 16)};
+            } else {
+                if (lane) d[0] = value(w[j] & 0xffffu);
+                d[1] = value(w[j] >> 16);
+            }
         }
         if (tid < kQR && (row_at(tid) >> 1 & 1))                         // the 128th column of a row that is off by one
             s[tid * kQP + 127] = r0 + tid < R && c0 + 127 < C ? load1<T>(x, (r0 + tid) * stride + c0 + 127) : 0.0f;
