@@ -784,7 +784,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_mx4_gemm_tiled(const Product A,
 inline bool good_dtype(int d) { return d == F32 || d == BF16 || d == F16; }
 inline bool aligned(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 inline int elem_bytes(int d) { return d == F32 ? 4 : 2; }
-constexpr long long kMaxSide = 1ll << 40, kMaxGrid = 1ll << 30;
+constexpr long long kMaxSide = 1ll << 28, kMaxGrid = 1ll << 23;       // a launch counts its threads in 32 bits
 
 // blocks down the columns need the padding rows' zeros too
 inline long long quantise_tiles(const Matrix &m) {
@@ -841,6 +841,7 @@ Plan plan(long long M, long long N, long long kt) {
         if (t < best) best = t, p.tail = tail;
     }
     for (int splits = 1; splits <= 16 && splits <= kt; splits += splits < 4 ? 1 : splits / 2) {
+        if (splits > 1 && tiles_of(M, N, 128) * splits > 4 * cu_count()) break;
         const double t = small_ns(M, N, kt, splits);
         if (t < best) {
             best = t;
@@ -945,7 +946,7 @@ inline bool quantise_fits(long long R, long long C) {
     return R <= 65535ll * kSumTiles * kQR && C <= kMaxSide && round_up(R, 128) / kQR * ((C + kQC - 1) / kQC) <= kMaxGrid;
 }
 inline bool product_fits(long long M, long long N, long long K) {
-    return M <= kMaxSide && N <= kMaxSide && K <= kMaxSide && tiles_of(M, N, 128) <= kMaxGrid / 16 && (N + 15) / 16 <= kMaxGrid &&
+    return M <= kMaxSide && N <= kMaxSide && K <= kMaxSide && tiles_of(M, N, 128) <= kMaxGrid && (N + 15) / 16 <= kMaxGrid &&
            round_up(K, 128) / 128 <= kMaxGrid;
 }
 inline size_t product_bytes(long long M, long long N, long long K) {

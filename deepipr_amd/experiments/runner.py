@@ -142,6 +142,8 @@ def rounded_report(model, trainer, valid_loader, device, passport):
 
 
 def run(args, private, train_loader=None, valid_loader=None, wm_loader=None):
+    if args.get('round_weights') and not args.get('eval'):
+        raise ValueError('--round-weights reports on a trained net: it needs --eval')
     rank, local_rank, world = D.init_from_env(args.get('backend'))
     dev_name = args.get('device') or ('cuda' if torch.cuda.is_available() else None)
     if dev_name is None:

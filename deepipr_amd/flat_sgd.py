@@ -32,7 +32,7 @@ class FlatSGD(torch.optim.Optimizer):
     def __init__(self, params, lr=0.01, momentum=0.9, weight_decay=1e-4, bucket_fractions=(0.45, 0.8, 0.95),
                  process_group=None, max_grad_norm=None):
         """max_grad_norm: the step uses the gradients scaled by min(1, max_grad_norm / (norm + 1e-6)), the norm that of the averaged
-        gradients of ALL parameters (torch.nn.utils.clip_grad_norm_'s rule); the gradients themselves stay as they are and
+        gradients of ALL parameters; the gradients themselves stay as they are and
         `grad_norm` (0-d, on the device) holds the norm of the last step.  None: no norm is computed.  The value can be changed
         between steps (`opt.max_grad_norm = 0.5`), captured ones included; switching it on or off after a capture cannot follow."""
         if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:

@@ -1,9 +1,9 @@
 """Global gradient norm and clipping over many tensors (csrc/deepipr_gradnorm.hip, include/deepipr_hip.h: deepipr_grad_*).
 
 The reference steps without clipping (experiments/trainer.py:144-145); this is what stands in front of `optimizer.step()` when a run
-clips.  n = (sum |g|^p)^(1/p) over every element of every tensor, f = min(1, max_norm / (n + 1e-6)), g *= f: the rule of
-torch.nn.utils.clip_grad_norm_, in two launches whatever the number of tensors (up to 240 each), without a host synchronisation, with
-the sum held in 64 bits and added in a fixed order.  Calls only enqueue work on the current stream and can be captured into a hipGraph;
+clips.  n = (sum |g|^p)^(1/p) over every element of every tensor, f = min(1, max_norm / (n + 1e-6)), g *= f, in two launches (for up
+to 240 tensors; two more for every further 240), without a host synchronisation, with the sum held in 64 bits and added in a fixed
+order.  Calls only enqueue work on the current stream and can be captured into a hipGraph;
 a captured call keeps the tensors' addresses.
 
 FlatSGD(max_grad_norm=...) does the same inside its step: with several ranks the norm has to be that of the EXCHANGED gradients, which
@@ -57,12 +57,12 @@ def clip_grads_(tensors, max_norm, norm_type=2.0):
     if not tensors:
         return torch.zeros(())
     norm = P.kernels.grad_clip(tensors, max_norm, code)
-    torch.autograd.graph.increment_version(tensors)
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
     return norm
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
-    """torch.nn.utils.clip_grad_norm_ for parameters on one GPU: the gradients that are there, clipped in place; -> their norm.
+    """The gradients that the parameters have, clipped in place; -> their norm before.
     error_if_nonfinite=True reads the norm on the host first and raises, leaving the gradients as they were."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]

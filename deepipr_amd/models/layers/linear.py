@@ -22,15 +22,11 @@ class Mx4Linear(nn.Linear):
         self._kept_version = None
 
     @classmethod
-    def of(cls, linear):
-        """The layer that shares `linear`'s parameters."""
-        new = cls.__new__(cls)
-        nn.Module.__init__(new)
-        new.in_features, new.out_features = linear.in_features, linear.out_features
-        new.weight, new.bias = linear.weight, linear.bias
-        new._without_codes()
-        new.training = linear.training
-        return new
+    def adopt_(cls, linear):
+        """`linear` itself, from now on an Mx4Linear: parameters, hooks and every reference to it stay."""
+        linear.__class__ = cls
+        linear._without_codes()
+        return linear
 
     def keep(self):
         q = mx4.quantize(self.weight.detach())
@@ -62,15 +58,12 @@ class Mx4Linear(nn.Linear):
 
 
 def use_mx4_linear_(model):
-    """Every plain nn.Linear below `model` becomes an Mx4Linear on the same parameters (optimisers built before or after see the same
-    tensors); -> how many."""
-    count = 0
-    for parent in list(model.modules()):
-        for name, child in list(parent.named_children()):
-            if type(child) is nn.Linear:
-                setattr(parent, name, Mx4Linear.of(child))
-                count += 1
-    return count
+    """Every plain nn.Linear of `model` becomes an Mx4Linear in place (optimisers built before or after see the same parameters);
+    -> how many."""
+    found = [m for m in model.modules() if type(m) is nn.Linear]
+    for m in found:
+        Mx4Linear.adopt_(m)
+    return len(found)
 
 
 @torch.no_grad()

@@ -76,7 +76,7 @@ def _by_rows(x):
 
 
 def quantize(x, dim=-1):
-    """x [R, C] (float32 / bfloat16 / float16, either direction contiguous) -> Mx4Matrix with blocks along `dim`."""
+    """x [R, C] (float32 / bfloat16 / float16, either direction contiguous) -> Mx4Matrix with blocks along `dim`.  Not differentiable."""
     x = _matrix(x)
     if dim not in (-2, -1, 0, 1):
         raise ValueError('mx4: dim 0 or 1 (got %r)' % (dim,))

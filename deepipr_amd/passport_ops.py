@@ -1041,6 +1041,14 @@ class HipKernels:
             raise RuntimeError('deepipr_amd %s takes float32, bfloat16 and float16 (got %s)' % (what, dtype))
         return code
 
+    @staticmethod
+    def _mx4_held(what, codes, scales, rows, cols):
+        """The buffers of a [rows, cols] matrix have the sizes that the kernels read."""
+        panels = -(-cols // 128)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.numel() != panels * rows * 64 or \
+                scales.numel() != panels * -(-rows // 64) * 256 or not codes.is_contiguous() or not scales.is_contiguous():
+            raise RuntimeError('deepipr_amd %s: the buffers are not those of a %d x %d matrix in 4 bits' % (what, rows, cols))
+
     def _mx4_buffers(self, rows, cols, dev):
         lib = _lib.lib()
         return (torch.empty(lib.deepipr_mx4_code_bytes(rows, cols), dtype=torch.uint8, device=dev),
@@ -1069,6 +1077,7 @@ class HipKernels:
 
     def mx4_dequantize(self, codes, scales, rows, cols, transposed, dtype):
         dev = self._mx4_chk('mx4_dequantize', codes, scales)
+        self._mx4_held('mx4_dequantize', codes, scales, rows, cols)
         code = self._mx4_type('mx4_dequantize', dtype)
         with _on(dev):
             out = torch.empty((cols, rows) if transposed else (rows, cols), dtype=dtype, device=dev)
@@ -1079,6 +1088,8 @@ class HipKernels:
     def mx4_matmul(self, a, b, m, n, k, bias, dtype):
         """a, b: (codes, scales) of [m, k] and [n, k] -> a b^T + bias, [m, n] of `dtype`."""
         dev = self._mx4_chk('mx4_matmul', a[0], a[1], b[0], b[1], bias)
+        self._mx4_held('mx4_matmul', a[0], a[1], m, k)
+        self._mx4_held('mx4_matmul', b[0], b[1], n, k)
         code = self._mx4_type('mx4_matmul', dtype)
         bcode = 0 if bias is None else self._mx4_type('mx4_matmul', bias.dtype)
         lib = _lib.lib()
@@ -1096,6 +1107,9 @@ class HipKernels:
         dev = self._mx4_chk(what, x, w if kept is None else kept[0], bias)
         m, k = x.shape
         n = w.shape[0] if kept is None else kept[2]
+        if kept is not None:
+            self._mx4_chk(what, x, kept[1])
+            self._mx4_held(what, kept[0], kept[1], n, k)
         xcode = self._mx4_type(what, x.dtype)
         lib = _lib.lib()
         with _on(dev):

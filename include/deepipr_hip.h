@@ -407,8 +407,7 @@ int deepipr_sgd_momentum_step_multi(float *param, float *momentum_buf, const lon
  * to 64 bits before they are squared or added, partial sums are added in a fixed order: bit-reproducible, no overflow or underflow
  * inside the sum.  A NaN anywhere gives NaN, an infinity without NaN gives infinity; an empty list gives 0.
  *   deepipr_grad_norm   *norm = n.
- *   deepipr_grad_clip   g *= f in place, f = min(1, max_norm / (n + 1e-6)) (torch.nn.utils.clip_grad_norm_'s rule); *norm = n, the norm
- *                       BEFORE clipping.  f == 1 writes nothing (1 * g is g in every type).  A NaN norm makes every gradient NaN, an
+ *   deepipr_grad_clip   g *= f in place, f = min(1, max_norm / (n + 1e-6)); *norm = n, the norm BEFORE clipping.  f == 1 writes nothing (1 * g is g in every type).  A NaN norm makes every gradient NaN, an
  *                       infinite one makes the finite gradients 0.  Products are rounded once to the tensor's type.  Tensors that
  *                       share memory are refused.
  *   deepipr_sgd_momentum_step_clipped   the step of deepipr_sgd_momentum_step_dev behind that rule, on gradients that lie where
@@ -419,7 +418,7 @@ int deepipr_sgd_momentum_step_multi(float *param, float *momentum_buf, const lon
  * The list is HOST memory, read before the call returns (captured launches keep it); `data` is device memory of `count` elements, any
  * alignment that fits the element type; entries with count 0 are skipped.  workspace: deepipr_grad_norm_workspace_bytes() bytes, used
  * between the launches of one call: calls that may run at the same time need one each.
- * replaces: torch.nn.utils.clip_grad_norm_ in front of optimizer.step() (experiments/trainer.py:144-145 has no clipping). */
+ * The reference steps without clipping (experiments/trainer.py:144-145). */
 #define DEEPIPR_F32 0
 #define DEEPIPR_BF16 1
 #define DEEPIPR_F16 2

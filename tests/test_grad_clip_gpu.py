@@ -115,6 +115,10 @@ def test_refusals_and_orders_of_dimensions():
     version = x._version
     assert abs(float(grad_clip.clip_grads_([x.t()], 0.5)) - want) <= want * 2 ** -23
     assert x._version == version + 1                       # autograd sees the write
+    with torch.inference_mode():
+        y = torch.ones(7, device=DEV)
+        grad_clip.clip_grads_([y], 1.0)
+        assert abs(float(y.norm()) - 1.0) < 1e-5
     c = torch.randn(2, 5, 3, 4, device=DEV).to(memory_format=torch.channels_last)
     k = c.clone()
     grad_clip.clip_grads_([c], 0.5)

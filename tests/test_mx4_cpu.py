@@ -21,7 +21,7 @@ def test_c_entries_refuse_before_any_launch():
         return lib.deepipr_mx4_quantize(x, dtype, rows, cols, stride, rc, rs, cc, cs, sums, ws, n, None)
     for bad in (dict(x=None), dict(dtype=3), dict(rows=0), dict(cols=0), dict(rows=-1), dict(stride=39), dict(rc=None), dict(cs=None),
                 dict(rc=None, rs=None, cc=None, cs=None), dict(x=p + 2), dict(rc=p + 8), dict(sums=p), dict(sums=p, ws=p, n=1),
-                dict(sums=p, ws=p, n=1 << 20, cc=None, cs=None), dict(rows=1 << 41), dict(rows=1 << 36, cols=1 << 20, stride=1 << 20)):
+                dict(sums=p, ws=p, n=1 << 20, cc=None, cs=None), dict(rows=1 << 41), dict(rows=1 << 27, cols=1 << 20, stride=1 << 20)):
         assert quant(**bad) == -1 and b'mx4_quantize' in lib.deepipr_last_error(), bad
 
     def deq(codes=p, scales=p, rows=4, cols=40, out=p, dtype=0):
@@ -32,7 +32,7 @@ def test_c_entries_refuse_before_any_launch():
     def mm(a=p, sa=p, b=p, sb=p, bias=None, bt=0, m=4, n=5, k=6, out=p, dtype=0, ws=None, nbytes=0):
         return lib.deepipr_mx4_matmul(a, sa, b, sb, bias, bt, m, n, k, out, dtype, ws, nbytes, None)
     for bad in (dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(out=None), dict(m=0), dict(n=0), dict(k=0), dict(dtype=-1),
-                dict(bias=p, bt=9), dict(a=p + 8), dict(bias=p + 1, bt=1), dict(out=p + 1, dtype=1), dict(m=1 << 41), dict(m=1 << 38, n=1 << 38)):
+                dict(bias=p, bt=9), dict(a=p + 8), dict(bias=p + 1, bt=1), dict(out=p + 1, dtype=1), dict(m=1 << 41), dict(m=1 << 27, n=1 << 27)):
         assert mm(**bad) == -1 and b'mx4_matmul' in lib.deepipr_last_error(), bad
 
 

@@ -313,6 +313,11 @@ def test_refusals_of_products():
         mx4.linear(x.double(), q)
     with pytest.raises(RuntimeError, match='GPU only'):
         mx4.linear(x.cpu(), q)
+    for codes, scales in ((q.codes[:-16], q.scales), (q.codes, q.scales[:-256]), (q.codes.int(), q.scales), (q.codes.cpu(), q.scales)):
+        bad = mx4.Mx4Matrix(codes, scales, 8, 64, 1)
+        for call in (bad.dequantize, lambda: mx4.matmul(mx4.quantize(x), bad), lambda: mx4.linear(x, bad)):
+            with pytest.raises(RuntimeError):
+                call()
     with pytest.raises(RuntimeError, match='twice|once_differentiable|marked'):
         a = x.clone().requires_grad_()
         g, = torch.autograd.grad(mx4.linear(a, w).square().sum(), a, create_graph=True)
@@ -379,6 +384,22 @@ def test_captured_training_passes_and_streams():
         torch.cuda.synchronize()
         for got, want in zip(outs, eager):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_launches_are_accounted():
+    """The in-situ profile sees the launches of the new entry points."""
+    from deepipr_amd import _lib, grad_clip, mx4
+    x, w = _random((300, 500), torch.float32, 25), _random((200, 500), torch.float32, 26)
+    _lib.profile_enable(True)
+    try:
+        mx4.linear(x, w)
+        mx4.quantize(x).dequantize()
+        grad_clip.clip_grads_([x], 0.5)
+        got = _lib.profile_read()
+    finally:
+        _lib.profile_enable(False)
+    for name, least in (('mx4_quantize', 2), ('mx4_dequantize', 1), ('mx4_matmul', 1), ('grad_norm', 1), ('grad_clip', 1)):
+        assert got[name][1] >= least and got[name][0] > 0, (name, got[name])
 
 
 def test_offsets_past_32_bits():

@@ -50,6 +50,12 @@ def test_layer_matches_its_formula_and_shares_parameters():
     assert torch.allclose(lin.weight.grad, _v(dy, 0).t() @ _v(x, 0), atol=1e-5)
     assert torch.allclose(lin.bias.grad, dy.sum(0), atol=1e-5)
     assert 'mx4' in repr(lin)
+    alone, calls = nn.Linear(8, 4), []
+    alone.register_forward_hook(lambda *a: calls.append(1))
+    assert use_mx4_linear_(alone) == 1 and isinstance(alone, Mx4Linear)
+    alone(torch.randn(2, 8))
+    assert calls == [1]                                            # hooks stay
+
 
 
 def test_keep_release_and_stale_weights():
@@ -104,6 +110,8 @@ def test_train_v1_with_clipping(tmp_path, extra):
     rep = train_v1.main(argv + ['--eval', '--exp-id', '1', '--round-weights', 'mx4'])
     assert rep['weights'] and set(rep['signature_before']) == set(rep['signature_after']) != set()
     assert np.isfinite(rep['after']['loss'])
+    with pytest.raises(ValueError, match='--eval'):
+        train_v1.main(argv + ['--round-weights', 'mx4'])
 
 
 def test_clipping_keeps_the_step_small(tmp_path):
