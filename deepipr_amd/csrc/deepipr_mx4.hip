@@ -946,7 +946,7 @@ inline bool quantise_fits(long long R, long long C) {
     return R <= 65535ll * kSumTiles * kQR && C <= kMaxSide && round_up(R, 128) / kQR * ((C + kQC - 1) / kQC) <= kMaxGrid;
 }
 inline bool product_fits(long long M, long long N, long long K) {
-    return M <= kMaxSide && N <= kMaxSide && K <= kMaxSide && tiles_of(M, N, 128) <= kMaxGrid && (N + 15) / 16 <= kMaxGrid &&
+    return M <= kMaxSide && N <= kMaxSide && K <= kMaxSide && tiles_of(M, N, 128) <= kMaxGrid && (N + 15) / 16 < kMaxGrid &&
            round_up(K, 128) / 128 <= kMaxGrid;
 }
 inline size_t product_bytes(long long M, long long N, long long K) {

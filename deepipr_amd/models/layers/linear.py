@@ -9,8 +9,9 @@ from deepipr_amd import mx4
 class Mx4Linear(nn.Linear):
     """nn.Linear with the same parameters and state_dict.  Training and evaluation quantise weight and input in the call
     (mx4.linear: output, dx and dw in 4 bits, dbias exact).  A net that only answers can `keep()` its weight in 4 bits instead of
-    quantising it per call; the kept codes are buffers outside the state_dict and are dropped by train(), load_state_dict() and
-    release().  A kept weight has no backward pass, and changing `weight` in place without a new keep() is an error."""
+    quantising it per call; the kept codes are buffers outside the state_dict and are dropped by train(), load_state_dict(), release(),
+    by a new `weight` and in copies of the layer.  A kept weight has no backward pass, and changing `weight` in place without a new
+    keep() is an error (what autograd does not see, a write through `weight.data`, needs a keep() of its own)."""
 
     def __init__(self, in_features, out_features, bias=True, device=None, dtype=None):
         super().__init__(in_features, out_features, bias, device, dtype)
@@ -36,6 +37,15 @@ class Mx4Linear(nn.Linear):
     def release(self):
         self.kept_codes = self.kept_scales = self._kept_version = None
         return self
+
+    def register_parameter(self, name, param):               # (also what `layer.weight = ...` calls)
+        if name == 'weight' and '_kept_version' in self.__dict__:
+            self.release()
+        super().register_parameter(name, param)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.release()
 
     def train(self, mode=True):
         if mode:

@@ -407,9 +407,9 @@ int deepipr_sgd_momentum_step_multi(float *param, float *momentum_buf, const lon
  * to 64 bits before they are squared or added, partial sums are added in a fixed order: bit-reproducible, no overflow or underflow
  * inside the sum.  A NaN anywhere gives NaN, an infinity without NaN gives infinity; an empty list gives 0.
  *   deepipr_grad_norm   *norm = n.
- *   deepipr_grad_clip   g *= f in place, f = min(1, max_norm / (n + 1e-6)); *norm = n, the norm BEFORE clipping.  f == 1 writes nothing (1 * g is g in every type).  A NaN norm makes every gradient NaN, an
- *                       infinite one makes the finite gradients 0.  Products are rounded once to the tensor's type.  Tensors that
- *                       share memory are refused.
+ *   deepipr_grad_clip   g *= f in place, f = min(1, max_norm / (n + 1e-6)); *norm = n, the norm BEFORE clipping.  f == 1 writes
+ *                       nothing (1 * g is g in every type).  A NaN norm makes every gradient NaN, an infinite one makes the finite
+ *                       gradients 0.  Products are rounded once to the tensor's type.  Tensors that share memory are refused.
  *   deepipr_sgd_momentum_step_clipped   the step of deepipr_sgd_momentum_step_dev behind that rule, on gradients that lie where
  *                       autograd left them: d = (f * grad_scale) * g + weight_decay * p; buf = momentum * buf + d; p -= lr * buf, with
  *                       n the 2-norm of grad_scale * g over the whole list.  hyper (device) = {lr, momentum, weight_decay, grad_scale,

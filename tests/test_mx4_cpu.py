@@ -32,7 +32,8 @@ def test_c_entries_refuse_before_any_launch():
     def mm(a=p, sa=p, b=p, sb=p, bias=None, bt=0, m=4, n=5, k=6, out=p, dtype=0, ws=None, nbytes=0):
         return lib.deepipr_mx4_matmul(a, sa, b, sb, bias, bt, m, n, k, out, dtype, ws, nbytes, None)
     for bad in (dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(out=None), dict(m=0), dict(n=0), dict(k=0), dict(dtype=-1),
-                dict(bias=p, bt=9), dict(a=p + 8), dict(bias=p + 1, bt=1), dict(out=p + 1, dtype=1), dict(m=1 << 41), dict(m=1 << 27, n=1 << 27)):
+                dict(bias=p, bt=9), dict(a=p + 8), dict(bias=p + 1, bt=1), dict(out=p + 1, dtype=1), dict(m=1 << 41), dict(m=1 << 27, n=1 << 27),
+                dict(n=1 << 27)):                                  # 2^23 workgroups of 512 threads: 2^32
         assert mm(**bad) == -1 and b'mx4_matmul' in lib.deepipr_last_error(), bad
 
 

@@ -1,4 +1,5 @@
 """Mx4Linear, use_mx4_linear_, round_weights_ and the command-line options, on the CPU stand-in of the kernels."""
+import copy
 import os
 import sys
 
@@ -141,3 +142,19 @@ def test_a_step_of_the_set_together():
     f = 0.1 / (n + 1e-6)
     assert torch.allclose(lin.weight, w0 - 0.5 * f * gw, atol=1e-6) and torch.allclose(lin.bias, b0 - 0.5 * f * gb, atol=1e-6)
     assert mx4.quantize(lin.weight.detach()).shape == (10, 64)
+
+
+def test_kept_codes_do_not_outlive_their_weight():
+    lin = Mx4Linear(40, 24)
+    x = torch.randn(3, 40)
+    with torch.no_grad():
+        lin.keep()
+        assert lin.kept_codes is not None and torch.equal(lin(x), mx4.linear(x, lin.weight, lin.bias))
+        twin = copy.deepcopy(lin)                                  # a copy's weight has a version count of its own
+        assert twin.kept_codes is None and torch.equal(twin(x), lin(x))
+        lin.weight = nn.Parameter(torch.randn(24, 40))
+        assert lin.kept_codes is None and torch.equal(lin(x), mx4.linear(x, lin.weight, lin.bias))
+        lin.keep()
+        lin.weight.mul_(2)
+        with pytest.raises(RuntimeError, match='keep'):
+            lin(x)
