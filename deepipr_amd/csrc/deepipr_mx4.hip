@@ -471,61 +471,88 @@ template <int X> __device__ __forceinline__ void load_block(const void *x, long 
     }
 }
 
-// Few rows (at most 16 MT): bound by reading b once.  A workgroup of eight waves takes 16 rows of b and all of a; wave i the steps
-// i, i + 8, ... of the columns, four of them on their way at once: with 16 rows a workgroup, 4096 rows of b fill 256 CUs and all
-// of b is asked for at once.  v_mfma_scale_f32_16x16x128_f8f6f4: lane l gives block l / 16 of row l % 16.  The waves' sums are added
-// through LDS in wave order.
-// X >= 0 (MT = 1): a comes in its own type X and the workgroup first quantises all of it into LDS, one block a thread and turn, while its
+// Few rows or small tiles: a workgroup of eight waves takes 16 MT rows of a and 16 NT of b; wave i the steps i, i + 8, ... of the columns, a few
+// of them on their way at once, straight to registers; the waves' sums are added through LDS in wave order.
+// v_mfma_scale_f32_16x16x128_f8f6f4: 16 lanes give one of the four blocks of 16 rows each.
+//   NT = 1, all of a in one workgroup (at most 64 rows): bound by reading b once; with 16 rows of b a workgroup, 4096 rows fill 256 CUs and all
+//           of b is asked for at once.
+//   NT = 2, 4 (64 x 32 and 64 x 64 outputs): up to a few hundred rows, where 128 x 128 tiles would leave CUs free or need the columns shared
+//           out over workgroups and a second launch to add up.  Bound by the L2s (253 x 4096 x 9216: 160 MB in 10 us).  Measured in us, this /
+//           the larger tiles at their best: 253 x 4096 x 9216 13.6 / 21.9, 256 x 1000 x 2048 4.4 / 9.9, 128 x 4096 x 4096 6.2 / 12.1, 1000^3
+//           4.7 / 8.0; 512 x 4096 x 4096 14.2 / 13.4, 2048^3 18.4 / 10.4.  Each step's place refilled at once instead of two steps
+//           together: 13.6 / 15.1, and 14.9 / 22.8 with b out of HBM.
+// X >= 0 (MT = NT = 1): a comes in its own type X and the workgroup first quantises all of it into LDS, one block a thread and turn, while its
 // first fetches of b are on their way.  Every workgroup does so again, but a launch is saved (3 us of the host's time, 2 of the card's).
 // Measured (us, fused / apart): 1 x 4096 x 9216 fp32 5.5 / 8.6, 4 x: 8.3 / 8.5, 8 x 4096 x 4096 7.0 / 6.9; 16 x 4096 x 4096 bf16 6.9 / 8.0,
 // fp32 10.9 / 7.0: up to 4096 bytes x blocks.
 constexpr int kFusedBlocks = 2048;
-template <int T, int MT, int X>
-__global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product P) {
-    constexpr int U = 4;
-    __shared__ f32x4 red[8][MT][64];
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c, unsigned sa, int ha, unsigned sb, int hb) {
+    const i32x8 av = {static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z), static_cast<int>(a.w), 0, 0, 0, 0};
+    const i32x8 bv = {static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z), static_cast<int>(b.w), 0, 0, 0, 0};
+    const int x = static_cast<int>(sa), y = static_cast<int>(sb);           // the halves' bytes (ha, hb are constants of the unrolled loops)
+    if (ha == 0 && hb == 0) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, x, 0, y);
+    if (ha == 0) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, x, 1, y);
+    if (hb == 0) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 1, x, 0, y);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 1, x, 1, y);
+}
+// Out of word l of a 64-row group in lane l: [i] = the words of the rows 16 i + l % 16 (and 32 more) for all four blocks
+template <int TILES> __device__ __forceinline__ u32x2 words(unsigned w, int shift) {
+    if (TILES == 1) return u32x2{w >> shift, 0};
+    const u32x2 v = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    return u32x2{v.x >> shift, v.y >> shift};
+}
+template <int T, int MT, int NT, int X>
+__global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product A, const Product B, unsigned first) {
+    constexpr int U = NT == 1 ? 4 : 2;
+    __shared__ f32x4 red[8][MT * NT][64];
     __shared__ u32x4 codes[X >= 0 ? kFusedBlocks : 1];
     __shared__ unsigned char scales[X >= 0 ? kFusedBlocks : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long n0 = static_cast<long long>(blockIdx.x) * 16;
-    const int r = lane & 15, blk = lane >> 4;
-    // the byte of a scale word that holds this lane's block for a row: (block / 2, row / 32)
-    const auto word_of = [&](long long row) { return row / 64 * 64 + (blk & 1) * 32 + (row & 31); };
-    const auto byte_of = [&](long long row) { return static_cast<int>((blk >> 1) * 2 + (row >> 5 & 1)) * 8; };
-    const long long brow = min(n0 + r, P.N - 1);
-    const unsigned char *pb = P.b + brow * 64 + blk * 16, *pa[MT];
-    const unsigned *qb = P.sb + word_of(brow), *qa[MT];
-    const int hb = byte_of(brow);
-    int ha[MT];
+    const bool of_a = blockIdx.x < first;
+    const Product &P = of_a ? A : B;
+    // neighbours share their rows of b: with NT > 1 they meet in one XCD's L2
+    const int index = of_a ? blockIdx.x : blockIdx.x - first, count = of_a ? first : gridDim.x - first;
+    const int id = NT == 1 ? index : dipr_xcd_contiguous(index, count);
+    const int tiles_m = static_cast<int>((P.last - P.first + 16 * MT - 1) / (16 * MT));
+    const long long n0 = static_cast<long long>(id / tiles_m) * (16 * NT), m0 = P.first + id % tiles_m * (16 * MT);
+    const int r = lane & 15, blk = (lane >> 4 & 1) * 2 + (lane >> 5);      // (any order of the four blocks will do that a and b share)
+    // A single tile's lane loads the scale word of its own row and block.  Two or four tiles are half of or a whole 64-row group: lane l loads
+    // the group's word l, and a swap of rows of 16 lanes hands every tile its words.
+    const unsigned char *pb[NT], *pa[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) pb[i] = P.b + min(n0 + i * 16 + r, P.N - 1) * 64 + blk * 16;
+    const auto word_of = [&](long long row, int tiles) {
+        return row / 64 * 64 + (tiles > 1 ? lane : (blk & 1) * 32 + static_cast<int>((row + r) & 31));
+    };
+    const auto shift_of = [&](long long row) { return (blk >> 1) * 16 + static_cast<int>(row >> 5 & 1) * 8; };
+    const unsigned *qb = P.sb + word_of(n0, NT), *qa = nullptr;
+    const int hb = shift_of(n0);
+    int ha = 0;
     if (X < 0) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const long long row = min(P.first + t * 16 + r, P.last - 1);
-            pa[t] = P.a + row * 64 + blk * 16;
-            qa[t] = P.sa + word_of(row);
-            ha[t] = byte_of(row);
-        }
+        for (int t = 0; t < MT; ++t) pa[t] = P.a + min(m0 + t * 16 + r, P.last - 1) * 64 + blk * 16;
+        qa = P.sa + word_of(m0, MT);
+        ha = shift_of(m0);
     }
     const long long gm = row_groups(P.M) * 64, gn = row_groups(P.N) * 64;
-    f32x4 acc[MT] = {};
-    u32x4 fb[U], fa[U][MT];
-    unsigned wb[U], wa[U][MT];
-    const auto fetch = [&](int k0) {
+    f32x4 acc[NT][MT] = {};
+    u32x4 fb[U][NT], fa[U][MT];
+    unsigned wb[U], wa[U];
+    const auto fetch = [&](int u, int step) {             // (behind the last step: that one again)
+        const long long k = min(step, P.kt - 1);
+        wb[u] = qb[k * gn];
+        if (X < 0) wa[u] = qa[k * gm];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long long k = min(k0 + 8 * u, P.kt - 1);
-            fb[u] = *reinterpret_cast<const u32x4 *>(pb + k * P.N * 64);
-            wb[u] = qb[k * gn];
-            if (X < 0) {
+        for (int i = 0; i < NT; ++i) fb[u][i] = *reinterpret_cast<const u32x4 *>(pb[i] + k * P.N * 64);
+        if (X < 0) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    fa[u][t] = *reinterpret_cast<const u32x4 *>(pa[t] + k * P.M * 64);
-                    wa[u][t] = qa[t][k * gm] >> ha[t];
-                }
-            }
+            for (int t = 0; t < MT; ++t) fa[u][t] = *reinterpret_cast<const u32x4 *>(pa[t] + k * P.M * 64);
         }
     };
-    fetch(wave);
+    if (NT == 1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) fetch(u, wave + 8 * u);
+    }
     if (X >= 0) {
         const int per = P.kt * 4, blocks = static_cast<int>(P.M) * per;
         for (int i = threadIdx.x; i < blocks; i += 512) {
@@ -539,45 +566,67 @@ __global__ __launch_bounds__(512) void k_mx4_gemm_rows(const Product P) {
         }
         __syncthreads();
     }
-    for (int k0 = wave; k0 < P.kt; k0 += 8 * U) {
-        if (k0 != wave) fetch(k0);
+    const auto multiply = [&](int u, int step) {
+        if (X >= 0) {
+            const int at = (r * P.kt + step) * 4 + blk;
+            const bool mine = r < static_cast<int>(P.M);
+            fa[u][0] = mine ? codes[at] : u32x4{0, 0, 0, 0};
+            wa[u] = mine ? scales[at] : 0;
+        }
+        const u32x2 sb = words<NT>(wb[u], hb), sa = words<MT>(wa[u], ha);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[i][t] = mfma16(fb[u][i], fa[u][t], acc[i][t], sb[i & 1], i >> 1, sa[t & 1], t >> 1);
+    };
+    int k = wave;
+    if (NT > 1 && k + 8 * (2 * U - 1) < P.kt) {          // each step's place is refilled at once
+#pragma unroll
+        for (int u = 0; u < U; ++u) fetch(u, k + 8 * u);
+        for (; k + 8 * (2 * U - 1) < P.kt; k += 8 * U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                multiply(u, k + 8 * u);
+                fetch(u, k + 8 * (U + u));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(u, k + 8 * u);
+        k += 8 * U;
+    }
+    for (; k < P.kt; k += 8 * U) {                       // the last steps, and all of a short or narrow product's
+        if (NT > 1 || k != wave) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) fetch(u, k + 8 * u);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (k0 + 8 * u >= P.kt) break;
-            if (X >= 0) {
-                const int at = (r * P.kt + k0 + 8 * u) * 4 + blk;
-                const bool mine = r < static_cast<int>(P.M);
-                fa[u][0] = mine ? codes[at] : u32x4{0, 0, 0, 0};
-                wa[u][0] = mine ? scales[at] : 0;
-            }
-            const i32x8 bv = {static_cast<int>(fb[u].x), static_cast<int>(fb[u].y), static_cast<int>(fb[u].z), static_cast<int>(fb[u].w), 0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const i32x8 av = {static_cast<int>(fa[u][t].x), static_cast<int>(fa[u][t].y), static_cast<int>(fa[u][t].z),
-                                  static_cast<int>(fa[u][t].w), 0, 0, 0, 0};
-                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv, av, acc[t], 4, 4, 0, static_cast<int>(wb[u] >> hb), 0,
-                                                                          static_cast<int>(wa[u][t]));
-            }
+            if (k + 8 * u >= P.kt) break;
+            multiply(u, k + 8 * u);
         }
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) red[wave][i * MT + t][lane] = acc[i][t];
     __syncthreads();
-    if (wave >= MT) return;
-    f32x4 v = red[0][wave][lane];
+    for (int tile = wave; tile < MT * NT; tile += 8) {
+        f32x4 v = red[0][tile][lane];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v += red[i][wave][lane];
-    const long long m = P.first + wave * 16 + r, n = n0 + blk * 4;
-    if (m >= P.last) return;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (P.bias && n + j < P.N) v[j] += bias_at(P.bias, P.bias_type, n + j);
-    if (n + 4 <= P.N) {
-        store4<T>(element<T>(P.out, m * P.N + n), v);
-    } else {
+        for (int i = 1; i < 8; ++i) v += red[i][tile][lane];
+        const long long m = m0 + tile % MT * 16 + r, n = n0 + tile / MT * 16 + (lane >> 4) * 4;
+        if (m >= P.last) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (n + j < P.N) store1<T>(P.out, m * P.N + n + j, v[j]);
+            if (P.bias && n + j < P.N) v[j] += bias_at(P.bias, P.bias_type, n + j);
+        if (n + 4 <= P.N) {
+            store4<T>(element<T>(P.out, m * P.N + n), v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < P.N) store1<T>(P.out, m * P.N + n + j, v[j]);
+        }
     }
 }
 
@@ -805,12 +854,12 @@ template <int T> void launch_quantise(DiprProf &prof, const Matrix &m, const Mat
 
 // ---- which kernels a product takes
 // Estimated from measured times (ns): a step of 128 columns costs a 256 x 256 tile 780, a 128 x 128 tile 270 where it has the CU for itself
-// and 690 where two share it; begin and end of a tile 6 000 / 3 000; a second launch that adds up partial sums 4 000 and their bytes at
-// 4 TB/s.  Measured (us): 8192^3 253 large, 355 small; 4096 x 4096 x 8200 65 / 78; 2048^3 18.3 / 10.1; 253 x 4096 x 9216 52 large, 24.5
+// and 690 where two share it, a 64 x 64 tile 140 (160 where several follow on a CU) and a 64 x 32 tile 100 (130); begin and end of a tile
+// 6 000 / 4 500 / 3 500 / 3 000; a second launch that adds up partial sums 4 000 and their bytes at 4 TB/s.  Measured (us): 8192^3 253 large, 355 small; 4096 x 4096 x 8200 65 / 78; 2048^3 18.3 / 10.1; 253 x 4096 x 9216 52 large, 24.5
 // small, 20.9 small with the columns in three; 512 x 512 x 16384 34.8 whole, 15.5 in eight; 1000^3 8.2 whole, 13 in two; 32 x 4096 x 9216 8.2
 // by the kernel for few rows, 12.1 at best by the others.
 struct Plan {
-    enum { kRows, kSmall, kLarge } form;
+    enum { kRows, k64x32, k64x64, kSmall, kLarge } form;
     int splits;                  // kSmall only
     long long tail;              // kLarge only: rows at the end that go to the kernel for few rows (0: none)
 };
@@ -827,7 +876,13 @@ inline double small_ns(long long m, long long n, long long kt, int splits) {
     const double slots = 2.0 * cu_count(), tiles = static_cast<double>(tiles_of(m, n, 128)) * splits;
     const double step = tiles <= slots / 2 ? 270.0 : 690.0 * (tiles > slots ? tiles / slots : 1.0);
     const double sums = splits > 1 ? 4000.0 + static_cast<double>(splits) * m * n * 8 / 4000.0 : 0.0;
-    return step * static_cast<double>((kt + splits - 1) / splits) + 3000.0 + sums;
+    return step * static_cast<double>((kt + splits - 1) / splits) + 4500.0 + sums;
+}
+inline long long strips_of(long long m, long long n, int nt) { return ((m + 63) / 64) * ((n + 16 * nt - 1) / (16 * nt)); }
+inline double strip_ns(long long m, long long n, long long kt, int nt) {
+    const long long rounds = (strips_of(m, n, nt) + cu_count() - 1) / cu_count();
+    const double step = nt == 2 ? (rounds > 1 ? 130.0 : 100.0) : (rounds > 1 ? 160.0 : 140.0);
+    return step * static_cast<double>(rounds) * static_cast<double>(kt) + (nt == 2 ? 3000.0 : 3500.0);
 }
 Plan plan(long long M, long long N, long long kt) {
     Plan p = {Plan::kRows, 1, 0};
@@ -850,21 +905,40 @@ Plan plan(long long M, long long N, long long kt) {
             p.tail = 0;
         }
     }
+    for (int nt = 2; nt <= 4; nt += 2) {
+        if (strips_of(M, N, nt) > 8 * cu_count()) continue;
+        const double t = strip_ns(M, N, kt, nt);
+        if (t < best) {
+            best = t;
+            p.form = nt == 2 ? Plan::k64x32 : Plan::k64x64;
+            p.splits = 1;
+            p.tail = 0;
+        }
+    }
     return p;
 }
 
 template <int T> void launch_rows(DiprProf &prof, const Product &P, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>((P.N + 15) / 16)), block(512);
     const long long rows = P.last - P.first;
-    if (rows <= 16) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 1, -1>), grid, block, st, P);
-    else if (rows <= 32) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 2, -1>), grid, block, st, P);
-    else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, -1>), grid, block, st, P);
+    if (rows <= 16) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 1, 1, -1>), grid, block, st, P, P, grid.x);
+    else if (rows <= 32) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 2, 1, -1>), grid, block, st, P, P, grid.x);
+    else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, 1, -1>), grid, block, st, P, P, grid.x);
 }
 
 template <int T> void launch_product(DiprProf &prof, Product P, const Product *other, float *part, hipStream_t st) {
     const dim3 block(kThreads);
     const Plan p = plan(P.M, P.N, P.kt);
     if (p.form == Plan::kRows) return launch_rows<T>(prof, P, st);
+    if (p.form == Plan::k64x32 || p.form == Plan::k64x64) {
+        const int nt = p.form == Plan::k64x32 ? 2 : 4;
+        const unsigned first = static_cast<unsigned>(strips_of(P.M, P.N, nt));
+        const dim3 grid(first + (other ? static_cast<unsigned>(strips_of(other->M, other->N, nt)) : 0u)), wide(512);
+        const Product &Q = other ? *other : P;
+        if (nt == 2) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, 2, -1>), grid, wide, st, P, Q, first);
+        else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, 4, -1>), grid, wide, st, P, Q, first);
+        return;
+    }
     Product O = other ? *other : P;
     const long long tails[2] = {p.tail, other ? plan(O.M, O.N, O.kt).tail : 0};
     Product *both[2] = {&P, &O};
@@ -998,9 +1072,9 @@ void product_of_rows(const void *x, int dtype, long long x_stride, const void *b
     prof.bytes = 2.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
     const dim3 grid(static_cast<unsigned>((N + 15) / 16)), block(512);
     switch (dtype) {
-        case F32: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<F32, 1, F32>), grid, block, st, P); break;
-        case BF16: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<BF16, 1, BF16>), grid, block, st, P); break;
-        default: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<F16, 1, F16>), grid, block, st, P); break;
+        case F32: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<F32, 1, 1, F32>), grid, block, st, P, P, grid.x); break;
+        case BF16: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<BF16, 1, 1, BF16>), grid, block, st, P, P, grid.x); break;
+        default: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<F16, 1, 1, F16>), grid, block, st, P, P, grid.x); break;
     }
 }
 

@@ -162,9 +162,12 @@ def test_products_are_exact(mnk, dtype):
 
 
 @pytest.mark.parametrize('mnk', [(64, 4200, 1200), (65, 300, 9000), (128, 128, 20000), (4104, 4096, 130), (4160, 4000, 300), (4352, 4100, 250),
-                                 (2500, 3000, 700)])
+                                 (2500, 3000, 700), (4104, 4096, 4100), (2300, 3900, 5000), (300, 100, 20000), (512, 4000, 2050),
+                                 (100, 500, 3000), (100, 500, 3100), (70, 30, 3900), (190, 490, 4200), (130, 510, 6300), (65, 33, 8200),
+                                 (250, 4000, 3000), (250, 4001, 3100), (253, 3999, 3900), (200, 3900, 4200), (256, 4090, 6300), (129, 4050, 8200)])
 def test_products_of_every_form_are_exact(mnk):
-    """Few rows; columns shared out over workgroups; whole tiles with a few rows behind them; large tiles with ragged ends."""
+    """Few rows; 64 x 32 and 64 x 64 tiles over all counts of steps a wave; columns shared out over workgroups; whole tiles with a few rows
+    behind them; large tiles with ragged ends."""
     from deepipr_amd import mx4
     m, n, k = mnk
     a, b = _codes(m, k, 4, (0,)).to(DEV), _codes(n, k, 5, (0,)).to(DEV)                # multiples of 1/4 below 2^20: exact
@@ -193,7 +196,7 @@ def _values(x, dim):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('mnk', [(1, 40, 100), (5, 70, 333), (65, 130, 257), (256, 300, 1024), (33, 1000, 2048)])
+@pytest.mark.parametrize('mnk', [(1, 40, 100), (5, 70, 333), (65, 130, 257), (256, 300, 1024), (33, 1000, 2048), (512, 512, 4000)])
 def test_linear_and_its_gradients(mnk, dtype):
     from deepipr_amd import mx4
     m, n, k = mnk
