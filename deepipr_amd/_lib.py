@@ -86,6 +86,7 @@ SIGNATURES = {
     'deepipr_mx4_matmul': (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _sz, _vp]),
     'deepipr_mx4_linear_saved_bytes': (_sz, [_i64, _i64, _i64, _int, _int]),
     'deepipr_mx4_linear_scratch_bytes': (_sz, [_i64, _i64, _i64, _int]),
+    'deepipr_mx4_linear_kept_scratch_bytes': (_sz, [_int, _i64, _i64, _i64]),
     'deepipr_mx4_linear_fwd': (_int, [_vp, _int, _i64, _vp, _int, _i64, _vp, _vp, _vp, _int, _i64, _i64, _i64, _int, _int, _vp, _sz,
                                       _vp, _vp, _sz, _vp]),
     'deepipr_mx4_linear_bwd': (_int, [_vp, _int, _i64, _i64, _i64, _i64, _int, _int, _vp, _sz, _vp, _int, _vp, _int, _f32p, _vp, _sz,

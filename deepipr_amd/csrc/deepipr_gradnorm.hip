@@ -26,8 +26,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kEntries = 240;                 // entries per launch: 240 * 16 bytes of the 4 KB of launch arguments
 constexpr int kMaxGroups = 1024;              // workgroups per launch: 4 of 4 waves per CU
-constexpr int kMinUnits = 64, kMaxUnits = 256;          // a run is 4096 to 16384 elements
+// A run is 1024 to 16384 elements: a workgroup takes about 0.1 us (clip 0.2) for every tensor in its run (measured: 20 000 elements in 239
+// tensors 14 us with runs of 1024 at least, 40 with 4096; a million in 100 11 / 9).
+constexpr unsigned kMinUnits = 16, kMaxUnits = 256;
 constexpr int kMaxPartials = 4096;            // workgroups of all launches of one list
+constexpr int kOneThreads = 1024;
+constexpr unsigned long long kOneUnits = 128; // up to 8192 elements in up to 4 tensors: one workgroup, one launch (5130 in two 5.4 us,
+constexpr int kOneEntries = 4;                // 7.0 in two launches, and one launch less on the host; 16384 in two 6.6 / 5.8)
 constexpr long long kEntryMax = 1ll << 29;    // elements per entry; longer tensors take several entries
 constexpr double kClipEps = 1e-6;
 
@@ -110,12 +115,14 @@ template <int P> __device__ __forceinline__ double wave_join(double v) {
     for (int off = 32; off > 0; off >>= 1) v = join<P>(v, __shfl_xor(v, off, 64));
     return v;
 }
-// The same value in every thread; `red`: 4 doubles of LDS
-template <int P> __device__ __forceinline__ double block_join(double v, double *red) {
+// The same value in every thread; `red`: a double of LDS for each of the TH / 64 waves
+template <int P, int TH> __device__ __forceinline__ double block_join(double v, double *red) {
     v = wave_join<P>(v);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    const double r = join<P>(join<P>(red[0], red[1]), join<P>(red[2], red[3]));
+    double r = join<P>(join<P>(red[0], red[1]), join<P>(red[2], red[3]));
+#pragma unroll
+    for (int i = 4; i < TH / 64; ++i) r = join<P>(r, red[i]);
     __syncthreads();
     return r;
 }
@@ -145,7 +152,7 @@ template <class F> __device__ __forceinline__ void walk(const List &L, F f) {
     }
 }
 
-template <int T, int P>
+template <int T, int P, int TH>
 __device__ __forceinline__ void norm_piece(const void *base, unsigned a, unsigned b, double *acc) {
     typedef typename Elem<T>::type E;
     constexpr int V = Elem<T>::kVec;
@@ -159,16 +166,16 @@ __device__ __forceinline__ void norm_piece(const void *base, unsigned a, unsigne
     const u32x4 *q = reinterpret_cast<const u32x4 *>(p);
     const unsigned nv = n / V;
     unsigned i = threadIdx.x;
-    for (; i + 3 * kThreads < nv; i += 4 * kThreads) {
+    for (; i + 3 * TH < nv; i += 4 * TH) {
         Pack<T> v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j].q = q[i + j * kThreads];
+        for (int j = 0; j < 4; ++j) v[j].q = q[i + j * TH];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int k = 0; k < V; ++k) take<P>(acc[k & 3], Elem<T>::get(v[j].e[k]));
     }
-    for (; i < nv; i += kThreads) {
+    for (; i < nv; i += TH) {
         Pack<T> v;
         v.q = q[i];
 #pragma unroll
@@ -178,19 +185,23 @@ __device__ __forceinline__ void norm_piece(const void *base, unsigned a, unsigne
     if (threadIdx.x < rest) take<P>(acc[0], Elem<T>::get(p[nv * V + threadIdx.x]));
 }
 
-template <int P>
-__global__ __launch_bounds__(kThreads) void k_norm_partials(const List L, double *__restrict__ part) {
-    __shared__ double red[4];
+// This workgroup's part of the sum, in every thread
+template <int P, int TH> __device__ __forceinline__ double norm_runs(const List &L, double *red) {
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
     walk(L, [&](int i, unsigned a, unsigned b) {
         const void *p = L.ptr[i];
         switch (L.count[i] >> 30) {
-            case F32: norm_piece<F32, P>(p, a, b, acc); break;
-            case BF16: norm_piece<BF16, P>(p, a, b, acc); break;
-            default: norm_piece<F16, P>(p, a, b, acc); break;
+            case F32: norm_piece<F32, P, TH>(p, a, b, acc); break;
+            case BF16: norm_piece<BF16, P, TH>(p, a, b, acc); break;
+            default: norm_piece<F16, P, TH>(p, a, b, acc); break;
         }
     });
-    const double s = block_join<P>(join<P>(join<P>(acc[0], acc[1]), join<P>(acc[2], acc[3])), red);
+    return block_join<P, TH>(join<P>(join<P>(acc[0], acc[1]), join<P>(acc[2], acc[3])), red);
+}
+template <int P>
+__global__ __launch_bounds__(kThreads) void k_norm_partials(const List L, double *__restrict__ part) {
+    __shared__ double red[4];
+    const double s = norm_runs<P, kThreads>(L, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
@@ -198,7 +209,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_partials(const List L, double
 template <int P> __device__ __forceinline__ double norm_of(const double *__restrict__ part, int n, double *red) {
     double v = 0.0;
     for (int i = threadIdx.x; i < n; i += kThreads) v = join<P>(v, part[i]);
-    v = block_join<P>(v, red);
+    v = block_join<P, kThreads>(v, red);
     return P == 2 ? sqrt(v) : v;
 }
 
@@ -217,7 +228,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_finish(const double *__restri
     if (threadIdx.x == 0) *norm = static_cast<float>(v);
 }
 
-template <int T>
+template <int T, int TH>
 __device__ __forceinline__ void scale_piece(void *base, unsigned a, unsigned b, double f) {
     typedef typename Elem<T>::type E;
     constexpr int V = Elem<T>::kVec;
@@ -230,18 +241,18 @@ __device__ __forceinline__ void scale_piece(void *base, unsigned a, unsigned b, 
     u32x4 *q = reinterpret_cast<u32x4 *>(p);
     const unsigned nv = n / V;
     unsigned i = threadIdx.x;
-    for (; i + 3 * kThreads < nv; i += 4 * kThreads) {
+    for (; i + 3 * TH < nv; i += 4 * TH) {
         Pack<T> v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j].q = q[i + j * kThreads];
+        for (int j = 0; j < 4; ++j) v[j].q = q[i + j * TH];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int k = 0; k < V; ++k) v[j].e[k] = Elem<T>::put(times(f, Elem<T>::get(v[j].e[k])));
-            q[i + j * kThreads] = v[j].q;
+            q[i + j * TH] = v[j].q;
         }
     }
-    for (; i < nv; i += kThreads) {
+    for (; i < nv; i += TH) {
         Pack<T> v;
         v.q = q[i];
 #pragma unroll
@@ -252,6 +263,16 @@ __device__ __forceinline__ void scale_piece(void *base, unsigned a, unsigned b, 
     if (threadIdx.x < rest) p[nv * V + threadIdx.x] = Elem<T>::put(times(f, Elem<T>::get(p[nv * V + threadIdx.x])));
 }
 
+template <int TH> __device__ __forceinline__ void scale_runs(const List &L, double f) {
+    walk(L, [&](int i, unsigned a, unsigned b) {
+        void *p = const_cast<void *>(L.ptr[i]);
+        switch (L.count[i] >> 30) {
+            case F32: scale_piece<F32, TH>(p, a, b, f); break;
+            case BF16: scale_piece<BF16, TH>(p, a, b, f); break;
+            default: scale_piece<F16, TH>(p, a, b, f); break;
+        }
+    });
+}
 // A factor of exactly 1 leaves every value as it is (1 * x = x in every type): nothing is read or written then.
 template <int P>
 __global__ __launch_bounds__(kThreads) void k_clip(const List L, const double *__restrict__ part, int n, float max_norm,
@@ -260,15 +281,19 @@ __global__ __launch_bounds__(kThreads) void k_clip(const List L, const double *_
     const double v = norm_of<P>(part, n, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(v);
     const double f = factor_of(v, max_norm);
-    if (f == 1.0) return;
-    walk(L, [&](int i, unsigned a, unsigned b) {
-        void *p = const_cast<void *>(L.ptr[i]);
-        switch (L.count[i] >> 30) {
-            case F32: scale_piece<F32>(p, a, b, f); break;
-            case BF16: scale_piece<BF16>(p, a, b, f); break;
-            default: scale_piece<F16>(p, a, b, f); break;
-        }
-    });
+    if (f != 1.0) scale_runs<kThreads>(L, f);
+}
+
+// A short list in one launch of one workgroup: the norm and, if CLIP, the scaling
+template <int P, bool CLIP>
+__global__ __launch_bounds__(kOneThreads) void k_one(const List L, float max_norm, float *__restrict__ norm) {
+    __shared__ double red[kOneThreads / 64];
+    double v = norm_runs<P, kOneThreads>(L, red);
+    if (P == 2) v = sqrt(v);
+    if (threadIdx.x == 0) *norm = static_cast<float>(v);
+    if (!CLIP) return;
+    const double f = factor_of(v, max_norm);
+    if (f != 1.0) scale_runs<kOneThreads>(L, f);
 }
 
 __device__ __forceinline__ void sgd1(float &p, float g, float &buf, float lr, float mu, float wd, double gs) {
@@ -447,6 +472,24 @@ template <int P> int partials(const char *what, const DeepiprTensor *t, int n, c
     return dipr_check_launch(what);
 }
 
+// A list that one workgroup takes
+inline bool is_short(const DeepiprTensor *t, int n, unsigned long long units) { return units <= kOneUnits && entries_of(t, n) <= kOneEntries; }
+template <bool CLIP> int one(const char *what, const DeepiprTensor *t, int n, unsigned long long units, int norm_type, size_t bytes, float max_norm,
+                             float *norm, hipStream_t st) {
+    DiprProf prof(CLIP ? DEEPIPR_K_GRAD_CLIP : DEEPIPR_K_GRAD_NORM);
+    prof.bytes = (CLIP ? 3.0 : 1.0) * static_cast<double>(bytes);
+    launches<false>(t, n, Cut{static_cast<unsigned>(units), 1}, [&](const List &L, int) {
+        const dim3 grid(1), block(kOneThreads);
+        switch (norm_type) {
+            case 2: DIPR_LAUNCH(prof, (k_one<2, CLIP>), grid, block, st, L, max_norm, norm); break;
+            case 1: DIPR_LAUNCH(prof, (k_one<1, CLIP>), grid, block, st, L, max_norm, norm); break;
+            default: DIPR_LAUNCH(prof, (k_one<0, CLIP>), grid, block, st, L, max_norm, norm); break;
+        }
+        return true;
+    });
+    return dipr_check_launch(what);
+}
+
 int check_common(const char *what, int norm_type, const void *workspace, size_t workspace_bytes) {
     if (norm_type != 0 && norm_type != 1 && norm_type != 2) return dipr_fail(DEEPIPR_EINVAL, "%s: norm_type 0 (infinity), 1 or 2", what);
     if (!workspace || workspace_bytes < kMaxPartials * sizeof(double))
@@ -483,6 +526,7 @@ int deepipr_grad_norm(const DeepiprTensor *tensors, int n, int norm_type, float 
     double *part = static_cast<double *>(workspace);
     const Cut per = cut(tensors, n, units);
     if (!per.groups) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
+    if (elements && is_short(tensors, n, units)) return one<false>(what, tensors, n, units, norm_type, bytes, 0.0f, norm, st);
     int used = 0;
     if (elements) {
         rc = list_partials(what, tensors, n, norm_type, per, bytes, part, &used, st);
@@ -516,6 +560,7 @@ int deepipr_grad_clip(const DeepiprTensor *tensors, int n, int norm_type, float 
     double *part = static_cast<double *>(workspace);
     const Cut per = cut(tensors, n, units);
     if (!per.groups) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
+    if (is_short(tensors, n, units)) return one<true>(what, tensors, n, units, norm_type, bytes, max_norm, norm, st);
     int used = 0;
     rc = list_partials(what, tensors, n, norm_type, per, bytes, part, &used, st);
     if (rc != DEEPIPR_OK) return rc;

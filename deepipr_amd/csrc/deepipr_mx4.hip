@@ -1112,10 +1112,10 @@ struct ForwardScratch {
     Quantised x, w;
     void *work;
     size_t bytes;
-    ForwardScratch(void *p, long long M, long long N, long long K) {
+    ForwardScratch(void *p, long long M, long long N, long long K, bool kept) {
         Cut c(p);
         x = take_matrix(c, M, K);
-        w = take_matrix(c, N, K);
+        if (!kept) w = take_matrix(c, N, K);
         work = c.take(product_bytes(M, N, K));
         bytes = c.used;
     }
@@ -1138,6 +1138,8 @@ inline bool linear_fits(long long M, long long N, long long K) {
     return M > 0 && N > 0 && K > 0 && quantise_fits(M, K) && quantise_fits(N, K) && quantise_fits(M, N) && product_fits(M, N, K) &&
            product_fits(M, K, N) && product_fits(N, K, M);
 }
+// Whether a product on kept weights quantises its rows itself
+inline bool is_fused(long long M, long long K, int dtype) { return M <= 16 && M * (round_up(K, 128) / 32) * elem_bytes(dtype) <= 2 * kFusedBlocks; }
 inline bool good_matrix(const void *p, int dtype, long long rows, long long cols, long long stride) {
     return p && good_dtype(dtype) && aligned(p, elem_bytes(dtype)) && (rows <= 1 || stride >= cols);
 }
@@ -1229,7 +1231,10 @@ size_t deepipr_mx4_linear_saved_bytes(long long M, long long N, long long K, int
 }
 size_t deepipr_mx4_linear_scratch_bytes(long long M, long long N, long long K, int backward) {
     if (!linear_fits(M, N, K)) return 0;
-    return backward ? BackwardScratch(nullptr, M, N, K).bytes : ForwardScratch(nullptr, M, N, K).bytes;
+    return backward ? BackwardScratch(nullptr, M, N, K).bytes : ForwardScratch(nullptr, M, N, K, false).bytes;
+}
+size_t deepipr_mx4_linear_kept_scratch_bytes(int x_dtype, long long M, long long N, long long K) {
+    return !good_dtype(x_dtype) || !linear_fits(M, N, K) || is_fused(M, K, x_dtype) ? 0 : ForwardScratch(nullptr, M, N, K, true).bytes;
 }
 
 int deepipr_mx4_linear_fwd(const void *x, int x_dtype, long long x_stride, const void *w, int w_dtype, long long w_stride, const void *w_codes,
@@ -1243,11 +1248,12 @@ int deepipr_mx4_linear_fwd(const void *x, int x_dtype, long long x_stride, const
         (bias && (!good_dtype(bias_dtype) || !aligned(bias, elem_bytes(bias_dtype)))))
         return dipr_fail(DEEPIPR_EINVAL, "%s: bad argument", what);
     const Saved s(saved, M, N, K, need_dx != 0, need_dw != 0);
-    const ForwardScratch f(scratch, M, N, K);
-    if (!scratch || !aligned(scratch, 16) || scratch_bytes < f.bytes || (s.bytes && (!saved || !aligned(saved, 16) || saved_bytes < s.bytes)))
+    const bool fused = kept && is_fused(M, K, x_dtype);
+    const ForwardScratch f(scratch, M, N, K, kept);
+    if ((!fused && (!scratch || !aligned(scratch, 16) || scratch_bytes < f.bytes)) || (s.bytes && (!saved || !aligned(saved, 16) || saved_bytes < s.bytes)))
         return dipr_fail(DEEPIPR_EINVAL, "%s: scratch or saved memory too small or misaligned", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (kept && M <= 16 && M * (round_up(K, 128) / 32) * elem_bytes(x_dtype) <= 2 * kFusedBlocks) {
+    if (fused) {
         product_of_rows(x, x_dtype, x_stride, w_codes, w_scales, bias, bias_dtype, M, N, K, out, st);
         return dipr_check_launch(what);
     }

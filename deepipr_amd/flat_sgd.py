@@ -99,6 +99,9 @@ class FlatSGD(torch.optim.Optimizer):
                 view.copy_(p)
                 p.data = view                                     # the Parameter now lives in the flat buffer
                 self._slots.append((p, off))
+        # the launch arguments of a clipped step whose gradients are all there, without the addresses (those are read in every step)
+        self._clip_rows = P.kernels.clipped_rows([p.numel() for p, _ in self._slots], [off for _, off in self._slots], total) \
+            if self._clips else None
         # Buckets in gradient-ready order, cut where the cumulative size passes each fraction.  For ResNet18
         # (reverse order: linear, layer4.1 42 %, layer4.0 33 %, layer3 19 %, rest 6 %) that is four all-reduces
         # of 19 / 15 / 8.5 / 2.7 MB; every bucket but the last is launched from a gradient hook while earlier
@@ -366,8 +369,8 @@ class FlatSGD(torch.optim.Optimizer):
             have = [(self.flat_grad[off:off + p.numel()], off) for i, (p, off) in enumerate(self._slots) if i not in skip] \
                 if missing else [(self.flat_grad, 0)]
             if have:
-                P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, [g for g, _ in have], [o for _, o in have],
-                                                    self._hyper, self.grad_norm)
+                rows = P.kernels.clipped_rows([g.numel() for g, _ in have], [o for _, o in have], self.flat_param.numel())
+                P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, [g for g, _ in have], rows, self._hyper, self.grad_norm)
             else:
                 self.grad_norm.zero_()
         elif not missing:
@@ -440,18 +443,15 @@ class FlatSGD(torch.optim.Optimizer):
         """One GPU, clipping: norm and update read the gradients where autograd left them (their addresses travel in the launch
         arguments), eager and captured alike; parameters without a gradient are left alone.  -> False if a gradient cannot be
         addressed that way (the packed path is taken then)."""
-        grads = [p.grad for p, _ in self._slots]
-        offsets = [off for _, off in self._slots]
+        grads, rows = [p.grad for p, _ in self._slots], self._clip_rows
         if any(g is None for g in grads):
-            offsets = [off for off, g in zip(offsets, grads) if g is not None]
-            grads = [g for g in grads if g is not None]
-        if {g.dtype for g in grads} - {torch.float32} or not all(map(torch.Tensor.is_contiguous, grads)) or \
-                set(map(torch.Tensor.get_device, grads)) - {self.flat_param.get_device()}:
-            return False
-        if grads:
-            P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, grads, offsets, self._hyper, self.grad_norm)
-        else:
+            have = [(g, off) for g, (_, off) in zip(grads, self._slots) if g is not None]
+            grads = [g for g, _ in have]
+            rows = P.kernels.clipped_rows([g.numel() for g in grads], [off for _, off in have], self.flat_param.numel())
+        if not grads:
             self.grad_norm.zero_()
+        elif not P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, grads, rows, self._hyper, self.grad_norm):
+            return False
         self._works = []
         self._launched = [False] * len(self._buckets)
         self._pending = [hi - lo for lo, hi in self._buckets]

@@ -954,9 +954,8 @@ class HipKernels:
             span *= size
         return True
 
-    def _tensor_list(self, what, tensors, rows=None):
-        """-> (device, host rows {address, elements, offset, type} as include/deepipr_hip.h: DeepiprTensor has them).  rows: the rows of
-        float32 tensors with everything but the addresses filled in."""
+    def _tensor_list(self, what, tensors):
+        """-> (device, host rows {address, elements, offset, type} as include/deepipr_hip.h: DeepiprTensor has them)."""
         if not tensors:
             raise RuntimeError('%s: an empty list of tensors' % what)
         devs = set(map(torch.Tensor.get_device, tensors))
@@ -965,17 +964,14 @@ class HipKernels:
                                % (what, sorted({str(t.device) for t in tensors})))
         if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(map(self._dense, tensors)):
             raise RuntimeError('deepipr_amd %s needs dense tensors (no gaps, no element twice)' % what)
-        if rows is None:
-            rows = np.empty((len(tensors), 4), dtype=np.int64)
-            try:
-                rows[:, 3] = [self._DTYPE_CODE[t.dtype] for t in tensors]
-            except KeyError as e:
-                raise RuntimeError('deepipr_amd %s takes float32, bfloat16 and float16 tensors (got %s)' % (what, e)) from None
-            rows[:, 1] = list(map(torch.Tensor.numel, tensors))
-            rows[:, 2] = 0
-        elif {t.dtype for t in tensors} != {torch.float32}:
-            raise RuntimeError('deepipr_amd %s takes float32 tensors' % what)
+        rows = np.empty((len(tensors), 4), dtype=np.int64)
+        try:
+            rows[:, 3] = [self._DTYPE_CODE[t.dtype] for t in tensors]
+        except KeyError as e:
+            raise RuntimeError('deepipr_amd %s takes float32, bfloat16 and float16 tensors (got %s)' % (what, e)) from None
         rows[:, 0] = list(map(torch.Tensor.data_ptr, tensors))
+        rows[:, 1] = list(map(torch.Tensor.numel, tensors))
+        rows[:, 2] = 0
         return tensors[0].device, rows
 
     def _norm_scratch(self, dev):
@@ -1002,24 +998,34 @@ class HipKernels:
                                                     nbytes, _stream(dev)), 'grad_clip')
         return norm
 
-    def sgd_momentum_step_clipped(self, flat_param, flat_buf, grads, offsets, hyper, norm):
-        """SGD on clipped gradients that lie where autograd left them: grads[i] belongs at offsets[i] of the flat buffers; `hyper`
-        = {lr, momentum, weight_decay, grad_scale, max_norm} on the device; the norm of grad_scale * grads goes to `norm`."""
-        dev = _chk(flat_param, flat_buf, hyper, norm)
-        rows = np.empty((len(grads), 4), dtype=np.int64)
-        rows[:, 1] = list(map(torch.Tensor.numel, grads))
+    def clipped_rows(self, numels, offsets, size):
+        """The host rows of sgd_momentum_step_clipped for gradients of `numels` floats that belong at `offsets` of flat buffers of `size`
+        floats, everything but the addresses filled in."""
+        rows = np.empty((len(numels), 4), dtype=np.int64)
+        rows[:, 1] = numels
         rows[:, 2] = offsets
         rows[:, 3] = _lib.F32
-        gdev, rows = self._tensor_list('sgd_momentum_step_clipped', grads, rows)
-        if gdev != dev or hyper.numel() != 5 or flat_buf.numel() != flat_param.numel():
-            raise RuntimeError('sgd_momentum_step_clipped: five hyper-parameters, buffers of one size, all on one device')
-        if rows[:, 2].min() < 0 or (rows[:, 1] + rows[:, 2]).max() > flat_param.numel():
+        if len(rows) and (rows[:, 2].min() < 0 or (rows[:, 1] + rows[:, 2]).max() > size):
             raise RuntimeError('sgd_momentum_step_clipped: a gradient reaches past the flat buffers')
+        return rows
+
+    def sgd_momentum_step_clipped(self, flat_param, flat_buf, grads, rows, hyper, norm):
+        """SGD on clipped gradients that lie where autograd left them, at the places of the flat buffers that `rows` (clipped_rows) gives
+        them; `hyper` = {lr, momentum, weight_decay, grad_scale, max_norm} on the device; the norm of grad_scale * grads goes to `norm`.
+        -> False, and nothing is done, where a gradient is not contiguous float32 on the buffers' device."""
+        dev = _chk(flat_param, flat_buf, hyper, norm)
+        if hyper.numel() != 5 or flat_buf.numel() != flat_param.numel() or len(grads) != len(rows):
+            raise RuntimeError('sgd_momentum_step_clipped: five hyper-parameters, buffers of one size, a row for every gradient')
+        if not all(map(torch.Tensor.is_contiguous, grads)) or {g.dtype for g in grads} != {torch.float32} or \
+                set(map(torch.Tensor.get_device, grads)) != {flat_param.get_device()}:
+            return False
+        rows[:, 0] = list(map(torch.Tensor.data_ptr, grads))
         with _on(dev):
             ws, nbytes = self._norm_scratch(dev)
             _lib.check(_lib.lib().deepipr_sgd_momentum_step_clipped(_p(flat_param), _p(flat_buf), rows.ctypes.data, len(rows),
                                                                     _p(hyper), _p(norm), ws.data_ptr(), nbytes, _stream(dev)),
                        'sgd_momentum_step_clipped')
+        return True
 
     # ---- matrices in 4 bits (include/deepipr_hip.h: deepipr_mx4_*; deepipr_amd/mx4.py is the public face) ----
     def _mx4_chk(self, what, *tensors):
@@ -1114,7 +1120,9 @@ class HipKernels:
         lib = _lib.lib()
         with _on(dev):
             out = torch.empty((m, n), dtype=x.dtype, device=dev)
-            scratch = torch.empty(lib.deepipr_mx4_linear_scratch_bytes(m, n, k, 0), dtype=torch.uint8, device=dev)
+            nbytes = lib.deepipr_mx4_linear_scratch_bytes(m, n, k, 0) if kept is None else \
+                lib.deepipr_mx4_linear_kept_scratch_bytes(xcode, m, n, k)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             saved = None
             if need_dx or need_dw:
                 saved = torch.empty(lib.deepipr_mx4_linear_saved_bytes(m, n, k, need_dx, need_dw), dtype=torch.uint8, device=dev)
@@ -1122,8 +1130,8 @@ class HipKernels:
                 (None, 0, 0, kept[0].data_ptr(), kept[1].data_ptr())
             _lib.check(lib.deepipr_mx4_linear_fwd(
                 x.data_ptr(), xcode, x.stride(0) if m > 1 else k, *wargs, _p(bias), 0 if bias is None else self._mx4_type(what, bias.dtype),
-                m, n, k, need_dx, need_dw, _p(saved), 0 if saved is None else saved.numel(), out.data_ptr(), scratch.data_ptr(),
-                scratch.numel(), _stream(dev)), 'mx4_linear_fwd')
+                m, n, k, need_dx, need_dw, _p(saved), 0 if saved is None else saved.numel(), out.data_ptr(), _p(scratch),
+                nbytes, _stream(dev)), 'mx4_linear_fwd')
         return out, saved
 
     def mx4_linear_bwd(self, dy, saved, k, need_dx, need_dw, dx_type, dw_type, want_db):

@@ -462,7 +462,8 @@ int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const D
  *           reads (the same two flags there).  x and w are read once each.
  *   deepipr_mx4_linear_bwd  dx [M][K] = Q(dy) Q(w) with blocks along N, dw [N][K] = Q(dy)^T Q(x) with blocks along M, dbias [N] the column
  *           sums of dy (not quantised); each may be NULL.  dy is read once.
- *           scratch: deepipr_mx4_linear_scratch_bytes(M, N, K, backward) bytes of this call's own; saved: deepipr_mx4_linear_saved_bytes().
+ *           scratch: deepipr_mx4_linear_scratch_bytes(M, N, K, backward) bytes of this call's own, with w == NULL
+ *           deepipr_mx4_linear_kept_scratch_bytes() (0 where up to 16 rows are quantised inside the product); saved: deepipr_mx4_linear_saved_bytes().
  * There is no counterpart in the reference (its classifiers are nn.Linear in fp32, models/alexnet_passport.py:27-36). */
 size_t deepipr_mx4_code_bytes(long long rows, long long cols);
 size_t deepipr_mx4_scale_bytes(long long rows, long long cols);
@@ -479,6 +480,7 @@ int deepipr_mx4_matmul(const void *a_codes, const void *a_scales, const void *b_
 
 size_t deepipr_mx4_linear_saved_bytes(long long M, long long N, long long K, int need_dx, int need_dw);
 size_t deepipr_mx4_linear_scratch_bytes(long long M, long long N, long long K, int backward);
+size_t deepipr_mx4_linear_kept_scratch_bytes(int x_dtype, long long M, long long N, long long K);
 int deepipr_mx4_linear_fwd(const void *x, int x_dtype, long long x_stride, const void *w, int w_dtype, long long w_stride,
                            const void *w_codes, const void *w_scales, const void *bias, int bias_dtype, long long M, long long N,
                            long long K, int need_dx, int need_dw, void *saved, size_t saved_bytes, void *out, void *scratch,

@@ -22,17 +22,23 @@ class LmKernels(OracleKernels):
             t.mul_(min(1.0, max_norm / (n + 1e-6)))
         return torch.tensor(n)
 
-    def sgd_momentum_step_clipped(self, flat_param, flat_buf, grads, offsets, hyper, norm):
+    def clipped_rows(self, numels, offsets, size):
+        return np.array([[0, n, off, 0] for n, off in zip(numels, offsets)], dtype=np.int64)
+
+    def sgd_momentum_step_clipped(self, flat_param, flat_buf, grads, rows, hyper, norm):
+        if not all(g.is_contiguous() for g in grads):
+            return False
         lr, mu, wd, gs, top = [float(v) for v in hyper.tolist()]
         n = abs(gs) * math.sqrt(sum(float(g.double().square().sum()) for g in grads))
         f = min(1.0, top / (n + 1e-6))
         norm.fill_(n)
         with torch.no_grad():
-            for g, off in zip(grads, offsets):
+            for g, (_, _, off, _) in zip(grads, rows.tolist()):
                 s = slice(off, off + g.numel())
                 d = f * gs * g.reshape(-1) + wd * flat_param[s]
                 flat_buf[s] = mu * flat_buf[s] + d
                 flat_param[s] -= lr * flat_buf[s]
+        return True
 
     def _mx4_chk(self, what, *tensors):
         return torch.device('cpu')

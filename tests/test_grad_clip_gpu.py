@@ -38,7 +38,8 @@ def _check_clipped(got, before, factor):
         assert bool(((t.double() - want).abs() <= tol).all())
 
 
-SIZES = [[1], [7], [64], [65, 1, 0, 3], [4096, 4095, 4097], [1 << 20, 5, 100003], [3] * 191, [1000 + 7 * i for i in range(400)]]
+SIZES = [[1], [7], [64], [65, 1, 0, 3], [4096, 4095, 4097], [1 << 20, 5, 100003], [3] * 191, [1000 + 7 * i for i in range(400)],
+         [8192], [8128, 1], [8192, 1], [100, 1, 1, 1, 1], [90] * 239]                    # around what one workgroup takes; many tiny ones
 
 
 @pytest.mark.parametrize('dtype', TYPES)
@@ -100,6 +101,23 @@ def test_range_of_the_sum_and_values_that_are_not_numbers():
     with pytest.raises(RuntimeError, match='norm is inf'):
         grad_clip.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)
     assert float(p.grad[2]) == 2.0
+
+
+@pytest.mark.parametrize('rest', [0, 30000])                        # one workgroup, several launches
+@pytest.mark.parametrize('dtype', TYPES)
+def test_values_that_are_not_numbers_in_short_and_long_lists(dtype, rest):
+    from deepipr_amd import grad_clip
+    for bad, others in ((math.nan, math.nan), (math.inf, 0.0), (-math.inf, 0.0)):
+        for kind in (2.0, 1.0, math.inf):
+            ts = [torch.ones(5, dtype=dtype, device=DEV), torch.tensor([1.0, bad], dtype=dtype, device=DEV)]
+            ts += [torch.ones(rest, dtype=dtype, device=DEV)] if rest else []
+            n = float(grad_clip.clip_grads_(ts, 1.0, kind))
+            assert math.isnan(n) if math.isnan(bad) else n == math.inf
+            assert bool(ts[1].isnan()[1]) and all(bool(t.isnan().all() if math.isnan(others) else (t == 0).all()) for t in (ts[0], ts[-1]) if t is not ts[1])
+    low = torch.full((max(rest, 6),), torch.finfo(dtype).min, dtype=dtype, device=DEV)      # the type's lowest value
+    n = grad_clip.grad_norm([low], 1.0)
+    want = low.double().abs().sum().item()
+    assert float(n) == math.inf if want > 3.5e38 else abs(float(n) - want) <= want * 2 ** -23
 
 
 def test_refusals_and_orders_of_dimensions():

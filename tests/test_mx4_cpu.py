@@ -54,6 +54,10 @@ def test_linear_entries_refuse_before_any_launch():
                 dict(dwt=3), dict(db=p + 2), dict(dx=None, dw=None, db=None), dict(scratch=None), dict(cb=3)):
         assert bwd(**bad) == -1 and b'mx4_linear_bwd' in lib.deepipr_last_error(), bad
     assert lib.deepipr_mx4_linear_saved_bytes(5, 6, 70, 0, 0) == 0 and lib.deepipr_mx4_linear_scratch_bytes(0, 6, 70, 0) == 0
+    # kept weights: none for rows that their product quantises (up to 4096 bytes x blocks), no room for the weight's codes otherwise
+    assert lib.deepipr_mx4_linear_kept_scratch_bytes(0, 1, 6, 9216) == lib.deepipr_mx4_linear_kept_scratch_bytes(1, 16, 6, 4096) == 0
+    assert 0 < lib.deepipr_mx4_linear_kept_scratch_bytes(0, 16, 600, 4096) < lib.deepipr_mx4_linear_scratch_bytes(16, 600, 4096, 0)
+    assert fwd(w=None, wc=p, wsc=p, dx=0, dw=0, m=17, cb=1) == -1 and b'scratch' in lib.deepipr_last_error()
     assert lib.deepipr_mx4_linear_saved_bytes(5, 6, 70, 1, 1) == 2 * lib.deepipr_mx4_linear_saved_bytes(5, 6, 70, 1, 0)
     assert lib.deepipr_mx4_matmul_workspace_bytes(128, 128, 20000) > 0 == lib.deepipr_mx4_matmul_workspace_bytes(64, 128, 20000)
 
