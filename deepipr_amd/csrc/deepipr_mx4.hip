@@ -193,28 +193,46 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const Matrix A, const
         for (int j = 0; j < 32; ++j) e[j] = 2 * j < left ? load1<T>(x, (r0 + h + 2 * j) * stride + c0 + c) : 0.0f;
 #pragma unroll
         for (int j = 0; j < 32; ++j) s[(h + 2 * j) * kQP + c] = e[j];
+    } else if (r0 + kQR <= R && c0 + kQC <= C) {
+        // rows of 16-bit elements off the grid: eight of them out of the two aligned pieces that hold them (200 704 x 1021 bf16 124 us, 151 by
+        // aligned words).  Both pieces hold an element of the row: nothing outside its last aligned piece is read.
+        u32x4 lo[LOADS], hi[LOADS];
+        const auto at = [&](int j) {
+            const int i = j * kThreads + tid;
+            return static_cast<const char *>(x) + ((r0 + i / PER) * stride + c0 + i % PER * V) * 2;
+        };
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int by = static_cast<int>(reinterpret_cast<uintptr_t>(at(j)) & 15);        // (pointers stay pointers: global loads)
+            lo[j] = *reinterpret_cast<const u32x4 *>(at(j) - by);
+            hi[j] = *reinterpret_cast<const u32x4 *>(at(j) + (by ? 16 - by : 0));
+        }
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int by = static_cast<int>(reinterpret_cast<uintptr_t>(at(j)) >> 1 & 7);   // elements
+            u32x4 l = lo[j], h = hi[j];
+            if (by & 2) l = u32x4{l.y, l.z, l.w, h.x}, h = u32x4{h.y, h.z, h.w, h.w};
+            if (by & 4) l = u32x4{l.z, l.w, h.x, h.y}, h.x = h.z;
+            if (by & 1) l = u32x4{l.x >> 16 | l.y << 16, l.y >> 16 | l.z << 16, l.z >> 16 | l.w << 16, l.w >> 16 | h.x << 16};
+            put(j * kThreads + tid, l);
+        }
     } else {
-        // the same for 16-bit elements, two to an aligned word (loads of single ones are four times slower); a row that starts in the middle
+        // the last rows and columns, two elements to an aligned word (loads of single ones are four times slower); a row that starts in the middle
         // of a word is off by one: its first and last words hold one element of it, and what else they hold is not used
         const int lane = tid & 63, row0 = (tid >> 6) * 16;
-        const auto row_at = [&](int r) { return reinterpret_cast<uintptr_t>(x) + static_cast<uintptr_t>(((r0 + r) * stride + c0) * 2); };
+        const auto row_at = [&](int r) { return static_cast<const char *>(x) + ((r0 + r) * stride + c0) * 2; };
+        const auto odd_at = [&](int r) { return static_cast<int>(reinterpret_cast<uintptr_t>(row_at(r)) >> 1 & 1); };
         const auto value = [&](unsigned h) { return T == BF16 ? bf16_to_f32(h) : f16_to_f32(h); };
         unsigned w[16];
-        if (r0 + kQR <= R && c0 + kQC <= C) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = *reinterpret_cast<const unsigned *>((row_at(row0 + j) & ~uintptr_t(3)) + 4 * lane);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const uintptr_t at = row_at(row0 + j);
-                const int odd = static_cast<int>(at >> 1 & 1);
-                w[j] = r0 + row0 + j < R && c0 + 2 * lane - odd < C ? *reinterpret_cast<const unsigned *>(at - 2 * odd + 4 * lane) : 0u;
-                if (c0 + 2 * lane - odd + 1 >= C) w[j] &= 0xffffu;
-            }
+        for (int j = 0; j < 16; ++j) {
+            const int odd = odd_at(row0 + j);
+            w[j] = r0 + row0 + j < R && c0 + 2 * lane - odd < C ? *reinterpret_cast<const unsigned *>(row_at(row0 + j) - 2 * odd + 4 * lane) : 0u;
+            if (c0 + 2 * lane - odd + 1 >= C) w[j] &= 0xffffu;
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const int odd = static_cast<int>(row_at(row0 + j) >> 1 & 1);
+            const int odd = odd_at(row0 + j);
             float *d = s + (row0 + j) * kQP + 2 * lane - odd;
             if (odd == 0) {
                 *reinterpret_cast<f32x2 *>(d) = f32x2{value(w[j] & 0xffffu), value(w[j] >> 16)};
@@ -223,7 +241,7 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const Matrix A, const
                 d[1] = value(w[j] >> 16);
             }
         }
-        if (tid < kQR && (row_at(tid) >> 1 & 1))                         // the 128th column of a row that is off by one
+        if (tid < kQR && odd_at(tid))                         // the 128th column of a row that is off by one
             s[tid * kQP + 127] = r0 + tid < R && c0 + 127 < C ? load1<T>(x, (r0 + tid) * stride + c0 + 127) : 0.0f;
     }
     __syncthreads();

@@ -34,9 +34,9 @@ def _max_norm(max_norm):
 
 def _as_list(tensors):
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    for t in tensors:
-        if t.layout is not torch.strided:
-            raise RuntimeError('deepipr_amd gradient norms take dense tensors (got layout %s)' % t.layout)
+    layouts = {t.layout for t in tensors} - {torch.strided}
+    if layouts:
+        raise RuntimeError('deepipr_amd gradient norms take dense tensors (got layout %s)' % layouts.pop())
     return tensors
 
 
@@ -57,7 +57,9 @@ def clip_grads_(tensors, max_norm, norm_type=2.0):
     if not tensors:
         return torch.zeros(())
     norm = P.kernels.grad_clip(tensors, max_norm, code)
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    if any(map(torch.Tensor.is_inference, tensors)):
+        tensors = [t for t in tensors if not t.is_inference()]
+    torch.autograd.graph.increment_version(tensors)
     return norm
 
 

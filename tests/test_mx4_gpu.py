@@ -12,7 +12,7 @@ from tests import mx4_oracle as oracle
 pytestmark = pytest.mark.gpu
 DEV = 'cuda:0'
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
-SHAPES = [(1, 1), (1, 32), (3, 33), (33, 3), (64, 128), (65, 129), (63, 127), (200, 300), (1, 9216), (130, 31), (257, 1000), (1000, 96)]
+SHAPES = [(1, 1), (1, 32), (3, 33), (33, 3), (64, 128), (65, 129), (63, 127), (200, 300), (1, 9216), (130, 31), (257, 1000), (1000, 96), (192, 261), (130, 391)]
 
 
 def _random(shape, dtype, seed, spread=True):
