@@ -871,11 +871,13 @@ template <int T> void launch_quantise(DiprProf &prof, const Matrix &m, const Mat
 }
 
 // ---- which kernels a product takes
-// Estimated from measured times (ns): a step of 128 columns costs a 256 x 256 tile 780, a 128 x 128 tile 270 where it has the CU for itself
-// and 690 where two share it, a 64 x 64 tile 140 (160 where several follow on a CU) and a 64 x 32 tile 100 (130); begin and end of a tile
-// 6 000 / 4 500 / 3 500 / 3 000; a second launch that adds up partial sums 4 000 and their bytes at 4 TB/s.  Measured (us): 8192^3 253 large, 355 small; 4096 x 4096 x 8200 65 / 78; 2048^3 18.3 / 10.1; 253 x 4096 x 9216 52 large, 24.5
-// small, 20.9 small with the columns in three; 512 x 512 x 16384 34.8 whole, 15.5 in eight; 1000^3 8.2 whole, 13 in two; 32 x 4096 x 9216 8.2
-// by the kernel for few rows, 12.1 at best by the others.
+// Estimated from measured times (ns).  A round of workgroups over the CUs costs its begin and end and its steps of 128 columns:
+//   256 x 256 tiles 10 000 + 860 a step; 128 x 128 tiles, up to two on a CU, 6 500 + 200 (on half the CUs), 270 (one a CU) or 690 a step; 64 x 64 tiles 1 500 and
+//   2 300 + 140 a step for each round; 64 x 32 tiles 2 000 and 1 000 + 100; 64 rows x 16 columns 2 200 and 700 + 85; a second launch that adds up
+//   partial sums 4 000 and their bytes at 4 TB/s.
+// Measured (us): 8192^3 251 large, 355 small; 4096 x 4096 x 8200 65 / 78; 2048^3 18.4 / 10.0, 64 x 32 19.5; 512 x 512 x 16384 34.8 small, 15.5 with
+// the columns in eight, 64 x 32 15.0; 64 x 8192 x 8192 14.0 by 16 columns, 64 x 32 10.0, 64 x 64 12.2; 64 x 4096 x 9216 8.6 / 9.4 / 11.9;
+// 8192 x 300 x 300 7.6 small, 64 x 32 9.2, 64 x 64 10.4; 4096 x 512 x 4096 12.7, 23.1, 17.5.
 struct Plan {
     enum { kRows, k64x32, k64x64, kSmall, kLarge } form;
     int splits;                  // kSmall only
@@ -888,32 +890,34 @@ inline int cu_count() {
 }
 inline double large_ns(long long m, long long n, long long kt) {
     const long long rounds = (tiles_of(m, n, 256) + cu_count() - 1) / cu_count();
-    return static_cast<double>(rounds) * (780.0 * kt + 6000.0);
+    return static_cast<double>(rounds) * (860.0 * kt + 10000.0);
 }
 inline double small_ns(long long m, long long n, long long kt, int splits) {
     const double slots = 2.0 * cu_count(), tiles = static_cast<double>(tiles_of(m, n, 128)) * splits;
-    const double step = tiles <= slots / 2 ? 270.0 : 690.0 * (tiles > slots ? tiles / slots : 1.0);
+    const double step = tiles <= slots / 4 ? 200.0 : tiles <= slots / 2 ? 270.0 : 690.0 * (tiles > slots ? tiles / slots : 1.0);
     const double sums = splits > 1 ? 4000.0 + static_cast<double>(splits) * m * n * 8 / 4000.0 : 0.0;
-    return step * static_cast<double>((kt + splits - 1) / splits) + 4500.0 + sums;
+    return step * static_cast<double>((kt + splits - 1) / splits) + 6500.0 + sums;
 }
 inline long long strips_of(long long m, long long n, int nt) { return ((m + 63) / 64) * ((n + 16 * nt - 1) / (16 * nt)); }
 inline double strip_ns(long long m, long long n, long long kt, int nt) {
-    const long long rounds = (strips_of(m, n, nt) + cu_count() - 1) / cu_count();
-    const double step = nt == 2 ? (rounds > 1 ? 130.0 : 100.0) : (rounds > 1 ? 160.0 : 140.0);
-    return step * static_cast<double>(rounds) * static_cast<double>(kt) + (nt == 2 ? 3000.0 : 3500.0);
+    const double rounds = static_cast<double>((strips_of(m, n, nt) + cu_count() - 1) / cu_count()), steps = static_cast<double>(kt);
+    return nt == 1 ? 2200.0 + rounds * (700.0 + 85.0 * steps) : nt == 2 ? 2000.0 + rounds * (1000.0 + 100.0 * steps) : 1500.0 + rounds * (2300.0 + 140.0 * steps);
 }
 Plan plan(long long M, long long N, long long kt) {
     Plan p = {Plan::kRows, 1, 0};
-    if (M <= 64) return p;
-    p.form = Plan::kLarge;
-    double best = large_ns(M, N, kt);
+    if (M <= 32) return p;
+    double best = strip_ns(M, N, kt, 1);
+    if (M > 64) {
+        p.form = Plan::kLarge;
+        best = large_ns(M, N, kt);
+    }
     // a few rows behind whole tiles: a tile row of their own could cost a round
     const long long tail = M % 256 <= 64 && M > 256 ? M % 256 : 0;
     if (tail) {
         const double t = large_ns(M - tail, N, kt) + 5000.0 + static_cast<double>(N * kt) / 80.0;
         if (t < best) best = t, p.tail = tail;
     }
-    for (int splits = 1; splits <= 16 && splits <= kt; splits += splits < 4 ? 1 : splits / 2) {
+    for (int splits = 1; M > 64 && splits <= 16 && splits <= kt; splits += splits < 4 ? 1 : splits / 2) {
         if (splits > 1 && tiles_of(M, N, 128) * splits > 4 * cu_count()) break;
         const double t = small_ns(M, N, kt, splits);
         if (t < best) {

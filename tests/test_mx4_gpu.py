@@ -163,6 +163,7 @@ def test_products_are_exact(mnk, dtype):
 
 @pytest.mark.parametrize('mnk', [(64, 4200, 1200), (65, 300, 9000), (128, 128, 20000), (4104, 4096, 130), (4160, 4000, 300), (4352, 4100, 250),
                                  (2500, 3000, 700), (4104, 4096, 4100), (2300, 3900, 5000), (300, 100, 20000), (512, 4000, 2050),
+                                 (4000, 4001, 4100), (64, 9216, 4096), (48, 4096, 4096), (33, 70, 9000),
                                  (100, 500, 3000), (100, 500, 3100), (70, 30, 3900), (190, 490, 4200), (130, 510, 6300), (65, 33, 8200),
                                  (250, 4000, 3000), (250, 4001, 3100), (253, 3999, 3900), (200, 3900, 4200), (256, 4090, 6300), (129, 4050, 8200)])
 def test_products_of_every_form_are_exact(mnk):
@@ -220,6 +221,22 @@ def test_linear_and_its_gradients(mnk, dtype):
     y2 = mx4.linear(x, w)
     dx2, = torch.autograd.grad(y2, x, dy)
     assert torch.equal(dx2, dx)
+
+
+@pytest.mark.parametrize('mnk', [(40, 100, 200), (300, 2000, 1500), (512, 512, 4000), (600, 1000, 3000), (4104, 4096, 4096)])
+def test_gradients_are_the_products_of_their_parts(mnk):
+    """Two products in one launch give what each gives alone, in every form that they share."""
+    from deepipr_amd import mx4
+    m, n, k = mnk
+    g = torch.Generator(device=DEV).manual_seed(m)
+    x, w, dy = (torch.randn(s, generator=g, device=DEV).bfloat16() for s in ((m, k), (n, k), (m, n)))
+    x.requires_grad_(), w.requires_grad_()
+    y = mx4.linear(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x, w = x.detach(), w.detach()
+    assert torch.equal(y, mx4.matmul(mx4.quantize(x, 1), mx4.quantize(w, 1), dtype=x.dtype))
+    assert torch.equal(dx, mx4.matmul(mx4.quantize(dy, 1), mx4.quantize(w, 0), dtype=x.dtype))
+    assert torch.equal(dw, mx4.matmul(mx4.quantize(dy, 0), mx4.quantize(x, 0), dtype=x.dtype))
 
 
 @pytest.mark.parametrize('dtype', TYPES)
