@@ -882,6 +882,7 @@ struct Plan {
     enum { kRows, k64x32, k64x64, kSmall, kLarge } form;
     int splits;                  // kSmall only
     long long tail;              // kLarge only: rows at the end that go to the kernel for few rows (0: none)
+    bool strips() const { return form == k64x32 || form == k64x64; }
 };
 inline long long tiles_of(long long m, long long n, int side) { return ((m + side - 1) / side) * ((n + side - 1) / side); }
 inline int cu_count() {
@@ -952,8 +953,11 @@ template <int T> void launch_product(DiprProf &prof, Product P, const Product *o
     const dim3 block(kThreads);
     const Plan p = plan(P.M, P.N, P.kt);
     if (p.form == Plan::kRows) return launch_rows<T>(prof, P, st);
-    if (p.form == Plan::k64x32 || p.form == Plan::k64x64) {
-        const int nt = p.form == Plan::k64x32 ? 2 : 4;
+    if (p.strips()) {
+        int nt = p.form == Plan::k64x32 ? 2 : 4;
+        if (other)                                       // one width for both
+            nt = strip_ns(P.M, P.N, P.kt, 2) + strip_ns(other->M, other->N, other->kt, 2) <=
+                         strip_ns(P.M, P.N, P.kt, 4) + strip_ns(other->M, other->N, other->kt, 4) ? 2 : 4;
         const unsigned first = static_cast<unsigned>(strips_of(P.M, P.N, nt));
         const dim3 grid(first + (other ? static_cast<unsigned>(strips_of(other->M, other->N, nt)) : 0u)), wide(512);
         const Product &Q = other ? *other : P;
@@ -1068,6 +1072,7 @@ Product product_of(const void *a, const void *sa, const void *b, const void *sb,
 // Whether two products of one output type can share a launch
 bool alike(const Product &p, const Product &q) {
     const Plan a = plan(p.M, p.N, p.kt), b = plan(q.M, q.N, q.kt);
+    if (a.strips() && b.strips()) return true;
     return a.form == b.form && a.form != Plan::kRows && a.splits == 1 && b.splits == 1 &&
            tiles_of(p.M, p.N, 128) + tiles_of(q.M, q.N, 128) <= kMaxGrid;
 }
