@@ -293,10 +293,11 @@ class FlatSGD(torch.optim.Optimizer):
     def _on_grad(self, param):
         if self._paused or self._mode != 'hooks':
             return
-        b = self._bucket_of[id(param)]
-        self._pending[b] -= 1
-        if self._pending[b] == 0 and not self._launched[b]:
-            self._launch(b, async_op=True)           # overlaps with the rest of backward
+        self._pending[self._bucket_of[id(param)]] -= 1
+        # In the buckets' own order, as step() sends the rest: a bucket that stays incomplete on this rank only (a parameter without a
+        # gradient) holds back the ones behind it, or the ranks' collectives would meet in different orders.
+        while False in self._launched[:-1] and self._pending[self._launched.index(False)] <= 0:
+            self._launch(self._launched.index(False), async_op=True)           # overlaps with the rest of backward
 
     # ------------------------------------------------------------------ optimiser interface
     def sync_hyper(self):
