@@ -28,6 +28,10 @@ from deepipr_amd import passport_ops as P
 _ALIGN = 64            # floats: every parameter starts on a 256-byte boundary of the flat buffer
 
 
+def _pad(n):
+    return (n + _ALIGN - 1) // _ALIGN * _ALIGN
+
+
 class FlatSGD(torch.optim.Optimizer):
     def __init__(self, params, lr=0.01, momentum=0.9, weight_decay=1e-4, bucket_fractions=(0.45, 0.8, 0.95),
                  process_group=None, max_grad_norm=None):
@@ -69,10 +73,14 @@ class FlatSGD(torch.optim.Optimizer):
             offsets.append(total)
             total += (p.numel() + _ALIGN - 1) // _ALIGN * _ALIGN
         self.flat_param = torch.zeros(total, dtype=torch.float32, device=dev)
-        self.flat_grad = torch.zeros(total, dtype=torch.float32, device=dev)
+        # With an exchange the gradient buffer ends in one float per parameter, 1 where this rank has its gradient: they travel with the
+        # last bucket, and every rank learns which parameters have a gradient on ANY rank (_missing_everywhere).
+        self._flags = total
+        self.flat_grad = torch.zeros(total + (_pad(len(order)) if self.comm else 0), dtype=torch.float32, device=dev)
         self.flat_buf = torch.zeros(total, dtype=torch.float32, device=dev)
         self._slots = []
         self._zero_pool = torch.zeros(_ALIGN, dtype=torch.float32, device=dev)
+        self._ones = torch.ones(len(order) if self.comm else 0, dtype=torch.float32, device=dev)
         # {lr, momentum, weight_decay, 1/world} live in device memory and the update kernel reads them there: a step
         # captured into a hipGraph (launch arguments frozen at capture) then still follows an lr schedule --
         # sync_hyper() rewrites the four floats whenever param_groups changed (GraphedTrainStep calls it before
@@ -139,8 +147,13 @@ class FlatSGD(torch.optim.Optimizer):
         lo, hi = self._buckets[b]
         start = self._slots[lo][1]
         last_p, last_off = self._slots[hi - 1]
-        end = last_off + (last_p.numel() + _ALIGN - 1) // _ALIGN * _ALIGN
-        return start, end
+        return start, last_off + _pad(last_p.numel())
+
+    def _message(self, lo, hi):
+        """The part of flat_grad that carries the slots lo..hi-1 (the last ones bring the flags)."""
+        last_p, last_off = self._slots[hi - 1]
+        end = self.flat_grad.numel() if hi == len(self._slots) else last_off + _pad(last_p.numel())
+        return self.flat_grad[self._slots[lo][1]:end]
 
     def _pack(self, b):
         """Gradients of bucket b -> their slots of flat_grad with ONE cat kernel (alignment pads and parameters
@@ -149,20 +162,23 @@ class FlatSGD(torch.optim.Optimizer):
         self._pack_slots(lo, hi)
 
     def _pack_slots(self, lo, hi):
-        start = self._slots[lo][1]
-        last_p, last_off = self._slots[hi - 1]
-        end = last_off + (last_p.numel() + _ALIGN - 1) // _ALIGN * _ALIGN
         pieces = []
         for p, off in self._slots[lo:hi]:
             n = p.numel()
-            pad = (n + _ALIGN - 1) // _ALIGN * _ALIGN - n
+            pad = _pad(n) - n
             if p.grad is None:
                 pieces.append(self._zeros(n + pad))
                 continue
             pieces.append(p.grad.reshape(-1))
             if pad:
                 pieces.append(self._zeros(pad))
-        torch.cat(pieces, out=self.flat_grad[start:end])
+        if self.comm and hi == len(self._slots):
+            at = 0
+            for i in self._missing_grads() + [len(self._slots)]:
+                pieces += [self._ones[:i - at], self._zeros(1)]
+                at = i + 1
+            pieces[-1] = self._zeros(self.flat_grad.numel() - self._flags - len(self._slots))
+        torch.cat(pieces, out=self._message(lo, hi))
 
     def _zeros(self, n):
         if self._zero_pool.numel() < n:
@@ -173,8 +189,7 @@ class FlatSGD(torch.optim.Optimizer):
         self._pack(b)
         self._launched[b] = True
         if self.comm:
-            start, end = self._range(b)
-            w = dist.all_reduce(self.flat_grad[start:end], op=dist.ReduceOp.SUM, group=self.group, async_op=async_op)
+            w = dist.all_reduce(self._message(*self._buckets[b]), op=dist.ReduceOp.SUM, group=self.group, async_op=async_op)
             if async_op:
                 self._works.append(w)
 
@@ -249,8 +264,7 @@ class FlatSGD(torch.optim.Optimizer):
         if lo >= hi:
             return
         cuda = self.flat_grad.is_cuda
-        start = self._slots[self._buckets[lo][0]][1]
-        end = self._range(hi - 1)[1]
+        slots = self._buckets[lo][0], self._buckets[hi - 1][1]
 
         def go():
             # pack (unless the stage's graph did it) + all-reduce as ORDINARY (async_op=False) operations of whichever
@@ -260,9 +274,9 @@ class FlatSGD(torch.optim.Optimizer):
             # profiles/r03_probe2.json); for the overlapped buckets the async form measured slower as well
             # (profiles/r03_ddp_rehearsal_async_buckets.jsonl).
             if not packed:
-                self._pack_slots(self._buckets[lo][0], self._buckets[hi - 1][1])
+                self._pack_slots(*slots)
             if self.comm:
-                dist.all_reduce(self.flat_grad[start:end], op=dist.ReduceOp.SUM, group=self.group)
+                dist.all_reduce(self._message(*slots), op=dist.ReduceOp.SUM, group=self.group)
         if cuda and overlap:
             if self._side is None:
                 self._side = torch.cuda.Stream(device=self.flat_grad.device)
@@ -319,6 +333,18 @@ class FlatSGD(torch.optim.Optimizer):
     def _missing_grads(self):
         return [i for i, (p, _) in enumerate(self._slots) if p.grad is None]
 
+    def _missing_everywhere(self, missing):
+        """Behind the exchange: the parameters that no rank has a gradient for -- the same list on every rank, so that all update the same
+        parameters by the same norm.  A rank that misses none knows that there are none; the others read the flags (a host read, on the
+        rare path of unused branches only)."""
+        if not self.comm or not missing:
+            return missing
+        if self.flat_param.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('FlatSGD: a step with several ranks in which a parameter has no gradient cannot be captured (it reads what the '
+                               'other ranks have)')
+        have = self.flat_grad[self._flags:].tolist()
+        return [i for i in missing if have[i] == 0.0]
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -364,18 +390,20 @@ class FlatSGD(torch.optim.Optimizer):
                     self._launch(b, async_op=False)
             for w in self._works:
                 w.wait()
+        missing = self._missing_everywhere(missing)
+        flat_grad = self.flat_grad[:self._flags]
         if self._clips:
-            # the same rule for every rank: norm and factor come from the exchanged sum (parameters without a gradient stay out)
+            # norm and factor come from the exchanged sum, the same list on every rank (parameters without a gradient on any stay out)
             skip = set(missing)
-            have = [(self.flat_grad[off:off + p.numel()], off) for i, (p, off) in enumerate(self._slots) if i not in skip] \
-                if missing else [(self.flat_grad, 0)]
+            have = [(flat_grad[off:off + p.numel()], off) for i, (p, off) in enumerate(self._slots) if i not in skip] \
+                if missing else [(flat_grad, 0)]
             if have:
                 rows = P.kernels.clipped_rows([g.numel() for g, _ in have], [o for _, o in have], self.flat_param.numel())
                 P.kernels.sgd_momentum_step_clipped(self.flat_param, self.flat_buf, [g for g, _ in have], rows, self._hyper, self.grad_norm)
             else:
                 self.grad_norm.zero_()
         elif not missing:
-            P.kernels.sgd_momentum_step_dev(self.flat_param, self.flat_grad, self.flat_buf, self._hyper)
+            P.kernels.sgd_momentum_step_dev(self.flat_param, flat_grad, self.flat_buf, self._hyper)
         else:
             # torch.optim.SGD skips parameters whose grad is None (no weight decay, no momentum update): update the
             # runs of slots that did receive a gradient, one launch per run (rare path: unused branches)
@@ -391,7 +419,7 @@ class FlatSGD(torch.optim.Optimizer):
                 lo = self._slots[i][1]
                 last_p, last_off = self._slots[j]
                 hi = last_off + (last_p.numel() + _ALIGN - 1) // _ALIGN * _ALIGN
-                P.kernels.sgd_momentum_step_dev(self.flat_param[lo:hi], self.flat_grad[lo:hi], self.flat_buf[lo:hi],
+                P.kernels.sgd_momentum_step_dev(self.flat_param[lo:hi], flat_grad[lo:hi], self.flat_buf[lo:hi],
                                                 self._hyper)
                 i = j + 1
         self._works = []
