@@ -18,6 +18,7 @@ import torch
 import torch.distributed as dist
 
 from deepipr_amd.models._builders import PASSPORT_TYPES
+from deepipr_amd.models.layers.linear import weights_written
 
 BUCKET_MB = 16
 
@@ -65,6 +66,7 @@ def broadcast_state(model, src=0):
     for m in model.modules():
         if isinstance(m, PASSPORT_TYPES):
             m.invalidate_key_cache()
+    weights_written(model.parameters())
 
 
 def replicate(model, device, bucket_mb=BUCKET_MB, static_graph=True):

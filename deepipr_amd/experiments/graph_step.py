@@ -12,6 +12,8 @@ key means are cached outside the graph); in-situ kernel timing (deepipr_profile_
 """
 import torch
 
+from deepipr_amd.models.layers.linear import weights_written
+
 
 class _NoStep:
     """Optimizer proxy handed to step_fn while capturing in 'fwd_bwd' mode: zero_grad is recorded, step() is not."""
@@ -122,7 +124,9 @@ class GraphedTrainStep:
         self.static_data.copy_(data, non_blocking=True)
         self.static_target.copy_(target, non_blocking=True)
         self.graph.replay()
-        if not self.optimizer_in_graph:
+        if self.optimizer_in_graph:
+            weights_written(p for p, g in self._captured_grads if g is not None)
+        else:
             for p, g in self._captured_grads:
                 p.grad = g
             self.optimizer.step()

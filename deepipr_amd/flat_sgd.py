@@ -24,6 +24,7 @@ import torch
 import torch.distributed as dist
 
 from deepipr_amd import passport_ops as P
+from deepipr_amd.models.layers.linear import weights_written
 
 _ALIGN = 64            # floats: every parameter starts on a 256-byte boundary of the flat buffer
 
@@ -343,6 +344,7 @@ class FlatSGD(torch.optim.Optimizer):
             raise RuntimeError('FlatSGD: a step with several ranks in which a parameter has no gradient cannot be captured (it reads what the '
                                'other ranks have)')
         have = self.flat_grad[self._flags:].tolist()
+        weights_written(self._slots[i][0] for i in missing if have[i])         # (those with a gradient of their own: step()'s hooks)
         return [i for i in missing if have[i] == 0.0]
 
     @torch.no_grad()

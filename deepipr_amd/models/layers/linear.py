@@ -1,9 +1,28 @@
 """A linear layer whose products run in 4 bits (deepipr_amd.mx4): what the classifiers' nn.Linear (models/alexnet_passport.py:27-36,
 models/resnet_passport.py:127-129) becomes under `--linear-format mx4`."""
+import weakref
+
 import torch
 import torch.nn as nn
+from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from deepipr_amd import mx4
+
+_kept = weakref.WeakSet()          # the layers that hold codes of their weight
+_hook = None
+
+
+def weights_written(params):
+    """For code that writes parameters where autograd does not see it (kernels that take addresses, replayed graphs, collectives): a layer
+    that keeps codes of one of `params` refuses to answer from them."""
+    if _kept:
+        ids = set(map(id, params))
+        torch.autograd.graph.increment_version([m.weight for m in _kept if id(m.weight) in ids])
+
+
+def _stepped(optimizer, args, kwargs):
+    if _kept:
+        weights_written(p for g in optimizer.param_groups for p in g['params'] if p.grad is not None)
 
 
 class Mx4Linear(nn.Linear):
@@ -11,7 +30,8 @@ class Mx4Linear(nn.Linear):
     (mx4.linear: output, dx and dw in 4 bits, dbias exact).  A net that only answers can `keep()` its weight in 4 bits instead of
     quantising it per call; the kept codes are buffers outside the state_dict and are dropped by train(), load_state_dict(), release(),
     by a new `weight` and in copies of the layer.  A kept weight has no backward pass, and changing `weight` in place without a new
-    keep() is an error (what autograd does not see, a write through `weight.data`, needs a keep() of its own)."""
+    keep() is an error, also where an optimiser or the framework's replayed train step does it (what neither autograd nor the framework sees,
+    a write through `weight.data` or by a graph that a program captured itself, needs a keep() of its own)."""
 
     def __init__(self, in_features, out_features, bias=True, device=None, dtype=None):
         super().__init__(in_features, out_features, bias, device, dtype)
@@ -30,12 +50,17 @@ class Mx4Linear(nn.Linear):
         return linear
 
     def keep(self):
+        global _hook
         q = mx4.quantize(self.weight.detach())
         self.kept_codes, self.kept_scales, self._kept_version = q.codes, q.scales, self.weight._version
+        _kept.add(self)
+        if _hook is None:                                    # fused optimisers write without raising a version
+            _hook = register_optimizer_step_post_hook(_stepped)
         return self.eval()
 
     def release(self):
         self.kept_codes = self.kept_scales = self._kept_version = None
+        _kept.discard(self)
         return self
 
     def register_parameter(self, name, param):               # (also what `layer.weight = ...` calls)

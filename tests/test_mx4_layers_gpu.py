@@ -141,3 +141,32 @@ def test_work_on_a_side_stream():
             y, n = mx4.linear(a, b), grad_clip.grad_norm([a, b])
             assert torch.equal(y, want) and torch.equal(n, norm)
     torch.cuda.synchronize()
+
+
+def _flat_net():
+    from deepipr_amd.models.layers.linear import Mx4Linear
+    torch.manual_seed(2)
+    return nn.Sequential(nn.Flatten(), Mx4Linear(3 * 8 * 8, 64), nn.ReLU(), Mx4Linear(64, 10)).to(DEV)
+
+
+@pytest.mark.parametrize('fused', [False, True])
+def test_a_replayed_step_ends_the_kept_codes(fused):
+    """A layer that is kept between the replays of a train step: the replay runs no Python of the layer or of the optimiser."""
+    from deepipr_amd.experiments.graph_step import GraphedTrainStep
+    from deepipr_amd.experiments.trainer import train_step_v1
+    from deepipr_amd.flat_sgd import FlatSGD
+    net = _flat_net()
+    opt = torch.optim.SGD(net.parameters(), lr=0.1, fused=True) if fused else FlatSGD(net.parameters(), lr=0.1)
+    x, t = _batches(1, size=8)[0]
+    step = GraphedTrainStep(train_step_v1, net, opt, x, t, warmup=0)
+    step(x, t)
+    with torch.no_grad():
+        lin = net[3].keep()
+        feats = torch.randn(4, 64, device=DEV)
+        lin(feats)
+        before = lin.weight.clone()
+        step(x, t)
+        torch.cuda.synchronize()
+        assert not torch.equal(lin.weight, before)
+        with pytest.raises(RuntimeError, match='keep'):
+            lin(feats)
