@@ -142,7 +142,9 @@ class GraphedEval:
     (`lambda d: model(d, ind=1)` for the private branch).  A graph is keyed on the batch shape (the ragged last batch gets
     its own; at most `max_graphs`, then eager) and stays valid while the things whose ADDRESSES it froze stay put: the
     parameters / buffers (updated in place by training) and every passport layer's pooled key means (passport_ops.PooledKeys:
-    a key that was replaced or stepped on yields a new tensor -- seen here before every replay, the shape is captured again).
+    a key that was replaced or stepped on yields a new tensor -- seen here before every replay, the shape is captured again).  A weight
+    that a layer keeps in 4 bits (Mx4Linear.keep) is no address of the graph: a change of it is seen the same way, and the capture's
+    eager pass then raises as the layer does.
     Returns (top-1 class [N, 1], summed loss, hits): the graph's own output tensors, overwritten by the next call."""
 
     def __init__(self, model, forward=None, max_graphs=4):
@@ -155,10 +157,13 @@ class GraphedEval:
 
     def _signature(self):
         from deepipr_amd.models.layers._passport_base import PassportLayerBase
+        from deepipr_amd.models.layers.linear import Mx4Linear
         sig = []
         for m in self.model.modules():
             if isinstance(m, PassportLayerBase) and m.get_bias_key() is not None and m.get_scale_key() is not None:
                 sig.append(id(m._pooled_means()[2]))
+            elif isinstance(m, Mx4Linear) and m.kept_codes is not None:
+                sig.append((m.weight._version, m._kept_version))
         sig.extend(t.data_ptr() for t in self.model.parameters())
         sig.extend(t.data_ptr() for t in self.model.buffers())
         return tuple(sig)

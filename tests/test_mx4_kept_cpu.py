@@ -105,3 +105,23 @@ def test_weights_of_another_rank_end_the_kept_codes(tmp_path):
     out = str(tmp_path / 'r')
     torch.multiprocessing.spawn(_worker, args=(_free_port(), out), nprocs=2, join=True)
     assert all('keep' in torch.load('%s.%d' % (out, r)) for r in range(2))
+
+
+def test_a_captured_evaluation_sees_a_changed_weight():
+    """GraphedEval replays only while its signature stays: addresses alone would stay."""
+    from deepipr_amd.experiments.graph_step import GraphedEval
+    lin, x = _layer()
+    net = nn.Sequential(lin, nn.ReLU()).eval()
+    ev = GraphedEval(net)
+    lin.keep()
+    sig = ev._signature()
+    with torch.no_grad():
+        net(x)
+        assert ev._signature() == sig
+        lin.weight.mul_(2)
+    assert ev._signature() != sig
+    lin.keep()
+    sig = ev._signature()
+    lin.weight.grad = torch.ones_like(lin.weight)
+    FlatSGD(lin.parameters(), lr=0.5).step()
+    assert ev._signature() != sig

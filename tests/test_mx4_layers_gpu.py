@@ -170,3 +170,31 @@ def test_a_replayed_step_ends_the_kept_codes(fused):
         assert not torch.equal(lin.weight, before)
         with pytest.raises(RuntimeError, match='keep'):
             lin(feats)
+
+
+def test_a_captured_evaluation_refuses_a_changed_weight():
+    from deepipr_amd.experiments.graph_step import GraphedEval
+    from deepipr_amd.flat_sgd import FlatSGD
+    net = _flat_net().eval()
+    x, t = _batches(1, size=8)[0]
+    lin, ev = net[3], GraphedEval(net)
+    with torch.no_grad():
+        lin.keep()
+        for _ in range(3):
+            assert torch.equal(ev(x, t)[0], net(x).max(1, keepdim=True)[1])
+        assert ev.captures == 1
+        lin.weight.mul_(-1)
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match='keep'):
+                ev(x, t)
+        lin.keep()
+        assert torch.equal(ev(x, t)[0], net(x).max(1, keepdim=True)[1])
+        opt = FlatSGD(lin.parameters(), lr=1.0)                       # (moves the weight to the flat buffer)
+        lin.keep()
+        ev(x, t)
+        lin.weight.grad = torch.randn_like(lin.weight)
+        opt.step()
+        with pytest.raises(RuntimeError, match='keep'):
+            ev(x, t)
+        lin.release()
+        assert torch.equal(ev(x, t)[0], net(x).max(1, keepdim=True)[1])
