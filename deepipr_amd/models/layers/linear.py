@@ -29,7 +29,7 @@ class Mx4Linear(nn.Linear):
     """nn.Linear with the same parameters and state_dict.  Training and evaluation quantise weight and input in the call
     (mx4.linear: output, dx and dw in 4 bits, dbias exact).  A net that only answers can `keep()` its weight in 4 bits instead of
     quantising it per call; the kept codes are buffers outside the state_dict and are dropped by train(), load_state_dict(), release(),
-    by a new `weight` and in copies of the layer.  A kept weight has no backward pass, and changing `weight` in place without a new
+    by a new `weight` or a new type of it and in copies of the layer.  A kept weight has no backward pass, and changing `weight` in place without a new
     keep() is an error, also where an optimiser or the framework's replayed train step does it (what neither autograd nor the framework sees,
     a write through `weight.data` or by a graph that a program captured itself, needs a keep() of its own)."""
 
@@ -76,6 +76,13 @@ class Mx4Linear(nn.Linear):
         if mode:
             self.release()
         return super().train(mode)
+
+    def _apply(self, fn, recurse=True):
+        dtype = self.weight.dtype
+        super()._apply(fn, recurse)
+        if self.weight.dtype != dtype:                       # rounded to another type: other values (a device keeps them)
+            self.release()
+        return self
 
     def _load_from_state_dict(self, *args, **kwargs):
         self.release()

@@ -125,3 +125,16 @@ def test_a_captured_evaluation_sees_a_changed_weight():
     lin.weight.grad = torch.ones_like(lin.weight)
     FlatSGD(lin.parameters(), lr=0.5).step()
     assert ev._signature() != sig
+
+
+def test_another_type_of_weight_ends_the_kept_codes():
+    lin, x = _layer()
+    with torch.no_grad():
+        lin.weight[0] = 2.0 ** -9 + 1.0                            # as bf16: 1
+        lin.weight[0, 0] = 1.25                                    # between the codes 1 and 1.5 of scale 1 / 4
+        want = lin.keep()(x)
+        assert torch.equal(lin.cpu().float()(x), want) and lin.kept_codes is not None          # the same device, the same type
+        lin.bfloat16()
+        assert lin.kept_codes is None and torch.equal(lin(x.bfloat16()), mx4.linear(x.bfloat16(), lin.weight, lin.bias))
+        lin.keep()
+        assert torch.equal(lin.to(torch.bfloat16)(x.bfloat16()), mx4.linear(x.bfloat16(), lin.weight, lin.bias)) and lin.kept_codes is not None
