@@ -51,6 +51,8 @@ class Mx4Linear(nn.Linear):
 
     def keep(self):
         global _hook
+        if self._parameters.get('weight') is None:
+            raise RuntimeError('Mx4Linear.keep: the weight is not a parameter of the layer (a parametrisation computes it anew in every call)')
         q = mx4.quantize(self.weight.detach())
         self.kept_codes, self.kept_scales, self._kept_version = q.codes, q.scales, self.weight._version
         _kept.add(self)
@@ -91,7 +93,8 @@ class Mx4Linear(nn.Linear):
     def forward(self, x):
         if self.kept_codes is None:
             return mx4.linear(x, self.weight, self.bias)
-        if self.weight._version != self._kept_version:
+        weight = self._parameters.get('weight')
+        if weight is None or weight._version != self._kept_version:
             raise RuntimeError('Mx4Linear: the weight changed after keep(); call keep() again, or release()')
         return mx4.linear(x, mx4.Mx4Matrix(self.kept_codes, self.kept_scales, self.out_features, self.in_features, 1), self.bias)
 

@@ -5,6 +5,7 @@ import pytest
 import torch
 import torch.distributed as dist
 import torch.nn as nn
+import torch.nn.utils.parametrize
 
 from deepipr_amd import mx4
 from deepipr_amd import passport_ops as P
@@ -138,3 +139,21 @@ def test_another_type_of_weight_ends_the_kept_codes():
         assert lin.kept_codes is None and torch.equal(lin(x.bfloat16()), mx4.linear(x.bfloat16(), lin.weight, lin.bias))
         lin.keep()
         assert torch.equal(lin.to(torch.bfloat16)(x.bfloat16()), mx4.linear(x.bfloat16(), lin.weight, lin.bias)) and lin.kept_codes is not None
+
+
+def test_a_computed_weight_is_not_kept():
+    """Its version says nothing: every call computes another tensor."""
+    class Twice(nn.Module):
+        def forward(self, w):
+            return w * 2
+    lin, x = _layer()
+    lin.weight = nn.Parameter(lin.weight.detach().clone())          # version 0, as that of a computed tensor
+    lin.keep()
+    nn.utils.parametrize.register_parametrization(lin, 'weight', Twice())
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match='keep'):
+            lin(x)
+        with pytest.raises(RuntimeError, match='not a parameter'):
+            lin.keep()
+        lin.release()
+        assert torch.equal(lin(x), mx4.linear(x, lin.weight, lin.bias))
