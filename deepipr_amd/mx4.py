@@ -18,6 +18,7 @@ what a 4-bit rounding of a trained net leaves of its signature (round_weights_).
 Calls only enqueue work on the current stream, allocate what they need from torch and can be captured into a hipGraph.
 """
 import torch
+from torch.autograd import forward_ad
 
 from deepipr_amd import passport_ops as P
 
@@ -166,9 +167,15 @@ def _rows_ok(x):
     return (x.stride(1) == 1 or x.shape[1] <= 1) and (x.stride(0) >= x.shape[1] or x.shape[0] <= 1)
 
 
+def _has_tangent(t):
+    """Whether t takes part in forward-mode differentiation (no_grad() does not end that)."""
+    return t is not None and forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def linear(x, weight, bias=None):
     """x [..., K] times weight^T plus bias [N], in 4 bits (see the module); -> [..., N] of x's type.  weight: Mx4Matrix [N, K] with blocks along
-    K (frozen: asking for a gradient of x raises), or a float matrix [N, K]; gradients of x, weight and bias as the module states them."""
+    K (frozen: asking for a gradient of x raises), or a float matrix [N, K]; gradients of x, weight and bias as the module states them.
+    Forward-mode derivatives are refused."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise TypeError('mx4.linear: x is a tensor of at least one dimension')
     kept = isinstance(weight, Mx4Matrix)
@@ -187,6 +194,8 @@ def linear(x, weight, bias=None):
     if kept:
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise RuntimeError('mx4.linear: a weight kept in 4 bits has no backward pass; pass the float weight, or use torch.no_grad()')
+        if _has_tangent(x) or _has_tangent(bias):
+            raise RuntimeError('mx4.linear has no forward-mode derivative')
         m = rows.shape[0]
         if m == 0 or n == 0 or k == 0:
             P.kernels._mx4_chk('mx4_linear', rows, weight.codes, bias)

@@ -158,3 +158,20 @@ def test_kept_codes_do_not_outlive_their_weight():
         lin.weight.mul_(2)
         with pytest.raises(RuntimeError, match='keep'):
             lin(x)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_is_refused(grad):
+    """Neither form loses a tangent without a word."""
+    x, w, b = torch.randn(3, 40), torch.randn(8, 40), torch.randn(8)
+    q = mx4.quantize(w)
+    for weight in (q, w):
+        with torch.set_grad_enabled(grad), torch.autograd.forward_ad.dual_level():
+            for dual in (0, 1):
+                args = [x, b]
+                args[dual] = torch.autograd.forward_ad.make_dual(args[dual], torch.ones_like(args[dual]))
+                with pytest.raises((RuntimeError, NotImplementedError), match='forward-mode|forward mode'):
+                    mx4.linear(args[0], weight, args[1])
+            assert mx4.linear(x, weight, b).shape == (3, 8)
+    with torch.no_grad():
+        assert mx4.linear(x, q, b).shape == (3, 8)
