@@ -132,17 +132,21 @@ def matmul(a, b, bias=None, dtype=torch.float32):
     return _product((a.codes, a.scales), (b.codes, b.scales), a.rows, b.rows, a.cols, _bias_of(bias, b.rows), dtype, a)
 
 
+def _forward(x, w, bias, need_dx, need_dw):
+    """-> the output, what the backward pass needs (or None)."""
+    (m, k), n = x.shape, w.shape[0]
+    b = _bias_of(bias, n)
+    if m == 0 or n == 0 or k == 0:
+        return _product(None, None, m, n, k, b, x.dtype, x), None
+    return P.kernels.mx4_linear_fwd(x.detach(), w.detach(), None, b, need_dx, need_dw)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias):
         need_dx, need_dw, _ = ctx.needs_input_grad
-        (m, k), n = x.shape, w.shape[0]
-        ctx.dims, ctx.types = (m, n, k), (x.dtype, w.dtype, None if bias is None else bias.dtype)
-        b = _bias_of(bias, n)
-        if m == 0 or n == 0 or k == 0:
-            ctx.save_for_backward(None)
-            return _product(None, None, m, n, k, b, x.dtype, x)
-        y, saved = P.kernels.mx4_linear_fwd(x, w, None, b, need_dx, need_dw)
+        ctx.dims, ctx.types = (x.shape[0], w.shape[0], x.shape[1]), (x.dtype, w.dtype, None if bias is None else bias.dtype)
+        y, saved = _forward(x, w, bias, need_dx, need_dw)
         ctx.save_for_backward(saved)
         return y
 
@@ -203,5 +207,9 @@ def linear(x, weight, bias=None):
         else:
             y, _ = P.kernels.mx4_linear_fwd(rows.detach(), None, (weight.codes, weight.scales, n), _bias_of(bias, n), False, False)
     else:
-        y = _Linear.apply(rows, weight if _rows_ok(weight) else weight.contiguous(), bias)
+        weight = weight if _rows_ok(weight) else weight.contiguous()
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+            y = _Linear.apply(rows, weight, bias)
+        else:                                                # (needs_input_grad names the tensors that require one, also without grad mode)
+            y, _ = _forward(rows, weight, bias, False, False)
     return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (n,))

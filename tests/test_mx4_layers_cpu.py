@@ -175,3 +175,25 @@ def test_forward_mode_is_refused(grad):
             assert mx4.linear(x, weight, b).shape == (3, 8)
     with torch.no_grad():
         assert mx4.linear(x, q, b).shape == (3, 8)
+
+
+def test_nothing_is_saved_without_grad_mode(monkeypatch):
+    """Evaluation: no buffer for a backward pass, and input and weight in one direction each (which share a launch)."""
+    asked, real = [], LmKernels.mx4_linear_fwd
+
+    def recorded(self, x, w, kept, bias, need_dx, need_dw):
+        asked.append((need_dx, need_dw))
+        return real(self, x, w, kept, bias, need_dx, need_dw)
+    monkeypatch.setattr(LmKernels, 'mx4_linear_fwd', recorded)
+    lin, x = Mx4Linear(40, 8), torch.randn(3, 40, requires_grad=True)
+    y = lin(x)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            assert torch.equal(lin(x), y) and not lin(x).requires_grad
+    assert asked == [(True, True)] + [(False, False)] * 4
+    y.sum().backward()
+    assert x.grad is not None and lin.weight.grad is not None
+    lin(x.detach())
+    lin.weight.requires_grad_(False)
+    lin(x)
+    assert asked[5:] == [(False, True), (True, False)]
