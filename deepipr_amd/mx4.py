@@ -137,6 +137,7 @@ def _forward(x, w, bias, need_dx, need_dw):
     (m, k), n = x.shape, w.shape[0]
     b = _bias_of(bias, n)
     if m == 0 or n == 0 or k == 0:
+        P.kernels._mx4_chk('mx4_linear', x, w, bias)
         return _product(None, None, m, n, k, b, x.dtype, x), None
     return P.kernels.mx4_linear_fwd(x.detach(), w.detach(), None, b, need_dx, need_dw)
 

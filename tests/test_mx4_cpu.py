@@ -78,3 +78,11 @@ def test_host_tensors_and_shapes_are_refused():
         mx4.linear(x, x[:, :3])
     with pytest.raises(ValueError, match='bias'):
         mx4.linear(x, x, x[0])
+
+
+def test_empty_host_tensors_are_refused_too():
+    x, w = torch.ones(4, 40), torch.ones(3, 40)
+    for a, b in ((x[:0], w), (x, w[:0]), (x[:, :0], w[:, :0])):
+        for grad in (False, True):
+            with pytest.raises(RuntimeError, match='GPU only'):
+                mx4.linear(a, b.clone().requires_grad_(grad))
