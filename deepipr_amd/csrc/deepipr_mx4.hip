@@ -285,26 +285,38 @@ __global__ __launch_bounds__(kThreads) void k_mx4_quantise(const Matrix A, const
     }
 }
 
-// sums [tiles][C] -> out [ceil(tiles / kSumTiles)][C]: eight threads a column, each every eighth tile in order, then the eight in order
+// Adds up groups of 128 tiles' sums of each column, in 64 bits: eight threads a column, each every eighth tile in order, then the eight in
+// order.  The first pass reads sums [tiles][C] in 32 bits.  With more than one group a group's sum takes the place of its first two rows
+// (low and high word; a group has at least two: the tiles come in pairs), which only this workgroup has read, and the next pass adds up
+// those: its item t lies in rows t * step and t * step + 1.  The last pass rounds once, to `out`.
 constexpr int kSumTiles = 128;
-__global__ __launch_bounds__(kThreads) void k_mx4_colsum(const float *__restrict__ sums, long long tiles, long long C, float *__restrict__ out) {
+template <bool FIRST>
+__global__ __launch_bounds__(kThreads) void k_mx4_colsum(float *sums, long long items, long long step, long long C, float *out) {
     __shared__ double red[8][32];
-    sums += blockIdx.y * kSumTiles * C;
-    out += blockIdx.y * C;
-    tiles = min(tiles - static_cast<long long>(blockIdx.y) * kSumTiles, static_cast<long long>(kSumTiles));
+    const long long t0 = static_cast<long long>(blockIdx.y) * kSumTiles;
+    const int n = static_cast<int>(min(items - t0, static_cast<long long>(kSumTiles)));
     const int col = threadIdx.x & 31, part = threadIdx.x >> 5;
     const long long c = static_cast<long long>(blockIdx.x) * 32 + col;
+    float *at = sums + t0 * step * C + c;
     double v = 0.0;
     if (c < C) {
 #pragma unroll 4
-        for (long long t = part; t < tiles; t += 8) v += static_cast<double>(sums[t * C + c]);
+        for (int t = part; t < n; t += 8) {
+            const float *p = at + t * step * C;
+            v += FIRST ? static_cast<double>(p[0]) : __hiloint2double(__float_as_int(p[C]), __float_as_int(p[0]));
+        }
     }
     red[part][col] = v;
     __syncthreads();
     if (part == 0 && c < C) {
 #pragma unroll
         for (int i = 1; i < 8; ++i) v += red[i][col];
-        out[c] = static_cast<float>(v);
+        if (gridDim.y == 1) {
+            out[c] = static_cast<float>(v);
+        } else {
+            at[0] = __int_as_float(__double2loint(v));
+            at[C] = __int_as_float(__double2hiint(v));
+        }
     }
 }
 
@@ -1023,18 +1035,18 @@ void quantise(int dtype, const Matrix &m, const Matrix *other, hipStream_t st) {
     }
 }
 void column_sums(const Matrix &m, float *out, hipStream_t st) {
-    float *sums = m.sums;
-    for (long long tiles = round_up(m.R, 128) / kQR;;) {                 // at most 128 tiles in one go: long batches take a second or third pass
-        const long long groups = (tiles + kSumTiles - 1) / kSumTiles;
-        float *to = groups == 1 ? out : sums + tiles * m.C;
-        hipLaunchKernelGGL(k_mx4_colsum, dim3(static_cast<unsigned>((m.C + 31) / 32), static_cast<unsigned>(groups)), dim3(kThreads), 0, st, sums,
-                           tiles, m.C, to);
+    long long items = round_up(m.R, 128) / kQR, step = 1;
+    for (;;) {                                                           // at most 128 items in one go: long batches take a second or third pass
+        const long long groups = (items + kSumTiles - 1) / kSumTiles;
+        const dim3 grid(static_cast<unsigned>((m.C + 31) / 32), static_cast<unsigned>(groups)), block(kThreads);
+        if (step == 1) hipLaunchKernelGGL((k_mx4_colsum<true>), grid, block, 0, st, m.sums, items, step, m.C, out);
+        else hipLaunchKernelGGL((k_mx4_colsum<false>), grid, block, 0, st, m.sums, items, step, m.C, out);
         if (groups == 1) return;
-        sums = to;
-        tiles = groups;
+        items = groups;
+        step *= kSumTiles;
     }
 }
-inline size_t sums_bytes(long long R, long long C) {                      // every level's sums
+inline size_t sums_bytes(long long R, long long C) {                      // the tiles' sums (and a row for every group of them, which stays free)
     size_t n = 0;
     for (long long tiles = round_up(R, 128) / kQR;; tiles = (tiles + kSumTiles - 1) / kSumTiles) {
         n += static_cast<size_t>(tiles);

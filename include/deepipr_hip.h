@@ -451,8 +451,8 @@ int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const D
  *           the row 32 t + r of the 64-row group, at [..][..][e][r][h][t] -- the order in which the matrix instruction's lanes take them.
  *   deepipr_mx4_quantize    x [rows][cols] (row_stride elements between rows) in one pass: blocks along the rows (row_codes / row_scales),
  *           and / or blocks along the columns, i.e. the matrix x^T [cols][rows] (col_codes / col_scales); either pair may be NULL.
- *           col_sums (may be NULL; needs the column direction): the sums of x's columns, fp32 sums of 32 and 64 rows, then 64-bit in row
- *           order; workspace: deepipr_mx4_quantize_workspace_bytes() bytes when col_sums is given.
+ *           col_sums (may be NULL; needs the column direction): the sums of x's columns, fp32 sums of 32 and 64 rows, added up in
+ *           64 bits in an order that the number of rows fixes, rounded once; workspace: deepipr_mx4_quantize_workspace_bytes() bytes when col_sums is given.
  *   deepipr_mx4_dequantize  the values in `dtype`: [rows][cols], or with transposed = 1 [cols][rows].
  *   deepipr_mx4_matmul      out [M][N] = A B^T (+ bias [N]), A [M][K] and B [N][K] quantised, on the block-scaled matrix instructions;
  *           fp32 products and sums, one rounding to `dtype`.  A NaN block makes NaN of every output whose row or column holds it.  workspace:
