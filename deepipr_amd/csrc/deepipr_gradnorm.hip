@@ -456,13 +456,19 @@ template <bool PLACED, class F> bool launches(const DeepiprTensor *t, int n, con
     return flush();
 }
 
-template <int P> int partials(const char *what, const DeepiprTensor *t, int n, const Cut &per, size_t bytes, double *part, int *used,
-                              hipStream_t st) {
+// Every launch is timed by itself, with its own bytes.
+inline double bytes_of(const List &L) {
+    double bytes = 0.0;
+    for (int i = 0; i < L.n; ++i) bytes += static_cast<double>(L.count[i] & 0x3fffffffu) * static_cast<double>(elem_bytes(L.count[i] >> 30));
+    return bytes;
+}
+
+template <int P> int partials(const char *what, const DeepiprTensor *t, int n, const Cut &per, double *part, int *used, hipStream_t st) {
     int at = 0;
-    DiprProf prof(DEEPIPR_K_GRAD_NORM);
-    prof.bytes = static_cast<double>(bytes);
     const bool ok = launches<false>(t, n, per, [&](const List &L, int runs) {
         if (at + runs > kMaxPartials) return false;
+        DiprProf prof(DEEPIPR_K_GRAD_NORM);
+        if (prof.a) prof.bytes = bytes_of(L);
         DIPR_LAUNCH(prof, (k_norm_partials<P>), dim3(runs), dim3(kThreads), st, L, part + at);
         at += runs;
         return true;
@@ -498,12 +504,11 @@ int check_common(const char *what, int norm_type, const void *workspace, size_t 
     return DEEPIPR_OK;
 }
 
-int list_partials(const char *what, const DeepiprTensor *t, int n, int norm_type, const Cut &per, size_t bytes, double *part, int *used,
-                  hipStream_t st) {
+int list_partials(const char *what, const DeepiprTensor *t, int n, int norm_type, const Cut &per, double *part, int *used, hipStream_t st) {
     switch (norm_type) {
-        case 2: return partials<2>(what, t, n, per, bytes, part, used, st);
-        case 1: return partials<1>(what, t, n, per, bytes, part, used, st);
-        default: return partials<0>(what, t, n, per, bytes, part, used, st);
+        case 2: return partials<2>(what, t, n, per, part, used, st);
+        case 1: return partials<1>(what, t, n, per, part, used, st);
+        default: return partials<0>(what, t, n, per, part, used, st);
     }
 }
 
@@ -529,13 +534,15 @@ int deepipr_grad_norm(const DeepiprTensor *tensors, int n, int norm_type, float 
     if (elements && is_short(tensors, n, units)) return one<false>(what, tensors, n, units, norm_type, bytes, 0.0f, norm, st);
     int used = 0;
     if (elements) {
-        rc = list_partials(what, tensors, n, norm_type, per, bytes, part, &used, st);
+        rc = list_partials(what, tensors, n, norm_type, per, part, &used, st);
         if (rc != DEEPIPR_OK) return rc;
     }
+    DiprProf prof(DEEPIPR_K_GRAD_NORM);
+    prof.bytes = used * 8.0;
     switch (norm_type) {
-        case 2: hipLaunchKernelGGL((k_norm_finish<2>), dim3(1), dim3(kThreads), 0, st, part, used, norm); break;
-        case 1: hipLaunchKernelGGL((k_norm_finish<1>), dim3(1), dim3(kThreads), 0, st, part, used, norm); break;
-        default: hipLaunchKernelGGL((k_norm_finish<0>), dim3(1), dim3(kThreads), 0, st, part, used, norm); break;
+        case 2: DIPR_LAUNCH(prof, k_norm_finish<2>, dim3(1), dim3(kThreads), st, part, used, norm); break;
+        case 1: DIPR_LAUNCH(prof, k_norm_finish<1>, dim3(1), dim3(kThreads), st, part, used, norm); break;
+        default: DIPR_LAUNCH(prof, k_norm_finish<0>, dim3(1), dim3(kThreads), st, part, used, norm); break;
     }
     return dipr_check_launch(what);
 }
@@ -562,11 +569,11 @@ int deepipr_grad_clip(const DeepiprTensor *tensors, int n, int norm_type, float 
     if (!per.groups) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
     if (is_short(tensors, n, units)) return one<true>(what, tensors, n, units, norm_type, bytes, max_norm, norm, st);
     int used = 0;
-    rc = list_partials(what, tensors, n, norm_type, per, bytes, part, &used, st);
+    rc = list_partials(what, tensors, n, norm_type, per, part, &used, st);
     if (rc != DEEPIPR_OK) return rc;
-    DiprProf prof(DEEPIPR_K_GRAD_CLIP);
-    prof.bytes = 2.0 * static_cast<double>(bytes);
     launches<false>(tensors, n, per, [&](const List &L, int runs) {
+        DiprProf prof(DEEPIPR_K_GRAD_CLIP);
+        if (prof.a) prof.bytes = 2.0 * bytes_of(L);
         switch (norm_type) {
             case 2: DIPR_LAUNCH(prof, (k_clip<2>), dim3(runs), dim3(kThreads), st, L, part, used, max_norm, norm); break;
             case 1: DIPR_LAUNCH(prof, (k_clip<1>), dim3(runs), dim3(kThreads), st, L, part, used, max_norm, norm); break;
@@ -600,11 +607,11 @@ int deepipr_sgd_momentum_step_clipped(float *param, float *momentum_buf, const D
     const Cut per = cut(grads, n, units);
     if (!per.groups) return dipr_fail(DEEPIPR_EINVAL, "%s: too many tensors", what);
     int used = 0;
-    rc = list_partials(what, grads, n, 2, per, bytes, part, &used, st);
+    rc = list_partials(what, grads, n, 2, per, part, &used, st);
     if (rc != DEEPIPR_OK) return rc;
-    DiprProf prof(DEEPIPR_K_SGD);
-    prof.bytes = 20.0 * static_cast<double>(elements);
     launches<true>(grads, n, per, [&](const List &L, int runs) {
+        DiprProf prof(DEEPIPR_K_SGD);
+        if (prof.a) prof.bytes = 5.0 * bytes_of(L);
         DIPR_LAUNCH(prof, k_sgd_clipped, dim3(runs), dim3(kThreads), st, L, part, used, param, momentum_buf, hyper, norm);
         return true;
     });

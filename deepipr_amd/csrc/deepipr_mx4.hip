@@ -473,8 +473,9 @@ struct Product {
     long long first, last;                               // rows first .. last - 1 of the output (first a multiple of 64)
     int kt, splits;                                      // splits > 1: out is float [splits][M][N], split i adds up its share of the steps
     void *out;
+    long long K;                                         // columns
     const void *x;                                       // a in its own type instead of a / sa (k_mx4_gemm_rows with X >= 0)
-    long long x_stride, K;
+    long long x_stride;
     int x_vec;                                           // its rows start on 16-byte boundaries
 };
 
@@ -953,7 +954,12 @@ Plan plan(long long M, long long N, long long kt) {
     return p;
 }
 
-template <int T> void launch_rows(DiprProf &prof, const Product &P, hipStream_t st) {
+inline double flops(const Product &P) { return 2.0 * static_cast<double>(P.last - P.first) * static_cast<double>(P.N) * static_cast<double>(P.K); }
+
+// Every launch is timed by itself, with its own operations.
+template <int T> void launch_rows(const Product &P, hipStream_t st) {
+    DiprProf prof(DEEPIPR_K_MX4_MATMUL);
+    prof.bytes = flops(P);
     const dim3 grid(static_cast<unsigned>((P.N + 15) / 16)), block(512);
     const long long rows = P.last - P.first;
     if (rows <= 16) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 1, 1, -1>), grid, block, st, P, P, grid.x);
@@ -961,10 +967,10 @@ template <int T> void launch_rows(DiprProf &prof, const Product &P, hipStream_t 
     else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, 1, -1>), grid, block, st, P, P, grid.x);
 }
 
-template <int T> void launch_product(DiprProf &prof, Product P, const Product *other, float *part, hipStream_t st) {
+template <int T> void launch_product(Product P, const Product *other, float *part, hipStream_t st) {
     const dim3 block(kThreads);
     const Plan p = plan(P.M, P.N, P.kt);
-    if (p.form == Plan::kRows) return launch_rows<T>(prof, P, st);
+    if (p.form == Plan::kRows) return launch_rows<T>(P, st);
     if (p.strips()) {
         int nt = p.form == Plan::k64x32 ? 2 : 4;
         if (other)                                       // one width for both
@@ -973,6 +979,8 @@ template <int T> void launch_product(DiprProf &prof, Product P, const Product *o
         const unsigned first = static_cast<unsigned>(strips_of(P.M, P.N, nt));
         const dim3 grid(first + (other ? static_cast<unsigned>(strips_of(other->M, other->N, nt)) : 0u)), wide(512);
         const Product &Q = other ? *other : P;
+        DiprProf prof(DEEPIPR_K_MX4_MATMUL);
+        prof.bytes = flops(P) + (other ? flops(Q) : 0.0);
         if (nt == 2) DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, 2, -1>), grid, wide, st, P, Q, first);
         else DIPR_LAUNCH(prof, (k_mx4_gemm_rows<T, 4, 4, -1>), grid, wide, st, P, Q, first);
         return;
@@ -984,12 +992,14 @@ template <int T> void launch_product(DiprProf &prof, Product P, const Product *o
         if (tails[i]) {
             Product Q = *both[i];
             Q.first = Q.M - tails[i];
-            launch_rows<T>(prof, Q, st);
+            launch_rows<T>(Q, st);
             both[i]->last -= tails[i];
         }
     const int side = p.form == Plan::kLarge ? 256 : 128;
     const unsigned first = static_cast<unsigned>(tiles_of(P.last, P.N, side)) * p.splits;
     const dim3 grid(first + (other ? static_cast<unsigned>(tiles_of(O.last, O.N, side)) : 0u));
+    DiprProf prof(DEEPIPR_K_MX4_MATMUL);
+    prof.bytes = flops(P) + (other ? flops(O) : 0.0);
     if (p.form == Plan::kLarge) {
         DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<T, 4, 4, 3>), grid, block, st, P, O, first);
     } else if (p.splits == 1) {
@@ -1001,8 +1011,9 @@ template <int T> void launch_product(DiprProf &prof, Product P, const Product *o
         Q.bias = nullptr;
         DIPR_LAUNCH(prof, (k_mx4_gemm_tiled<F32, 2, 2, 3>), grid, block, st, Q, Q, first);
         const long long want = (P.M * ((P.N + 3) / 4) + kThreads - 1) / kThreads;
-        hipLaunchKernelGGL((k_mx4_gemm_sum<T>), dim3(static_cast<unsigned>(want < 8192 ? want : 8192)), block, 0, st, part, p.splits, P.bias,
-                           P.bias_type, P.M, P.N, P.out);
+        DiprProf sum(DEEPIPR_K_MX4_MATMUL);              // time of the product, no operations of its own
+        DIPR_LAUNCH(sum, (k_mx4_gemm_sum<T>), dim3(static_cast<unsigned>(want < 8192 ? want : 8192)), block, st, part, p.splits, P.bias,
+                    P.bias_type, P.M, P.N, P.out);
     }
 }
 
@@ -1039,8 +1050,10 @@ void column_sums(const Matrix &m, float *out, hipStream_t st) {
     for (;;) {                                                           // at most 128 items in one go: long batches take a second or third pass
         const long long groups = (items + kSumTiles - 1) / kSumTiles;
         const dim3 grid(static_cast<unsigned>((m.C + 31) / 32), static_cast<unsigned>(groups)), block(kThreads);
-        if (step == 1) hipLaunchKernelGGL((k_mx4_colsum<true>), grid, block, 0, st, m.sums, items, step, m.C, out);
-        else hipLaunchKernelGGL((k_mx4_colsum<false>), grid, block, 0, st, m.sums, items, step, m.C, out);
+        DiprProf prof(DEEPIPR_K_MX4_QUANTIZE);
+        prof.bytes = static_cast<double>(items) * static_cast<double>(m.C) * (step == 1 ? 4.0 : 8.0);
+        if (step == 1) DIPR_LAUNCH(prof, k_mx4_colsum<true>, grid, block, st, m.sums, items, step, m.C, out);
+        else DIPR_LAUNCH(prof, k_mx4_colsum<false>, grid, block, st, m.sums, items, step, m.C, out);
         if (groups == 1) return;
         items = groups;
         step *= kSumTiles;
@@ -1076,6 +1089,7 @@ Product product_of(const void *a, const void *sa, const void *b, const void *sb,
     P.bias_type = bias_dtype;
     P.M = P.last = M;
     P.N = N;
+    P.K = K;
     P.kt = static_cast<int>(round_up(K, 128) / 128);
     P.splits = 1;
     P.out = out;
@@ -1090,12 +1104,10 @@ bool alike(const Product &p, const Product &q) {
 }
 // `other`: a second product that is alike, in the same launch
 void run(const Product &P, const Product *other, int dtype, void *workspace, hipStream_t st) {
-    DiprProf prof(DEEPIPR_K_MX4_MATMUL);
-    prof.bytes = 256.0 * (static_cast<double>(P.M) * P.N * P.kt + (other ? static_cast<double>(other->M) * other->N * other->kt : 0.0));
     switch (dtype) {
-        case F32: launch_product<F32>(prof, P, other, static_cast<float *>(workspace), st); break;
-        case BF16: launch_product<BF16>(prof, P, other, static_cast<float *>(workspace), st); break;
-        default: launch_product<F16>(prof, P, other, static_cast<float *>(workspace), st); break;
+        case F32: launch_product<F32>(P, other, static_cast<float *>(workspace), st); break;
+        case BF16: launch_product<BF16>(P, other, static_cast<float *>(workspace), st); break;
+        default: launch_product<F16>(P, other, static_cast<float *>(workspace), st); break;
     }
 }
 
@@ -1103,12 +1115,11 @@ void run(const Product &P, const Product *other, int dtype, void *workspace, hip
 void product_of_rows(const void *x, int dtype, long long x_stride, const void *b, const void *sb, const void *bias, int bias_dtype, long long M,
                      long long N, long long K, void *out, hipStream_t st) {
     Product P = product_of(nullptr, nullptr, b, sb, bias, bias_dtype, M, N, K, out);
-    P.K = K;
     P.x = x;
     P.x_stride = x_stride;
     P.x_vec = aligned(x, 16) && (M == 1 || x_stride * elem_bytes(dtype) % 16 == 0);
     DiprProf prof(DEEPIPR_K_MX4_MATMUL);
-    prof.bytes = 2.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+    prof.bytes = flops(P);
     const dim3 grid(static_cast<unsigned>((N + 15) / 16)), block(512);
     switch (dtype) {
         case F32: DIPR_LAUNCH(prof, (k_mx4_gemm_rows<F32, 1, 1, F32>), grid, block, st, P, P, grid.x); break;

@@ -96,7 +96,7 @@ int deepipr_event_synchronize(void *event);
 #define DEEPIPR_K_CONV1X1_DGRAD 35
 #define DEEPIPR_K_HEAD 36                 /* avg-pool + Linear of the CIFAR-geometry classifier, forward / backward (bytes) */
 #define DEEPIPR_K_GRAD_NORM 37            /* partial sums of a gradient list's norm (bytes) */
-#define DEEPIPR_K_GRAD_CLIP 38            /* the list scaled in place (bytes) */
+#define DEEPIPR_K_GRAD_CLIP 38            /* the list scaled in place (bytes of a list that is scaled: one within max_norm is not touched) */
 #define DEEPIPR_K_MX4_QUANTIZE 39         /* bytes */
 #define DEEPIPR_K_MX4_DEQUANTIZE 40       /* bytes */
 #define DEEPIPR_K_MX4_MATMUL 41           /* FLOPs */
