@@ -143,6 +143,7 @@ TEST_HOOK_SIGNATURES = {
     'deepipr_debug_tune': (_int, [_c.c_char_p, _int]),
     'deepipr_debug_trace': (_int, [_vp]),
     'deepipr_debug_wino_trace': (_int, [_vp]),
+    'deepipr_debug_mx4_plan': (_int, [_i64, _i64, _i64, _vp]),
 }
 ABI_VERSION = 13
 SYNC_WORDS = 2 * (256 * 30 * 4 + 4096 + 63 * 2048) + 16     # DEEPIPR_SYNC_WORDS

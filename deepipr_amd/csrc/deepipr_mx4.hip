@@ -1350,4 +1350,15 @@ int deepipr_mx4_linear_bwd(const void *dy, int dy_dtype, long long dy_stride, lo
     return dipr_check_launch(what);
 }
 
+#ifdef DEEPIPR_TEST_HOOKS
+int deepipr_debug_mx4_plan(long long M, long long N, long long K, long long *plan_out) {
+    if (!plan_out || M <= 0 || N <= 0 || K <= 0 || !product_fits(M, N, K)) return dipr_fail(DEEPIPR_EINVAL, "debug_mx4_plan: bad argument");
+    const Plan p = plan(M, N, round_up(K, 128) / 128);
+    plan_out[0] = p.form;
+    plan_out[1] = p.splits;
+    plan_out[2] = p.tail;
+    return DEEPIPR_OK;
+}
+#endif
+
 }  // extern "C"

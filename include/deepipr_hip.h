@@ -280,7 +280,7 @@ int deepipr_passport_bwd(const float *dy, const float *xhat, const float *gamma,
 int deepipr_set_resident(int mode);
 #ifdef DEEPIPR_TEST_HOOKS
 /* MEASUREMENT / TEST BUILD ONLY (libdeepipr_hip_trace.so, `make -C deepipr_amd/csrc trace`): the production library
- * exports neither symbol and its kernels carry neither the knobs nor the hooks.
+ * exports none of them and its kernels carry neither the knobs nor the hooks.
  * deepipr_debug_tune: planning knobs of the single-pass kernels, process-wide: "split_full" (default 1: split
  * channels over workgroups whenever they do not fill the chip; 0: only below half), "xcd_map" (default 0; 1: a
  * channel's slices on workgroups with equal index % 8), "small_t"; and the time-out test hooks "exchange_spin" (bound
@@ -297,6 +297,9 @@ int deepipr_debug_trace(unsigned long long *device_buffer);
  * sums in LDS, 4 stores issued, then for the first nine chunks: step top, LDS writes drained, barrier passed
  * (tools/wino_trace.py).  64 * 8 bytes per workgroup; NULL switches it off. */
 int deepipr_debug_wino_trace(unsigned long long *device_buffer);
+/* The kernels that a 4-bit product takes (256 CUs where there is no device): plan[0] = 0: up to 64 rows a workgroup of 16 columns, 1: 64 x 32
+ * tiles, 2: 64 x 64, 3: 128 x 128, 4: 256 x 256; plan[1]: workgroups that share a tile's columns; plan[2]: rows at the end that go apart. */
+int deepipr_debug_mx4_plan(long long M, long long N, long long K, long long *plan);
 #endif
 int deepipr_passport_bn_resident(int N, int C, int HW, int have_sync);
 /* Workgroups per channel the single-pass kernels would use for this shape when exchange words are passed (the larger
