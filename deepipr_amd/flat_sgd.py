@@ -166,7 +166,7 @@ class FlatSGD(torch.optim.Optimizer):
         pieces = []
         for p, off in self._slots[lo:hi]:
             n = p.numel()
-            pad = _pad(n) - n
+            pad = -n % _ALIGN
             if p.grad is None:
                 pieces.append(self._zeros(n + pad))
                 continue
