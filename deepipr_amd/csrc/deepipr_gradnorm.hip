@@ -214,7 +214,9 @@ template <int P> __device__ __forceinline__ double norm_of(const double *__restr
 }
 
 // min(1, max / (n + eps)); NaN and infinity go the way of the arithmetic: a NaN norm gives NaN, an infinite one 0.  The factor and its
-// product with a gradient are held in 64 bits: a norm near the end of float's range would leave a float factor with few digits.
+// product with a gradient are held in 64 bits: a norm near the end of float's range would leave a float factor with few digits.  The
+// product is rounded to 32 bits, and for 16-bit tensors again to their type: next to a border that can be the other neighbour (an
+// error of half a step and 2^-24 of the value).
 __device__ __forceinline__ double factor_of(double norm, float max_norm) {
     const double f = static_cast<double>(max_norm) / (norm + kClipEps);
     return f >= 1.0 ? 1.0 : f;

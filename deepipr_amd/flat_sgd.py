@@ -13,6 +13,8 @@ the MI355X-first form instead:
     (75 % of ResNet18's bytes sit in layer4, whose gradients are ready first); each bucket is packed with one
     `cat` kernel and all-reduced on RCCL's stream as soon as its last gradient has been accumulated, i.e.
     while the earlier layers are still back-propagating; only the small last bucket (2.7 MB) waits for step();
+  * behind the last bucket travels one float per parameter, 1 where this rank has its gradient: a missing gradient counts as
+    zero in the average, and a parameter stays out of the step only if no rank has a gradient for it;
   * one process per GPU; rank 0's parameters/buffers are broadcast once (distributed.broadcast_state).
 
 It is a torch.optim.Optimizer (param_groups, zero_grad, lr schedulers work unchanged) and goes wherever the

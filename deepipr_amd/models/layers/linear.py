@@ -104,7 +104,8 @@ class Mx4Linear(nn.Linear):
 
 def use_mx4_linear_(model):
     """Every plain nn.Linear of `model` becomes an Mx4Linear in place (optimisers built before or after see the same parameters);
-    -> how many."""
+    -> how many.  Where two branches go through the layer as one batch (the lockstep form of schemes V2 and V3), the weight gradient's blocks of
+    32 rows are those of that batch: unless a branch has a multiple of 32 rows, one block holds rows of both."""
     found = [m for m in model.modules() if type(m) is nn.Linear]
     for m in found:
         Mx4Linear.adopt_(m)

@@ -124,7 +124,7 @@ def _product(a, b, m, n, k, bias, dtype, like):
 
 def matmul(a, b, bias=None, dtype=torch.float32):
     """a [M, K] times the transpose of b [N, K] (as STORED: a.rows x a.cols, b.rows x b.cols; the blocks of both run along K), plus
-    bias [N]; -> [M, N] of `dtype`."""
+    bias [N]; -> [M, N] of `dtype`.  Not differentiable, in the bias neither."""
     if not isinstance(a, Mx4Matrix) or not isinstance(b, Mx4Matrix):
         raise TypeError('mx4.matmul takes quantised matrices (mx4.quantize)')
     if a.cols != b.cols:

@@ -412,7 +412,8 @@ int deepipr_sgd_momentum_step_multi(float *param, float *momentum_buf, const lon
  *   deepipr_grad_norm   *norm = n.
  *   deepipr_grad_clip   g *= f in place, f = min(1, max_norm / (n + 1e-6)); *norm = n, the norm BEFORE clipping.  f == 1 writes
  *                       nothing (1 * g is g in every type).  A NaN norm makes every gradient NaN, an infinite one makes the finite
- *                       gradients 0.  Products are rounded once to the tensor's type.  Tensors that share memory are refused.
+ *                       gradients 0.  Factor and product are held in 64 bits and rounded to 32, for 16-bit tensors from there to their type (at most
+ *                       2^-24 of the value more than half a step).  Tensors that share memory are refused.
  *   deepipr_sgd_momentum_step_clipped   the step of deepipr_sgd_momentum_step_dev behind that rule, on gradients that lie where
  *                       autograd left them: d = (f * grad_scale) * g + weight_decay * p; buf = momentum * buf + d; p -= lr * buf, with
  *                       n the 2-norm of grad_scale * g over the whole list.  hyper (device) = {lr, momentum, weight_decay, grad_scale,
