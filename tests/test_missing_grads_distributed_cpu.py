@@ -106,3 +106,15 @@ def test_ranks_stay_together_where_one_misses_a_gradient(mode, top, tmp_path):
     # 32-bit steps on both sides, in another order: as in tests/test_grad_clip_distributed_cpu.py
     assert all(torch.allclose(a, b, rtol=1e-4, atol=1e-6) for a, b in zip(p0, net.parameters()))
     assert all(torch.equal(a, b) for a, b in zip(p0[-2:], spare))
+
+
+def test_a_captured_step_that_would_have_to_read_the_flags_is_refused(world_of_one, monkeypatch):
+    from types import SimpleNamespace
+
+    from deepipr_amd.flat_sgd import FlatSGD
+    opt = FlatSGD(_net().parameters(), lr=0.1, max_grad_norm=1.0)
+    opt.flat_param = SimpleNamespace(is_cuda=True)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    assert opt._missing_everywhere([]) == []                           # nothing missing here: nothing to read
+    with pytest.raises(RuntimeError, match='cannot be captured'):
+        opt._missing_everywhere([1])
