@@ -8,7 +8,7 @@ from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from deepipr_amd import mx4
 
-_kept = weakref.WeakSet()          # the layers that hold codes of their weight
+_kept = weakref.WeakKeyDictionary()          # the layers that hold codes of their weight -> that weight (weakly)
 _hook = None
 
 
@@ -55,14 +55,14 @@ class Mx4Linear(nn.Linear):
             raise RuntimeError('Mx4Linear.keep: the weight is not a parameter of the layer (a parametrisation computes it anew in every call)')
         q = mx4.quantize(self.weight.detach())
         self.kept_codes, self.kept_scales, self._kept_version = q.codes, q.scales, self.weight._version
-        _kept.add(self)
+        _kept[self] = weakref.ref(self.weight)
         if _hook is None:                                    # fused optimisers write without raising a version
             _hook = register_optimizer_step_post_hook(_stepped)
         return self.eval()
 
     def release(self):
         self.kept_codes = self.kept_scales = self._kept_version = None
-        _kept.discard(self)
+        _kept.pop(self, None)
         return self
 
     def register_parameter(self, name, param):               # (also what `layer.weight = ...` calls)
@@ -93,8 +93,9 @@ class Mx4Linear(nn.Linear):
     def forward(self, x):
         if self.kept_codes is None:
             return mx4.linear(x, self.weight, self.bias)
-        weight = self._parameters.get('weight')
-        if weight is None or weight._version != self._kept_version:
+        weight, of = self._parameters.get('weight'), _kept[self]() if self in _kept else None
+        # (torch.func.functional_call puts other tensors in the parameters' place, or detached ones of the same memory)
+        if weight is None or of is None or weight._version != self._kept_version or (weight is not of and weight.data_ptr() != of.data_ptr()):
             raise RuntimeError('Mx4Linear: the weight changed after keep(); call keep() again, or release()')
         return mx4.linear(x, mx4.Mx4Matrix(self.kept_codes, self.kept_scales, self.out_features, self.in_features, 1), self.bias)
 

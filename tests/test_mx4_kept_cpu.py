@@ -157,3 +157,32 @@ def test_a_computed_weight_is_not_kept():
             lin.keep()
         lin.release()
         assert torch.equal(lin(x), mx4.linear(x, lin.weight, lin.bias))
+
+
+def test_another_tensor_in_the_weights_place():
+    """functional_call swaps the layer's tensors for one call."""
+    from torch.func import functional_call
+    lin, x = _layer()
+    lin.weight = nn.Parameter(lin.weight.detach().clone())          # version 0, as that of a fresh tensor
+    lin.keep()
+    with torch.no_grad():
+        want = lin(x)
+        own = {'weight': lin.weight, 'bias': lin.bias}
+        assert torch.equal(functional_call(lin, own, x), want)
+        assert torch.equal(functional_call(lin, {k: v.detach() for k, v in own.items()}, x), want)
+        other = {'weight': torch.randn(8, 40), 'bias': lin.bias}
+        assert other['weight']._version == lin._kept_version
+        with pytest.raises(RuntimeError, match='keep'):
+            functional_call(lin, other, x)
+        assert torch.equal(lin(x), want)
+        FlatSGD(lin.parameters(), lr=0.5)                          # the same parameter at another address
+        assert torch.equal(lin(x), want)
+
+
+def test_kept_layers_can_be_pickled(tmp_path):
+    lin, x = _layer()
+    lin.keep()
+    torch.save(lin, tmp_path / 'lin.pt')
+    twin = torch.load(tmp_path / 'lin.pt', weights_only=False)
+    with torch.no_grad():
+        assert twin.kept_codes is None and torch.equal(twin(x), lin(x))
