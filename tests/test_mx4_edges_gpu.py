@@ -84,3 +84,32 @@ def test_products_past_the_range(mnk):
         want = torch.mm(a.double(), b.double().t().contiguous())
         room = torch.mm(a.double().abs(), b.double().abs().t().contiguous()) * (k * 2.0 ** -23) + k * 2.0 ** -126
         assert bool(((got - want).abs() <= room).all()), (ea, eb)
+
+
+@pytest.mark.parametrize('xt', TYPES)
+@pytest.mark.parametrize('wt', TYPES)
+def test_input_weight_and_bias_of_different_types(xt, wt):
+    """Quantised in one launch only where the types are the same; every output in its own input's type, equal to the product of its parts."""
+    from deepipr_amd import mx4
+    g = torch.Generator(device=DEV).manual_seed(4)
+    for m, n, k in ((3, 40, 70), (300, 200, 500)):
+        x = torch.randn(m, k, generator=g, device=DEV).to(xt).requires_grad_()
+        w = torch.randn(n, k, generator=g, device=DEV).to(wt).requires_grad_()
+        for bt in TYPES:
+            b = torch.randn(n, generator=g, device=DEV).to(bt).requires_grad_()
+            y = mx4.linear(x, w, b)
+            dy = torch.randn(m, n, generator=g, device=DEV).to(xt)
+            dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+            assert (y.dtype, dx.dtype, dw.dtype, db.dtype) == (xt, xt, wt, bt)
+            qx, qw, qy = mx4.quantize_both(x), mx4.quantize_both(w), mx4.quantize_both(dy)
+            assert torch.equal(y, mx4.matmul(qx[0], qw[0], b.detach(), xt))
+            assert torch.equal(dx, mx4.matmul(qy[0], qw[1], dtype=xt)) and torch.equal(dw, mx4.matmul(qy[1], qx[1], dtype=wt))
+            exact = dy.double().sum(0)
+            # sums of 32 and 64 rows in 32 bits, one rounding to 32 and one to the bias's type
+            assert bool(((db.double() - exact).abs() <= 66 * 2.0 ** -24 * dy.double().abs().sum(0) + exact.abs() * torch.finfo(bt).eps / 2 * 1.001).all())
+            with torch.no_grad():
+                assert torch.equal(mx4.linear(x, w, b), y) and torch.equal(mx4.linear(x, qw[0], b), y)
+            for keep in range(3):                                    # one gradient alone: other directions, other launches
+                args = [t if i == keep else t.detach() for i, t in enumerate((x, w, b))]
+                got, = torch.autograd.grad(mx4.linear(*args), args[keep], dy)
+                assert torch.equal(got, (dx, dw, db)[keep])
